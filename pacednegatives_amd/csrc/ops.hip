@@ -99,7 +99,10 @@ __global__ void __launch_bounds__(ROW_BLOCK) rmsnorm_bwd_kernel(const bf16* __re
                     xh[i][j] = bf2f(xv[j]) * rs;
                     g[i][j] = dyo * bf2f(wv8[j]) * out_scale;
                     dwacc[i][j] += dyo * xh[i][j] * out_scale;
-                    dot += g[i][j] * xh[i][j];
+                    {   // each product is rounded before it is added: the sum's bits then do not hang on the instructions chosen
+#pragma clang fp contract(off)
+                        dot += g[i][j] * xh[i][j];
+                    }
                 }
             }
         }
