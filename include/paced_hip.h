@@ -154,6 +154,44 @@ int paced_rmsnorm_bwd(const void* dy, const void* x, const void* w, const float*
                       void* dx, void* dx2, float* dw, int M, int d, float out_scale,
                       float drop_p, uint32_t drop_seed, float drop2_p, uint32_t drop2_seed, void* stream);
 
+/* ---- layer norm (mean and variance), with a residual sum in front of it ---------------------------
+ * No counterpart in the reference's T5; the norm of the encoders that dense retrieval and BERT-like rankers use.
+ * f32 = 0: x, res, xsum, w, b, y, dy, dres, dx are bf16; f32 = 1: fp32.  Rows of d elements, row strides in elements, any
+ * alignment of the element type (16-byte aligned rows with d * size % 16 == 0 are moved in 16-byte pieces); 1 <= d <=
+ * paced_layernorm_max_width() (8192); M = 0 does nothing.
+ * fwd: s = x, or s = round(x + res) written to xsum (res and xsum are both given or both NULL);
+ *      y = (s - mean) rstd w + b;  mean[M], rstd[M] fp32 saved (each may be NULL).
+ * bwd: x is what was normalised (xsum where there was a residual);  g = dy w,  xh = (x - mean) rstd,
+ *      dx = rstd (g - sum(g)/d - xh sum(g xh)/d) + dres (dres may be NULL);
+ *      dw[d] += sum dy xh and db[d] += sum dy (fp32, each may be NULL; added in a fixed order, no atomics), through a
+ *      workspace of paced_layernorm_workspace_bytes(M, d) bytes (not read or written when dw and db are both NULL).
+ * An output may be the very tensor of an input of its shape (y = x, xsum = res, dx = dy or dres); partial overlaps may not. */
+int paced_layernorm_max_width(void);
+int paced_layernorm_fwd(const void* x, int ldx, const void* res, int ldr, void* xsum, int lds, const void* w, const void* b,
+                        void* y, int ldy, float* mean, float* rstd, int M, int d, int f32, float eps, void* stream);
+size_t paced_layernorm_workspace_bytes(int M, int d);
+int paced_layernorm_bwd(const void* dy, int lddy, const void* x, int ldx, const void* w, const float* mean, const float* rstd,
+                        const void* dres, int ldr, void* dx, int lddx, float* dw, float* db, int M, int d, int f32,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- activation checkpoints in 8 bits -------------------------------------------------------------
+ * What a forward pass keeps for the weight gradients (the saved inputs of nn.Linear, HF:84-93, 304-367, whose products
+ * are reached from lceT5.py:155), at half the bytes.  A checkpoint of x [T, n] bf16 is q [T, n] (e4m3 codes, one byte, rows
+ * of n bytes) and scale [ceil(T/32), n] (exponent + 127 in a byte, one for 32 tokens of a feature): value = code *
+ * 2^(scale - 127).  The scale is the smallest power of two, 2^-117 at least, that brings the block's largest magnitude to
+ * 448 or less; codes round to nearest, ties to even (and stop at 240 under the scale 2^120).  A block with a NaN or an
+ * infinity reads back as NaN throughout (scale 255).  n % 16 == 0, 16-byte aligned operands, row strides % 8 == 0; T >= 0.
+ * dequantize gives the checkpoint's values, all of which are bf16 values.
+ * dweight: dw [M, N] fp32 (+)= dy^T x for the checkpoint's values x [T, N] and dy [T, M] bf16 (rows of lddy elements, or
+ * head-major as in paced_gemm_bf16_heads: lddy = 64 and dy_heads > 0; the rows up to the next multiple of 64 must then be
+ * finite); M % 8 == 0, N % 16 == 0, lddw % 4 == 0.  Products are exact, sums fp32 in a fixed order (no atomics).
+ * accumulate = 0: dw is written, 1: added to.  workspace: paced_act8_dweight_workspace_bytes(T, M, N, accumulate) bytes. */
+int paced_act8_quantize(const void* x, int ldx, void* q, void* scale, int T, int n, void* stream);
+int paced_act8_dequantize(const void* q, const void* scale, void* y, int ldy, int T, int n, void* stream);
+size_t paced_act8_dweight_workspace_bytes(int T, int M, int N, int accumulate);
+int paced_act8_dweight(const void* dy, int lddy, long long dy_heads, const void* q, const void* scale, float* dw, int lddw,
+                       int T, int M, int N, int accumulate, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- token embedding, HF:678,725 (gather + dropout) and its scatter-add gradient ------------ */
 int paced_embedding_fwd(const long long* ids, const void* table, void* out, int M, int d, int vocab,
                         float drop_p, uint32_t drop_seed, void* stream);

@@ -41,6 +41,14 @@ SIGNATURES = {
     "paced_gemm_tile_bits_bytes": (_ll, [_i, _i]),
     "paced_rmsnorm_fwd": (_i, [_vp, _vp, _vp, _vp, _i, _i, _f, _f, _f, _u32, _vp]),
     "paced_rmsnorm_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _f, _f, _u32, _f, _u32, _vp]),
+    "paced_layernorm_max_width": (_i, []),
+    "paced_layernorm_fwd": (_i, [_vp, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _f, _vp]),
+    "paced_layernorm_workspace_bytes": (_sz, [_i, _i]),
+    "paced_layernorm_bwd": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _vp, _sz, _vp]),
+    "paced_act8_quantize": (_i, [_vp, _i, _vp, _vp, _i, _i, _vp]),
+    "paced_act8_dequantize": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
+    "paced_act8_dweight_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "paced_act8_dweight": (_i, [_vp, _i, _ll, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
     "paced_embedding_fwd": (_i, [_vp, _vp, _vp, _i, _i, _i, _f, _u32, _vp]),
     "paced_embedding_bwd": (_i, [_vp, _vp, _vp, _i, _i, _i, _f, _u32, _vp]),
     "paced_dropout_apply": (_i, [_vp, _vp, _sz, _f, _u32, _vp]),

@@ -1,0 +1,388 @@
+// Layer norm, forward and backward, with an optional residual sum in front of it and the reduction of the weight's and the
+// bias's gradient:
+//   s = x (+ res, rounded to the tensors' type: it is what the backward pass reads)      xsum = s
+//   mean = sum(s) / d     rstd = 1 / sqrt(sum((s - mean)^2) / d + eps)     y = (s - mean) rstd w + b
+//   xh = (s - mean) rstd    g = dy w    dx = rstd (g - sum(g) / d - xh sum(g xh) / d) (+ dres)
+//   dw += sum over rows of dy xh        db += sum over rows of dy
+// Bound by memory: every stream is read or written once.  A TEAM of threads holds a whole row in registers, so the mean, the
+// squares about it and the output take one read of the row; statistics and sums are 32-bit.  Column sums stay in registers
+// over all rows that a team works on, are added over a workgroup's teams in LDS, and leave as one partial row per workgroup;
+// a second kernel adds those in a fixed order (no atomics: equal inputs give equal bits).
+#include "common.h"
+
+namespace {
+
+constexpr int LN_BLOCK = 256;
+constexpr int LN_MAX_D = 8192;
+
+// V elements of type T as they are loaded: 16 bytes where rows allow it, single elements otherwise
+template <class T, int V> struct Piece;
+template <> struct Piece<bf16, 8> {
+    u32x4 r;
+    __device__ __forceinline__ float get(int j) const { return __uint_as_float((j & 1) ? (r[j >> 1] & 0xffff0000u) : (r[j >> 1] << 16)); }
+    __device__ __forceinline__ void put(const float (&f)[8]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bf16x2 v = {f2bf(f[2 * j]), f2bf(f[2 * j + 1])};
+            r[j] = __builtin_bit_cast(uint32_t, v);
+        }
+    }
+    __device__ __forceinline__ void load(const bf16* p) { r = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)); }
+    __device__ __forceinline__ void load_kept(const bf16* p) { r = *reinterpret_cast<const u32x4*>(p); }
+    __device__ __forceinline__ void store(bf16* p) const { __builtin_nontemporal_store(r, reinterpret_cast<u32x4*>(p)); }
+    __device__ __forceinline__ void clear() { r = u32x4{0u, 0u, 0u, 0u}; }
+};
+template <> struct Piece<float, 4> {
+    f32x4 r;
+    __device__ __forceinline__ float get(int j) const { return r[j]; }
+    __device__ __forceinline__ void put(const float (&f)[4]) { r = f32x4{f[0], f[1], f[2], f[3]}; }
+    __device__ __forceinline__ void load(const float* p) { r = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p)); }
+    __device__ __forceinline__ void load_kept(const float* p) { r = *reinterpret_cast<const f32x4*>(p); }
+    __device__ __forceinline__ void store(float* p) const { __builtin_nontemporal_store(r, reinterpret_cast<f32x4*>(p)); }
+    __device__ __forceinline__ void clear() { r = f32x4{0.f, 0.f, 0.f, 0.f}; }
+};
+template <class T> struct Piece<T, 1> {
+    T r;
+    __device__ __forceinline__ float get(int) const { return (float)r; }
+    __device__ __forceinline__ void put(const float (&f)[1]) { r = (T)f[0]; }
+    __device__ __forceinline__ void load(const T* p) { r = *p; }
+    __device__ __forceinline__ void load_kept(const T* p) { r = *p; }
+    __device__ __forceinline__ void store(T* p) const { *p = r; }
+    __device__ __forceinline__ void clear() { r = (T)0.f; }
+};
+
+// sum over the TEAM threads of a row (16 or 64 lanes of a wave, or the whole workgroup through `sh`, two sets of four slots)
+template <int TEAM>
+__device__ __forceinline__ float team_sum(float v, float* sh) {
+#pragma unroll
+    for (int o = (TEAM < 64 ? TEAM : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if (TEAM > 64) {
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = sh[0] + sh[1] + sh[2] + sh[3];
+    }
+    return v;
+}
+
+template <class T> struct LnFwd {
+    const T *x, *res, *w, *b;
+    T *xsum, *y;
+    float *mean, *rstd;
+    int ldx, ldr, lds, ldy, M, d;
+    float eps;
+};
+
+template <class T, int V, int TEAM, int PER>
+__global__ void __launch_bounds__(LN_BLOCK) ln_fwd_kernel(LnFwd<T> a) {
+    constexpr int RPB = LN_BLOCK / TEAM;
+    __shared__ float sh[4][4];
+    const int l = threadIdx.x % TEAM, t = threadIdx.x / TEAM;
+    const float inv_d = 1.f / (float)a.d;
+    for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.M; row0 += (long long)gridDim.x * RPB) {
+        const bool ok = row0 + t < a.M;
+        const size_t row = ok ? row0 + t : a.M - 1;         // a team past the end repeats the last row and stores nothing
+        Piece<T, V> p[PER], q[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = (l + i * TEAM) * V;
+            p[i].clear();
+            q[i].clear();
+            if (c < a.d) {
+                p[i].load(a.x + row * a.ldx + c);
+                if (a.res) q[i].load(a.res + row * a.ldr + c);
+            }
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = (l + i * TEAM) * V;
+            if (a.res) {
+                float f[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) f[j] = p[i].get(j) + q[i].get(j);
+                p[i].put(f);
+                if (ok && c < a.d) p[i].store(a.xsum + row * a.lds + c);
+            }
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum += p[i].get(j);
+        }
+        const float mean = team_sum<TEAM>(sum, sh[0]) * inv_d;
+        float sq = 0.f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if ((l + i * TEAM) * V < a.d) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) { const float f = p[i].get(j) - mean; sq += f * f; }
+            }
+        const float rstd = 1.f / sqrtf(team_sum<TEAM>(sq, sh[1]) * inv_d + a.eps);
+        if (l == 0 && ok) {
+            if (a.mean) a.mean[row] = mean;
+            if (a.rstd) a.rstd[row] = rstd;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = (l + i * TEAM) * V;
+            if (ok && c < a.d) {
+                Piece<T, V> w, b, o;
+                w.load_kept(a.w + c);
+                b.load_kept(a.b + c);
+                float f[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) f[j] = (p[i].get(j) - mean) * rstd * w.get(j) + b.get(j);
+                o.put(f);
+                o.store(a.y + row * a.ldy + c);
+            }
+        }
+        if (TEAM > 64) __syncthreads();                     // the next row's sums reuse `sh`
+    }
+}
+
+template <class T> struct LnBwd {
+    const T *dy, *x, *w, *dres;
+    const float *mean, *rstd;
+    T* dx;
+    float* part;                    // [gridDim.x][2][d]: sums of dy xh, then of dy; NULL: no column sums
+    int lddy, ldx, ldr, lddx, M, d;
+};
+
+// two waves per SIMD: a thread carries its pieces of three rows and two column sums in up to 256 registers
+template <class T, int V, int TEAM, int PER>
+__global__ void __launch_bounds__(LN_BLOCK) __attribute__((amdgpu_waves_per_eu(2)))
+ln_bwd_kernel(LnBwd<T> a) {
+    constexpr int RPB = LN_BLOCK / TEAM;
+    __shared__ float sh[4][4];
+    extern __shared__ float cols[];                         // [4 waves][d]
+    const int l = threadIdx.x % TEAM, t = threadIdx.x / TEAM;
+    const float inv_d = 1.f / (float)a.d;
+    float sw[PER][V], sb[PER][V];
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) sw[i][j] = sb[i][j] = 0.f;
+    for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.M; row0 += (long long)gridDim.x * RPB) {
+        const bool ok = row0 + t < a.M;
+        const size_t row = ok ? row0 + t : a.M - 1;
+        Piece<T, V> p[PER], q[PER], r[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = (l + i * TEAM) * V;
+            p[i].clear();
+            q[i].clear();
+            r[i].clear();
+            if (c < a.d) {
+                p[i].load(a.dy + row * a.lddy + c);
+                q[i].load(a.x + row * a.ldx + c);
+                if (a.dres) r[i].load(a.dres + row * a.ldr + c);
+            }
+        }
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float sg = 0.f, sgx = 0.f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = (l + i * TEAM) * V;
+            if (c < a.d) {
+                Piece<T, V> w;
+                w.load_kept(a.w + c);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float dy = p[i].get(j), xh = (q[i].get(j) - mean) * rstd, g = dy * w.get(j);
+                    sg += g;
+                    sgx += g * xh;
+                    if (ok) { sw[i][j] += dy * xh; sb[i][j] += dy; }
+                }
+            }
+        }
+        sg = team_sum<TEAM>(sg, sh[0]) * inv_d;
+        sgx = team_sum<TEAM>(sgx, sh[1]) * inv_d;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = (l + i * TEAM) * V;
+            if (ok && c < a.d) {
+                Piece<T, V> w, o;
+                w.load_kept(a.w + c);
+                float f[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float xh = (q[i].get(j) - mean) * rstd;
+                    f[j] = rstd * (p[i].get(j) * w.get(j) - sg - xh * sgx) + r[i].get(j);
+                }
+                o.put(f);
+                o.store(a.dx + row * a.lddx + c);
+            }
+        }
+        if (TEAM > 64) __syncthreads();
+    }
+    if (!a.part) return;
+    float* out = a.part + (size_t)blockIdx.x * 2 * a.d;
+    if (TEAM >= LN_BLOCK) {                                 // one team: its registers are the workgroup's sums
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int c = (l + i * TEAM) * V + j;
+                if (c < a.d) { out[c] = sw[i][j]; out[a.d + c] = sb[i][j]; }
+            }
+        return;
+    }
+    // teams of one wave first (lanes that hold the same columns), then the four waves through LDS, in a fixed order; the two
+    // sums one after the other in the same LDS
+    const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                float u = k ? sb[i][j] : sw[i][j];
+#pragma unroll
+                for (int o = TEAM; o < 64; o <<= 1) u += __shfl_xor(u, o, 64);
+                const int c = (l + i * TEAM) * V + j;
+                if (lane < TEAM && c < a.d) cols[wv * a.d + c] = u;
+            }
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.d; c += LN_BLOCK)
+            out[k * a.d + c] = (cols[c] + cols[a.d + c]) + (cols[2 * a.d + c] + cols[3 * a.d + c]);
+        __syncthreads();
+    }
+}
+
+// dw[c] += sum over g of part[g][0][c], db[c] += ... [1][c]: 32 columns of a workgroup, 8 threads over the partial rows of each
+__global__ void __launch_bounds__(LN_BLOCK) ln_cols_kernel(const float* __restrict__ part, int G, int d, float* dw, float* db) {
+    __shared__ float sh[8][33];
+    const int l = threadIdx.x & 31, k = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + l;
+    float s = 0.f;
+    if (c < 2 * d)
+        for (int g = k; g < G; g += 8) s += part[(size_t)g * 2 * d + c];
+    sh[k][l] = s;
+    __syncthreads();
+    if (k == 0 && c < 2 * d) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) s += sh[i][l];
+        if (c < d) { if (dw) dw[c] += s; }
+        else if (db) db[c - d] += s;
+    }
+}
+
+// workgroups of the backward kernel: two to a compute unit, none without a row
+int ln_bwd_grid(int M) {
+    const int most = 2 * paced_cu_count();
+    return M < most ? M : most;
+}
+
+template <class T, int V, int TEAM, int PER>
+int ln_fwd_go(const LnFwd<T>& a, hipStream_t s) {
+    const long long blocks = ((long long)a.M + LN_BLOCK / TEAM - 1) / (LN_BLOCK / TEAM);
+    const int grid = (int)(blocks < 8192 ? blocks : 8192);
+    hipLaunchKernelGGL((ln_fwd_kernel<T, V, TEAM, PER>), dim3(grid), dim3(LN_BLOCK), 0, s, a);
+    PACED_CHECK_LAUNCH();
+    return PACED_OK;
+}
+template <class T, int V, int TEAM, int PER>
+int ln_bwd_go(const LnBwd<T>& a, int grid, hipStream_t s) {
+    const int smem = TEAM < LN_BLOCK && a.part ? 4 * a.d * 4 : 0;              // 32 KiB at most: these teams take d <= 2048
+    hipLaunchKernelGGL((ln_bwd_kernel<T, V, TEAM, PER>), dim3(grid), dim3(LN_BLOCK), smem, s, a);
+    PACED_CHECK_LAUNCH();
+    return PACED_OK;
+}
+
+// the narrowest team whose registers hold a row of d elements
+#define LN_TEAM(T, V, TEAM, PER, ...) if (d <= V * TEAM * PER) return GO(T, V, TEAM, PER);
+#define LN_PICK_BF16 LN_TEAM(bf16, 8, 16, 1) LN_TEAM(bf16, 8, 16, 2) LN_TEAM(bf16, 8, 16, 4) LN_TEAM(bf16, 8, 16, 6) \
+                     LN_TEAM(bf16, 8, 64, 2) LN_TEAM(bf16, 8, 64, 4) LN_TEAM(bf16, 8, 256, 2) LN_TEAM(bf16, 8, 256, 4)
+#define LN_PICK_F32 LN_TEAM(float, 4, 16, 2) LN_TEAM(float, 4, 16, 8) LN_TEAM(float, 4, 64, 3) LN_TEAM(float, 4, 64, 4) LN_TEAM(float, 4, 64, 8) \
+                    LN_TEAM(float, 4, 256, 4) LN_TEAM(float, 4, 256, 8)
+#define LN_PICK_ONE(T) LN_TEAM(T, 1, 16, 4) LN_TEAM(T, 1, 64, 4) LN_TEAM(T, 1, 64, 16) LN_TEAM(T, 1, 256, 8) LN_TEAM(T, 1, 256, 32)
+
+template <class T> int ln_fwd_pick(const LnFwd<T>& a, bool vec, hipStream_t s);
+template <class T> int ln_bwd_pick(const LnBwd<T>& a, bool vec, int grid, hipStream_t s);
+#define GO(T, V, TEAM, PER) ln_fwd_go<T, V, TEAM, PER>(a, s)
+template <> int ln_fwd_pick<bf16>(const LnFwd<bf16>& a, bool vec, hipStream_t s) {
+    const int d = a.d;
+    if (vec) { LN_PICK_BF16 }
+    LN_PICK_ONE(bf16)
+    return PACED_ERR_ARG;
+}
+template <> int ln_fwd_pick<float>(const LnFwd<float>& a, bool vec, hipStream_t s) {
+    const int d = a.d;
+    if (vec) { LN_PICK_F32 }
+    LN_PICK_ONE(float)
+    return PACED_ERR_ARG;
+}
+#undef GO
+#define GO(T, V, TEAM, PER) ln_bwd_go<T, V, TEAM, PER>(a, grid, s)
+template <> int ln_bwd_pick<bf16>(const LnBwd<bf16>& a, bool vec, int grid, hipStream_t s) {
+    const int d = a.d;
+    if (vec) { LN_PICK_BF16 }
+    LN_PICK_ONE(bf16)
+    return PACED_ERR_ARG;
+}
+template <> int ln_bwd_pick<float>(const LnBwd<float>& a, bool vec, int grid, hipStream_t s) {
+    const int d = a.d;
+    if (vec) { LN_PICK_F32 }
+    LN_PICK_ONE(float)
+    return PACED_ERR_ARG;
+}
+#undef GO
+
+// whether rows at p, ld elements apart, can be moved in 16-byte pieces
+bool vec_ok(const void* p, int ld, int size) { return !p || (((uintptr_t)p & 15) == 0 && (long long)ld * size % 16 == 0); }
+
+template <class T>
+int ln_fwd(const void* x, int ldx, const void* res, int ldr, void* xsum, int lds, const void* w, const void* b, void* y, int ldy,
+           float* mean, float* rstd, int M, int d, float eps, hipStream_t s) {
+    const int size = (int)sizeof(T);
+    const bool vec = (long long)d * size % 16 == 0 && vec_ok(x, ldx, size) && vec_ok(res, ldr, size) && vec_ok(xsum, lds, size) &&
+                     vec_ok(y, ldy, size) && vec_ok(w, 0, size) && vec_ok(b, 0, size);
+    return ln_fwd_pick<T>(LnFwd<T>{(const T*)x, (const T*)res, (const T*)w, (const T*)b, (T*)xsum, (T*)y, mean, rstd, ldx, ldr, lds, ldy, M, d, eps}, vec, s);
+}
+template <class T>
+int ln_bwd(const void* dy, int lddy, const void* x, int ldx, const void* w, const float* mean, const float* rstd, const void* dres, int ldr,
+           void* dx, int lddx, float* part, int grid, int M, int d, hipStream_t s) {
+    const int size = (int)sizeof(T);
+    const bool vec = (long long)d * size % 16 == 0 && vec_ok(dy, lddy, size) && vec_ok(x, ldx, size) && vec_ok(dres, ldr, size) &&
+                     vec_ok(dx, lddx, size) && vec_ok(w, 0, size);
+    return ln_bwd_pick<T>(LnBwd<T>{(const T*)dy, (const T*)x, (const T*)w, (const T*)dres, mean, rstd, (T*)dx, part, lddy, ldx, ldr, lddx, M, d}, vec, grid, s);
+}
+
+}  // namespace
+
+extern "C" int paced_layernorm_max_width(void) { return LN_MAX_D; }
+
+extern "C" int paced_layernorm_fwd(const void* x, int ldx, const void* res, int ldr, void* xsum, int lds, const void* w, const void* b,
+                                   void* y, int ldy, float* mean, float* rstd, int M, int d, int f32, float eps, void* stream) {
+    PACED_CHECK_ARG(M >= 0 && d > 0 && d <= LN_MAX_D, "paced_layernorm_fwd: need M >= 0 and d in [1, %d] (M=%d d=%d)", LN_MAX_D, M, d);
+    if (M == 0) return PACED_OK;
+    PACED_CHECK_ARG(x && w && b && y, "paced_layernorm_fwd: null operand");
+    PACED_CHECK_ARG((res == nullptr) == (xsum == nullptr), "paced_layernorm_fwd: res and xsum go together");
+    PACED_CHECK_ARG(ldx >= d && ldy >= d && (!res || (ldr >= d && lds >= d)), "paced_layernorm_fwd: row strides must be at least d");
+    PACED_CHECK_ARG(eps >= 0.f, "paced_layernorm_fwd: eps must not be negative");
+    return f32 ? ln_fwd<float>(x, ldx, res, ldr, xsum, lds, w, b, y, ldy, mean, rstd, M, d, eps, (hipStream_t)stream)
+               : ln_fwd<bf16>(x, ldx, res, ldr, xsum, lds, w, b, y, ldy, mean, rstd, M, d, eps, (hipStream_t)stream);
+}
+
+extern "C" size_t paced_layernorm_workspace_bytes(int M, int d) {
+    if (M <= 0 || d <= 0) return 0;
+    return (size_t)ln_bwd_grid(M) * 2 * (size_t)d * 4;
+}
+
+extern "C" int paced_layernorm_bwd(const void* dy, int lddy, const void* x, int ldx, const void* w, const float* mean, const float* rstd,
+                                   const void* dres, int ldr, void* dx, int lddx, float* dw, float* db, int M, int d, int f32,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+    PACED_CHECK_ARG(M >= 0 && d > 0 && d <= LN_MAX_D, "paced_layernorm_bwd: need M >= 0 and d in [1, %d] (M=%d d=%d)", LN_MAX_D, M, d);
+    if (M == 0) return PACED_OK;
+    PACED_CHECK_ARG(dy && x && w && mean && rstd && dx, "paced_layernorm_bwd: null operand");
+    PACED_CHECK_ARG(lddy >= d && ldx >= d && lddx >= d && (!dres || ldr >= d), "paced_layernorm_bwd: row strides must be at least d");
+    const bool sums = dw || db;
+    const size_t need = sums ? paced_layernorm_workspace_bytes(M, d) : 0;
+    PACED_CHECK_ARG(!sums || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 3) == 0),
+                    "paced_layernorm_bwd: the column sums need a workspace of %zu bytes, got %zu", need, workspace_bytes);
+    const int grid = ln_bwd_grid(M);
+    float* part = sums ? (float*)workspace : nullptr;
+    const int rc = f32 ? ln_bwd<float>(dy, lddy, x, ldx, w, mean, rstd, dres, ldr, dx, lddx, part, grid, M, d, (hipStream_t)stream)
+                       : ln_bwd<bf16>(dy, lddy, x, ldx, w, mean, rstd, dres, ldr, dx, lddx, part, grid, M, d, (hipStream_t)stream);
+    if (rc != PACED_OK || !sums) return rc;
+    hipLaunchKernelGGL(ln_cols_kernel, dim3((2 * d + 31) / 32), dim3(LN_BLOCK), 0, (hipStream_t)stream, part, grid, d, dw, db);
+    PACED_CHECK_LAUNCH();
+    return PACED_OK;
+}

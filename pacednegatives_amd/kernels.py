@@ -6,6 +6,7 @@ not match what its grid assumes.
 """
 from __future__ import annotations
 
+import contextlib
 import os
 
 import torch
@@ -42,6 +43,60 @@ def _rows2d(t, name):
     if t.dim() != 2 or t.stride(1) != 1:
         raise ValueError(f"{name} must be 2-D with unit inner stride, got shape {tuple(t.shape)} strides {t.stride()}")
     return t.stride(0)
+
+
+def _one_device(**tensors):
+    """The device that all given tensors (None: absent) live on, as a context for the launch: the current device, or a
+    switch to theirs.  Work then goes to that device's current stream."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a device tensor")
+        if dev is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the tensors before it on {dev}")
+        dev = t.device
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _rows_of(t, shape, dtype, name):
+    """Row stride of a [rows, d] operand of the given shape and type (rows of unit stride; a single row may have any)."""
+    if t is None:
+        return 0
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} must have unit inner stride, got strides {t.stride()}")
+    if shape[0] <= 1:
+        return shape[1]
+    if not shape[1] <= t.stride(0) < 2 ** 31:
+        raise ValueError(f"{name}: rows overlap or lie too far apart (strides {t.stride()})")
+    return t.stride(0)
+
+
+def _flat(t, n, dtype, name):
+    """A contiguous vector of n elements."""
+    if t is None:
+        return
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must hold {n} contiguous elements, got {tuple(t.shape)} with strides {t.stride()}")
+
+
+def _workspace(workspace, need, device):
+    """The caller's workspace if it is large enough, else a new one (freed to torch's allocator when the call returns: the
+    stream orders its next use)."""
+    if need == 0:
+        return None
+    if workspace is None:
+        return torch.empty(need, dtype=U8, device=device)
+    if workspace.dtype != U8 or not workspace.is_contiguous() or workspace.device != device:
+        raise ValueError(f"workspace must be a contiguous uint8 tensor on {device}")
+    return workspace if workspace.numel() >= need else torch.empty(need, dtype=U8, device=device)
 
 
 def _operand(t, name):
@@ -183,6 +238,107 @@ def rmsnorm_bwd(dy, x, w, rstd, dx, *, dres=None, dx2=None, dw=None, out_scale=1
     _lib.check(lib.paced_rmsnorm_bwd(_p(dy), _p(x), _p(w), _p(rstd), _p(dres), _p(dx), _p(dx2), _p(dw), M, d, out_scale,
                                      drop_p, drop_seed, drop2_p, drop2_seed, _stream()), "paced_rmsnorm_bwd")
     return dx
+
+
+def layernorm_fwd(x, w, b, y, mean=None, rstd=None, *, eps=1e-5, res=None, xsum=None):
+    """y = layer norm of x, or of x + res (written to ``xsum`` in the tensors' type: the backward pass's ``x``), weighted by w
+    and b; bf16 or fp32 [M, d] rows.  ``mean`` and ``rstd`` (fp32 [M]) are what ``layernorm_bwd`` needs."""
+    lib = _lib.load()
+    with _one_device(x=x, w=w, b=b, y=y, mean=mean, rstd=rstd, res=res, xsum=xsum):
+        if x.dim() != 2 or x.dtype not in (BF16, F32):
+            raise ValueError(f"x must be a bf16 or fp32 matrix, got {x.dtype} {tuple(x.shape)}")
+        if (res is None) != (xsum is None):
+            raise ValueError("res and xsum go together")
+        M, d = x.shape
+        ldx, ldy = _rows_of(x, (M, d), x.dtype, "x"), _rows_of(y, (M, d), x.dtype, "y")
+        ldr, lds = _rows_of(res, (M, d), x.dtype, "res"), _rows_of(xsum, (M, d), x.dtype, "xsum")
+        _flat(w, d, x.dtype, "w"); _flat(b, d, x.dtype, "b"); _flat(mean, M, F32, "mean"); _flat(rstd, M, F32, "rstd")
+        _lib.check(lib.paced_layernorm_fwd(_p(x), ldx, _p(res), ldr, _p(xsum), lds, _p(w), _p(b), _p(y), ldy, _p(mean), _p(rstd), M, d,
+                                           int(x.dtype == F32), eps, _stream()), "paced_layernorm_fwd")
+    return y
+
+
+def layernorm_bwd(dy, x, w, mean, rstd, dx, *, dres=None, dw=None, db=None, workspace=None):
+    """Backward of ``layernorm_fwd``; x is what was normalised.  dx = gradient through the norm (+ ``dres``); ``dw`` and ``db``
+    (fp32 [d]) are added to, in a fixed order."""
+    lib = _lib.load()
+    with _one_device(dy=dy, x=x, w=w, mean=mean, rstd=rstd, dx=dx, dres=dres, dw=dw, db=db):
+        if x.dim() != 2 or x.dtype not in (BF16, F32):
+            raise ValueError(f"x must be a bf16 or fp32 matrix, got {x.dtype} {tuple(x.shape)}")
+        M, d = x.shape
+        lddy, ldx, lddx = _rows_of(dy, (M, d), x.dtype, "dy"), _rows_of(x, (M, d), x.dtype, "x"), _rows_of(dx, (M, d), x.dtype, "dx")
+        ldr = _rows_of(dres, (M, d), x.dtype, "dres")
+        _flat(w, d, x.dtype, "w"); _flat(mean, M, F32, "mean"); _flat(rstd, M, F32, "rstd"); _flat(dw, d, F32, "dw"); _flat(db, d, F32, "db")
+        need = lib.paced_layernorm_workspace_bytes(M, d) if dw is not None or db is not None else 0
+        ws = _workspace(workspace, need, x.device)
+        _lib.check(lib.paced_layernorm_bwd(_p(dy), lddy, _p(x), ldx, _p(w), _p(mean), _p(rstd), _p(dres), ldr, _p(dx), lddx, _p(dw), _p(db),
+                                           M, d, int(x.dtype == F32), _p(ws), need, _stream()), "paced_layernorm_bwd")
+    return dx
+
+
+def act8_quantize(x, q=None, scale=None):
+    """8-bit checkpoint of x (bf16 [T, n], n % 16 == 0) for the backward pass: (q, scale) = e4m3 codes uint8 [T, n] and one
+    power of two for 32 tokens of a feature, uint8 [ceil(T/32), n] (see include/paced_hip.h)."""
+    lib = _lib.load()
+    if x.dim() != 2 or x.shape[1] % 16 or x.shape[1] == 0:
+        raise ValueError(f"x must be [T, n] with n a multiple of 16, got {tuple(x.shape)}")
+    T, n = x.shape
+    blocks = (T + 31) // 32
+    if q is None:
+        q = torch.empty(T, n, dtype=U8, device=x.device)
+    if scale is None:
+        scale = torch.empty(blocks, n, dtype=U8, device=x.device)
+    with _one_device(x=x, q=q, scale=scale):
+        ldx = _rows_of(x, (T, n), BF16, "x")
+        _flat(q, T * n, U8, "q"); _flat(scale, blocks * n, U8, "scale")
+        _lib.check(lib.paced_act8_quantize(_p(x), ldx, _p(q), _p(scale), T, n, _stream()), "paced_act8_quantize")
+    return q, scale
+
+
+def _checkpoint(q, scale):
+    if q.dim() != 2 or q.shape[1] % 16 or q.shape[1] == 0:
+        raise ValueError(f"q must be [T, n] with n a multiple of 16, got {tuple(q.shape)}")
+    T, n = q.shape
+    if tuple(scale.shape) != ((T + 31) // 32, n):
+        raise ValueError(f"scale must be [ceil(T/32), n] = {((T + 31) // 32, n)}, got {tuple(scale.shape)}")
+    _flat(q, T * n, U8, "q"); _flat(scale, scale.numel(), U8, "scale")
+    return T, n
+
+
+def act8_dequantize(q, scale, y):
+    """The values of a checkpoint (bf16 [T, n]); nothing is rounded."""
+    lib = _lib.load()
+    with _one_device(q=q, scale=scale, y=y):
+        T, n = _checkpoint(q, scale)
+        _lib.check(lib.paced_act8_dequantize(_p(q), _p(scale), _p(y), _rows_of(y, (T, n), BF16, "y"), T, n, _stream()), "paced_act8_dequantize")
+    return y
+
+
+def act8_dweight(dy, q, scale, dw, *, accumulate=True, workspace=None):
+    """dw (fp32 [out, in]) += dy^T x for the checkpoint x = (q, scale) of [T, in] and dy bf16 [T, out] (or head-major, see
+    _operand); ``accumulate=False`` writes dw."""
+    lib = _lib.load()
+    with _one_device(dy=dy, q=q, scale=scale, dw=dw):
+        T, N = _checkpoint(q, scale)
+        if dy.dtype != BF16:
+            raise ValueError(f"dy must be {BF16}, got {dy.dtype}")
+        if dy.dim() == 3:
+            rows, M, lddy, heads = _operand(dy, "dy")
+            if rows != T:
+                raise ValueError(f"dy has {rows} rows, the checkpoint {T}")
+            if dy.shape[0] == 1:
+                heads = T * 64                               # a single head may have any stride
+        else:
+            if dy.dim() != 2:
+                raise ValueError(f"dy must be [T, out] or head-major, got {tuple(dy.shape)}")
+            M, heads = dy.shape[1], 0
+            lddy = _rows_of(dy, (T, M), BF16, "dy")
+        lddw = _rows_of(dw, (M, N), F32, "dw")
+        need = lib.paced_act8_dweight_workspace_bytes(T, M, N, int(bool(accumulate)))
+        ws = _workspace(workspace, need, dy.device)
+        _lib.check(lib.paced_act8_dweight(_p(dy), lddy, heads, _p(q), _p(scale), _p(dw), lddw, T, M, N, int(bool(accumulate)), _p(ws), need,
+                                          _stream()), "paced_act8_dweight")
+    return dw
 
 
 def embedding_fwd(ids, table, out, *, drop_p=0.0, drop_seed=0):
