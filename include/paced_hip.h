@@ -264,6 +264,24 @@ int paced_cross2_bwd(const void* enc, int ld, const void* qk, const void* dz, co
  * dlogits (bf16, may be NULL) = (softmax - onehot) * gscale. */
 int paced_cross_entropy(const float* logits, const long long* labels, float* loss, void* dlogits,
                         int rows, int V, int ldl, long long ignore_index, float gscale, void* stream);
+/* The same loss for logits z = scale * h w^T that are never stored (the LM head HF:1047 and nn.CrossEntropyLoss,
+ * lceT5.py:110,117-118, in one; or queries against a batch of documents), and its gradients.
+ * h [R, d], w [V, d] bf16, d % 64 == 0, 16-byte aligned rows, row strides % 8 == 0; labels int64 [R]; a label that is
+ * ignore_index or outside [0, V) makes its row an ignored one (loss 0, no gradient; its lse is still written).  R = 0 is allowed.
+ * fwd: loss[R], lse[R] fp32 (lse may be NULL); log-sum-exp in fp32, the label's term apart from the others', so that small
+ *      losses keep their relative precision.
+ * bwd: gloss[r] = d objective / d loss[r] (fp32); dh [R, d] bf16 is written, dw [V, d] is written in bf16 (dw_f32 = 0) or added
+ *      to in fp32 (dw_f32 = 1); each may be NULL.  The logits' gradient gloss (softmax - onehot) scale is rounded to bf16
+ *      between the products, as paced_cross_entropy's dlogits are; sums are fp32 in a fixed order, without atomics.  An
+ *      ignored row's h must be finite where dw is wanted (0 times it is added).
+ * workspace: ..._workspace_bytes() bytes (256 MiB + about 64 MiB at most, whatever V is, up to R of half a million). */
+size_t paced_linear_ce_fwd_workspace_bytes(int R, int V);
+int paced_linear_ce_fwd(const void* h, int ldh, const void* w, int ldw, const long long* labels, float* loss, float* lse,
+                        int R, int V, int d, long long ignore_index, float scale, void* workspace, size_t workspace_bytes, void* stream);
+size_t paced_linear_ce_bwd_workspace_bytes(int R, int V, int d);
+int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ldw, const long long* labels, const float* lse, const float* gloss,
+                        void* dh, int lddh, void* dw, int lddw, int dw_f32, int R, int V, int d, long long ignore_index, float scale,
+                        void* workspace, size_t workspace_bytes, void* stream);
 /* lceT5.py:119-121 after the caller's view at :134,151: ce[r] = pce[r] + sum|mean nce[r*n..(r+1)*n) */
 int paced_lce_group(const float* pce, const float* nce, float* ce, int R, int n, int use_mean, void* stream);
 /* LCEWeights.forward, lceT5.py:91-99, vectorised, plus the reductions training_step needs (:138-147):

@@ -65,6 +65,10 @@ SIGNATURES = {
     "paced_cross2_bwd": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _i, _vp, _ll, _i, _i, _i, _i, _f, _u32, _vp]),
     "paced_cross_attn_bwd": (_i, [_vp, _i, _vp, _i, _i, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _f, _u32, _vp]),
     "paced_cross_entropy": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _ll, _f, _vp]),
+    "paced_linear_ce_fwd_workspace_bytes": (_sz, [_i, _i]),
+    "paced_linear_ce_fwd": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _ll, _f, _vp, _sz, _vp]),
+    "paced_linear_ce_bwd_workspace_bytes": (_sz, [_i, _i, _i]),
+    "paced_linear_ce_bwd": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _ll, _f, _vp, _sz, _vp]),
     "paced_lce_group": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
     "paced_lce_weights": (_i, [_vp, _vp, _vp, _vp, _i, _vp]),
     "paced_eta_weights": (_i, [_vp, _vp, _f, _i, _vp, _vp, _i, _vp]),

@@ -339,7 +339,8 @@ extern "C" int paced_act8_dweight(const void* dy, int lddy, long long dy_heads, 
     else PACED_CHECK_ARG(T == 0 || (lddy >= M && lddy % 8 == 0), "paced_act8_dweight: dy's row stride must be at least M and a multiple of 8 (lddy=%d)", lddy);
     hipStream_t s = (hipStream_t)stream;
     if (T == 0) {                                   // an empty sum
-        if (!accumulate) hipLaunchKernelGGL(slab_sum_kernel, dim3(flat_blocks((long long)M * (N >> 2))), dim3(256), 0, s, nullptr, 0, 0LL, dw, lddw, M, N, 0);
+        if (accumulate) return PACED_OK;
+        hipLaunchKernelGGL(slab_sum_kernel, dim3(flat_blocks((long long)M * (N >> 2))), dim3(256), 0, s, nullptr, 0, 0LL, dw, lddw, M, N, 0);
         PACED_CHECK_LAUNCH();
         return PACED_OK;
     }

@@ -12,7 +12,12 @@ enum Epi : int {
     EPI_MASK_BITS = 6,   // C = acc * (bit (m, n) of the byte matrix aux ? mask_scale : 0)
     EPI_COUNT,           // ---- epilogues below are internal to the pool scorer (mining.hip)
     EPI_TOPK_DENSE = 7,  // cand[n][m] = key(acc, row_base + m)
-    EPI_TOPK_FILTER = 8  // if acc >= thr[n]: cand[n][cnt[n]++] = key(acc, row_base + m)
+    EPI_TOPK_FILTER = 8, // if acc >= thr[n]: cand[n][cnt[n]++] = key(acc, row_base + m)
+    // ---- internal to the linear-head cross entropy (linear_ce.hip); rows m are tokens, columns n vocabulary entries
+    EPI_CE_STATS = 9,    // part[n / W][m] = (max, sum of 2^(z - max)) of z = acc * alpha * log2 e over W columns but the label's
+                         // (W = 64; 32 for the 64x64 tiles); target[m] = the label's acc * alpha
+    EPI_CE_GRAD = 10,    // C(bf16) = g[m] (2^(z - lse[m] log2 e) - [n is m's label]); columns N .. next multiple of 64 are zeros
+    EPI_SLAB_F32 = 11    // C(f32) + split * strideC elements (+)= acc * alpha: one owner per element, no atomics
 };
 
 struct GemmParams {
@@ -40,6 +45,15 @@ struct GemmParams {
     const float* tk_thr;
     int tk_cap;
     unsigned int tk_row_base;
+    // linear-head cross entropy only
+    const long long* ce_labels;   // [M]; a label counts when it is not ce_ignore and lies in [0, ce_vocab)
+    const float* ce_lse;          // [M]
+    const float* ce_g;            // [M]
+    f32x2* ce_part;
+    float* ce_target;
+    long long ce_ignore;
+    int ce_vocab, ce_first;       // vocabulary size, entry of column 0
+    int accumulate;               // EPI_SLAB_F32: add to what is there
 };
 
 // Order-preserving 64-bit key: larger key <=> (higher score, then lower pool row).
@@ -57,6 +71,7 @@ __host__ __device__ __forceinline__ float topk_key_score(unsigned long long key)
 __host__ __device__ __forceinline__ unsigned int topk_key_row(unsigned long long key) { return ~(unsigned int)key; }
 
 // Launches the tiled kernel for (trans_a, trans_b, epilogue); arguments are already validated.
+extern "C" int paced_gemm_last_kernel(void);
 int paced_gemm_launch(const GemmParams& p, bool trans_a, bool trans_b, int epilogue, int splits, hipStream_t stream);
 
 

@@ -23,8 +23,76 @@ namespace {
 // output matrix of batch member b (fp32 for the fp32 / atomic epilogues, bf16 otherwise)
 template <int EPI>
 __device__ __forceinline__ void* batch_c(const GemmParams& p, int b) {
-    constexpr int ES = (EPI == EPI_F32 || EPI == EPI_ATOMIC_F32) ? 4 : 2;
+    constexpr int ES = (EPI == EPI_F32 || EPI == EPI_ATOMIC_F32 || EPI == EPI_SLAB_F32) ? 4 : 2;
     return reinterpret_cast<char*>(p.C) + (long long)b * p.strideC * ES;
+}
+
+// ---- linear-head cross entropy -----------------------------------------------------------------------------------
+// Rows of a wave's 16-row block i are on its lanes' low four bits.  What a row needs (label, log-sum-exp, weight) is loaded
+// by inline assembly that waits for itself: a load the compiler can see would drain the K loop's LDS-DMA (epilogue_rows_impl).
+constexpr float CE_LOG2E = 1.4426950408889634f;
+
+template <int MI, class T>
+__device__ __forceinline__ void ce_load_rows(const T* const (&src)[MI], T (&v)[MI]) {
+    static_assert(MI == 2 || MI == 4 || MI == 8, "row blocks of a wave");
+    if constexpr (sizeof(T) == 8) {
+        if constexpr (MI == 8)
+            asm volatile("global_load_dwordx2 %0, %8, off\n\tglobal_load_dwordx2 %1, %9, off\n\tglobal_load_dwordx2 %2, %10, off\n\tglobal_load_dwordx2 %3, %11, off\n\t"
+                         "global_load_dwordx2 %4, %12, off\n\tglobal_load_dwordx2 %5, %13, off\n\tglobal_load_dwordx2 %6, %14, off\n\tglobal_load_dwordx2 %7, %15, off\n\t"
+                         "s_waitcnt vmcnt(0) ; hidden-load wait"
+                         : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+                         : "v"(src[0]), "v"(src[1]), "v"(src[2]), "v"(src[3]), "v"(src[4]), "v"(src[5]), "v"(src[6]), "v"(src[7]) : "memory");
+        else if constexpr (MI == 4)
+            asm volatile("global_load_dwordx2 %0, %4, off\n\tglobal_load_dwordx2 %1, %5, off\n\tglobal_load_dwordx2 %2, %6, off\n\tglobal_load_dwordx2 %3, %7, off\n\t"
+                         "s_waitcnt vmcnt(0) ; hidden-load wait"
+                         : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]) : "v"(src[0]), "v"(src[1]), "v"(src[2]), "v"(src[3]) : "memory");
+        else
+            asm volatile("global_load_dwordx2 %0, %2, off\n\tglobal_load_dwordx2 %1, %3, off\n\ts_waitcnt vmcnt(0) ; hidden-load wait"
+                         : "=&v"(v[0]), "=&v"(v[1]) : "v"(src[0]), "v"(src[1]) : "memory");
+    } else {
+        if constexpr (MI == 8)
+            asm volatile("global_load_dword %0, %8, off\n\tglobal_load_dword %1, %9, off\n\tglobal_load_dword %2, %10, off\n\tglobal_load_dword %3, %11, off\n\t"
+                         "global_load_dword %4, %12, off\n\tglobal_load_dword %5, %13, off\n\tglobal_load_dword %6, %14, off\n\tglobal_load_dword %7, %15, off\n\t"
+                         "s_waitcnt vmcnt(0) ; hidden-load wait"
+                         : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+                         : "v"(src[0]), "v"(src[1]), "v"(src[2]), "v"(src[3]), "v"(src[4]), "v"(src[5]), "v"(src[6]), "v"(src[7]) : "memory");
+        else if constexpr (MI == 4)
+            asm volatile("global_load_dword %0, %4, off\n\tglobal_load_dword %1, %5, off\n\tglobal_load_dword %2, %6, off\n\tglobal_load_dword %3, %7, off\n\t"
+                         "s_waitcnt vmcnt(0) ; hidden-load wait"
+                         : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]) : "v"(src[0]), "v"(src[1]), "v"(src[2]), "v"(src[3]) : "memory");
+        else
+            asm volatile("global_load_dword %0, %2, off\n\tglobal_load_dword %1, %3, off\n\ts_waitcnt vmcnt(0) ; hidden-load wait"
+                         : "=&v"(v[0]), "=&v"(v[1]) : "v"(src[0]), "v"(src[1]) : "memory");
+    }
+}
+
+// labels of this lane's rows, as columns of the launch (ignored, or of another piece: outside [0, N))
+template <class Cfg>
+__device__ __forceinline__ void ce_columns(const GemmParams& p, int m0, int wm, int lane, int (&col)[Cfg::MI], bool (&dead)[Cfg::MI]) {
+    const u32x2* src[Cfg::MI];
+    u32x2 v[Cfg::MI];
+#pragma unroll
+    for (int i = 0; i < Cfg::MI; ++i)
+        src[i] = reinterpret_cast<const u32x2*>(p.ce_labels + min(m0 + Cfg::moff(wm, i) + (lane & 15), p.M - 1));
+    ce_load_rows<Cfg::MI>(src, v);
+#pragma unroll
+    for (int i = 0; i < Cfg::MI; ++i) {
+        const long long label = (long long)(((unsigned long long)v[i][1] << 32) | v[i][0]);
+        dead[i] = label == p.ce_ignore || label < 0 || label >= p.ce_vocab;
+        col[i] = dead[i] ? -1 : (int)label - p.ce_first;
+    }
+}
+
+// gradient of four consecutive columns n .. n + 3 of a row: g (2^(z - lse2) - [label])
+__device__ __forceinline__ f32x4 ce_grad4(const GemmParams& p, const f32x4& a, float c, float lse2, float g, int col, bool dead, int n) {
+    f32x4 o;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        float v = __builtin_amdgcn_exp2f(__builtin_fmaf(a[r], c, -lse2)) * g;
+        if (n + r == col) v -= g;
+        o[r] = dead || n + r >= p.N ? 0.f : v;       // (an ignored row's logits may be anything)
+    }
+    return o;
 }
 
 template <int EPI>
@@ -158,13 +226,14 @@ __device__ __forceinline__ WorkItem decode_item(const GemmParams& p, int L, int 
     const bf16* baseB = p.B + (long long)it.b * p.strideB + (TB ? (p.b_heads ? (size_t)(it.n0 >> 6) * p.b_heads : (size_t)it.n0) : (size_t)it.n0 * p.ldb);
     // (a transposed A whose M is not a multiple of 8: the last 16-byte piece of a contraction row straddles M; it is kept
     // in range, lda >= M rounded up to 8 guarantees the bytes exist, and the output rows >= M it feeds are never stored)
+    // (K is a multiple of 64 for an A that is not transposed, but for linear_ce.hip's P, whose rows are zeros up to one)
     // Head-major operands: the range runs to the end of the operand's last head.  What a ragged tile reads past its own
     // rows is then the next head's data (finite) instead of zeros: output rows past M are never stored, and a contraction
     // row past K meets the other operand's zeros (only one operand of a product may be head-major and transposed).
     const uint32_t recA = TA ? (p.a_heads ? (uint32_t)(((size_t)((p.M + 63) / 64 - 1 - (it.m0 >> 6)) * p.a_heads + (size_t)p.K * 64) * 2)
                                           : (uint32_t)(((size_t)(p.K - 1) * p.lda + ((rowsA + 7) & ~7)) * 2))
                         : p.a_heads ? (uint32_t)(((size_t)(p.K / 64 - 1) * p.a_heads + (size_t)rowsA * 64) * 2)
-                        : (uint32_t)(((size_t)(rowsA - 1) * p.lda + p.K) * 2);
+                        : (uint32_t)(((size_t)(rowsA - 1) * p.lda + ((p.K + 63) & ~63)) * 2);
     const uint32_t recB = TB ? (p.b_heads ? (uint32_t)(((size_t)((p.N + 63) / 64 - 1 - (it.n0 >> 6)) * p.b_heads + (size_t)p.K * 64) * 2)
                                           : (uint32_t)(((size_t)(p.K - 1) * p.ldb + rowsB) * 2))
                         : (uint32_t)(((size_t)(rowsB - 1) * p.ldb + p.K) * 2);
@@ -253,6 +322,110 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, void* Cb, int m0, 
         }
         return;
     }
+    if (EPI == EPI_CE_STATS) {
+        int col[MI];
+        bool dead[MI];
+        ce_columns<Cfg>(p, m0, wm, lane, col, dead);
+        const float c = p.alpha * CE_LOG2E;
+        const int nw = n0 + Cfg::noff(wn, 0), nl = (lane >> 4) * 4;        // the wave's first column; this lane's within 16
+        if (nw >= p.N) return;
+        const bool edge = nw + NJ * 16 > p.N;
+        f32x2* part = p.ce_part + (size_t)(nw / (NJ * 16)) * p.M;
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int m = m0 + Cfg::moff(wm, i) + (lane & 15);
+            const int rel = col[i] - nw;
+            float z[NJ * 4];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) z[j * 4 + r] = acc[i][j][r] * c;
+            if (edge) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) if (nw + j * 16 + nl + r >= p.N) z[j * 4 + r] = -INFINITY;
+            }
+            if (__ballot(rel >= 0 && rel < NJ * 16)) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (rel == j * 16 + nl + r) {
+                            if (m < p.M) p.ce_target[m] = acc[i][j][r] * p.alpha;
+                            z[j * 4 + r] = -INFINITY;
+                        }
+            }
+            float mx = z[0];
+#pragma unroll
+            for (int k = 1; k < NJ * 4; ++k) mx = fmaxf(mx, z[k]);
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float at = mx == -INFINITY ? 0.f : mx;
+            float s = 0.f;
+#pragma unroll
+            for (int k = 0; k < NJ * 4; ++k) s += __builtin_amdgcn_exp2f(z[k] - at);
+            s += __shfl_xor(s, 16, 64);
+            s += __shfl_xor(s, 32, 64);
+            if (lane < 16 && m < p.M) part[m] = f32x2{mx, s};
+        }
+        return;
+    }
+    if (EPI == EPI_CE_GRAD) {
+        int col[MI];
+        bool dead[MI];
+        ce_columns<Cfg>(p, m0, wm, lane, col, dead);
+        const float *srcl[MI], *srcg[MI];
+        float lse[MI], g[MI];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int mc = min(m0 + Cfg::moff(wm, i) + (lane & 15), p.M - 1);
+            srcl[i] = p.ce_lse + mc;
+            srcg[i] = p.ce_g + mc;
+        }
+        ce_load_rows<MI>(srcl, lse);
+        ce_load_rows<MI>(srcg, g);
+        const float c = p.alpha * CE_LOG2E;
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int m = m0 + Cfg::moff(wm, i) + (lane & 15);
+            if (m >= p.M) continue;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int n = n0 + Cfg::noff(wn, j) + (lane >> 4) * 4;
+                if (n >= ((p.N + 63) & ~63)) continue;
+                const f32x4 o = ce_grad4(p, acc[i][j], c, lse[i] * CE_LOG2E, g[i], col[i], dead[i], n);
+                *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16*>(Cb) + (size_t)m * p.ldc + n) = __builtin_convertvector(o, bf16x4);
+            }
+        }
+        return;
+    }
+    if (EPI == EPI_SLAB_F32) {
+        float* C = reinterpret_cast<float*>(Cb);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int m = m0 + Cfg::moff(wm, i) + (lane & 15);
+            float* row = C + (size_t)min(m, p.M - 1) * p.ldc;
+            f32x4 old[NJ];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) old[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (p.accumulate) {           // (columns past N: the address is clamped to the row's first, the value is not stored)
+#pragma unroll
+                for (int j = 0; j < NJ; j += 2) {
+                    const int na = n0 + Cfg::noff(wn, j) + (lane >> 4) * 4, nb = n0 + Cfg::noff(wn, j + 1) + (lane >> 4) * 4;
+                    const float *sa = row + (na < p.N ? na : 0), *sb = row + (nb < p.N ? nb : 0);
+                    asm volatile("global_load_dwordx4 %0, %2, off\n\tglobal_load_dwordx4 %1, %3, off\n\ts_waitcnt vmcnt(0) ; hidden-load wait"
+                                 : "=&v"(old[j]), "=&v"(old[j + 1]) : "v"(sa), "v"(sb) : "memory");
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int n = n0 + Cfg::noff(wn, j) + (lane >> 4) * 4;
+                if (m < p.M && n < p.N) *reinterpret_cast<f32x4*>(row + n) = acc[i][j] * p.alpha + old[j];      // N is a multiple of 4
+            }
+        }
+        return;
+    }
     if (EPI == EPI_ATOMIC_F32) {
         float* C = reinterpret_cast<float*>(Cb);
 #pragma unroll
@@ -320,7 +493,7 @@ __global__ void __launch_bounds__(Cfg::WGM * Cfg::WGN * 64) gemm_bf16_kernel(Gem
                 Ops::template multiply<NATURAL>(smem, 0, wm, wn, lane, acc);
                 __syncthreads();
             }
-            epilogue<Cfg, EPI>(p, batch_c<EPI>(p, it.b), it.m0, it.n0, wm, wn, lane, acc);
+            epilogue<Cfg, EPI>(p, batch_c<EPI>(p, EPI == EPI_SLAB_F32 ? it.kbeg / p.k_per_split : it.b), it.m0, it.n0, wm, wn, lane, acc);
             L = item_of(b, ++round, G, total_items);
             if (L >= 0) it = decode_item<Cfg, TA, TB>(p, L, ntm, ntn);
         }
@@ -381,7 +554,7 @@ __global__ void __launch_bounds__(Cfg::WGM * Cfg::WGN * 64) gemm_ring_kernel(Gem
         buf = buf + 1 == NS ? 0 : buf + 1;
         nbuf = nbuf + 1 == NS ? 0 : nbuf + 1;
     }
-    epilogue<Cfg, EPI>(p, batch_c<EPI>(p, it.b), it.m0, it.n0, wm, wn, lane, acc);
+    epilogue<Cfg, EPI>(p, batch_c<EPI>(p, EPI == EPI_SLAB_F32 ? it.kbeg / p.k_per_split : it.b), it.m0, it.n0, wm, wn, lane, acc);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -669,7 +842,7 @@ __global__ void __launch_bounds__(512) gemm_phased_kernel(GemmParams p, int ntm,
     StepStream<TA, TB> st;
     st.wi = decode_item<CfgPhased, TA, TB>(p, L, ntm, ntn);
     st.k = st.wi.kbeg; st.round = 0; st.live = true;
-    int m0 = st.wi.m0, n0 = st.wi.n0, bz = st.wi.b;
+    int m0 = st.wi.m0, n0 = st.wi.n0, bz = EPI == EPI_SLAB_F32 ? st.wi.kbeg / p.k_per_split : st.wi.b;
     int nsteps = (st.wi.kend - st.wi.kbeg + BK - 1) / BK;
 
     {
@@ -790,6 +963,7 @@ __global__ void __launch_bounds__(512) gemm_phased_kernel(GemmParams p, int ntm,
             bz = L / per_batch;
             const int rr = L - bz * per_batch;
             const int split = rr / ntiles, tt = rr - split * ntiles;
+            if (EPI == EPI_SLAB_F32) bz = split;
             int tm, tn;
             if (ntm >= ntn) { tm = tt / ntn; tn = tt - tm * ntn; } else { tn = tt / ntm; tm = tt - tn * ntm; }
             m0 = tm * 256; n0 = tn * 256;
@@ -1197,10 +1371,11 @@ int launch(const GemmParams& p, int splits, hipStream_t stream) {
     else {
         // the 256x256 tile pays off once there is about one tile per CU (split slices count for atomics)
         const long long t256 = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256) * p.batch;
-        large = p.M >= 256 && p.N >= 256 && (t256 >= 200 || (EPI == EPI_ATOMIC_F32 && t256 >= 9));
+        large = p.M >= 256 && p.N >= 256 && (t256 >= 200 || (EPI == EPI_ATOMIC_F32 && t256 >= 9) || (EPI == EPI_SLAB_F32 && t256 * splits >= 128));
     }
     // the phased kernel moves bf16 outputs (and their residual / mask operand) in 16-byte row pieces
-    const bool rows16 = (EPI == EPI_F32 || EPI == EPI_ATOMIC_F32 || EPI == EPI_TOPK_DENSE || EPI == EPI_TOPK_FILTER) ||
+    const bool rows16 = (EPI == EPI_F32 || EPI == EPI_ATOMIC_F32 || EPI == EPI_TOPK_DENSE || EPI == EPI_TOPK_FILTER ||
+                         EPI == EPI_CE_STATS || EPI == EPI_CE_GRAD || EPI == EPI_SLAB_F32) ||
                         (p.N % 8 == 0 && p.ldc % 8 == 0 && ((uintptr_t)p.C & 15) == 0 &&
                          (!(EPI == EPI_RES_DROP || EPI == EPI_MASK) || (p.ldaux % 8 == 0 && ((uintptr_t)p.aux & 15) == 0)));
     // ... and numbers dropout's quads with 32 bits
@@ -1229,6 +1404,9 @@ int dispatch_epi(const GemmParams& p, int epi, int splits, hipStream_t s) {
         case EPI_MASK_BITS: return launch<TA, TB, EPI_MASK_BITS>(p, splits, s);
         case EPI_F32: return launch<TA, TB, EPI_F32>(p, splits, s);
         case EPI_ATOMIC_F32: return launch<TA, TB, EPI_ATOMIC_F32>(p, splits, s);
+        case EPI_CE_STATS: if (!TA && !TB) return launch<false, false, EPI_CE_STATS>(p, splits, s); break;
+        case EPI_CE_GRAD: if (!TA && !TB) return launch<false, false, EPI_CE_GRAD>(p, splits, s); break;
+        case EPI_SLAB_F32: if (TB) return launch<TA, true, EPI_SLAB_F32>(p, splits, s); break;
         case EPI_TOPK_DENSE: if (!TA && !TB) return launch<false, false, EPI_TOPK_DENSE>(p, splits, s); break;
         case EPI_TOPK_FILTER: if (!TA && !TB) return launch<false, false, EPI_TOPK_FILTER>(p, splits, s); break;
     }

@@ -1,0 +1,207 @@
+// Softmax cross entropy of a linear head over a large vocabulary, without its logits:
+//   z = scale h w^T      lse_r = log sum_v exp z_rv      loss_r = lse_r - z_r,label (0 for an ignored row)
+//   P_rv = g_r (exp(z_rv - lse_r) - [v = label_r])       dh = scale P w      dw = scale P^T h
+// Forward: one product whose epilogue (EPI_CE_STATS in gemm.hip) leaves a maximum and a sum for every row and 64 columns, and
+// a second kernel that joins them; the logits never leave the registers.  The label's term is kept out of the sums, so that
+// a confident row's loss log(1 + sum of the others / its own) keeps its relative precision.
+// Backward: the vocabulary goes by in pieces.  A piece's logits are computed again and leave as P in bf16 (the MFMA operand
+// type; half a step of 2^-8 relative to each entry, as paced_cross_entropy's dlogits), which feeds the two other products.
+// dh is summed over pieces and slices of a piece in fp32 slabs with one owner per element, dw is complete with its piece:
+// nothing is added atomically, equal inputs give equal bits.
+// Matrix-core bound: 2 R V d operations forward, three times that backward.
+#include "gemm.h"
+#include <cmath>
+
+namespace {
+
+constexpr float LN2 = 0.6931471805599453f, LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+    const float mx = fmaxf(m, m2), at = mx == -INFINITY ? 0.f : mx;
+    s = s * __builtin_amdgcn_exp2f(m - at) + s2 * __builtin_amdgcn_exp2f(m2 - at);
+    m = mx;
+}
+
+// 8 rows of a workgroup, 32 threads over the column groups of each
+__global__ void __launch_bounds__(256) ce_join_kernel(const f32x2* __restrict__ part, int groups, const float* __restrict__ target,
+                                                      const long long* __restrict__ labels, long long ignore, int V,
+                                                      float* __restrict__ loss, float* __restrict__ lse, int R) {
+    __shared__ f32x2 sh[4][8];
+    const int r = threadIdx.x & 7, k = threadIdx.x >> 3;
+    const int row = blockIdx.x * 8 + r, rr = min(row, R - 1);
+    float m = -INFINITY, s = 0.f;
+    for (int g = k; g < groups; g += 32) {
+        const f32x2 v = part[(size_t)g * R + rr];
+        join(m, s, v[0], v[1]);
+    }
+#pragma unroll
+    for (int o = 8; o < 64; o <<= 1) join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+    if ((threadIdx.x & 63) < 8) sh[threadIdx.x >> 6][r] = f32x2{m, s};
+    __syncthreads();
+    if (threadIdx.x >= 8 || row >= R) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) join(m, s, sh[w][r][0], sh[w][r][1]);
+    const long long label = labels[row];
+    if (label == ignore || label < 0 || label >= V) {
+        loss[row] = 0.f;
+        if (lse) lse[row] = m * LN2 + logf(s);
+        return;
+    }
+    const float t = target[row], t2 = t * LOG2E;
+    float l;
+    if (m == -INFINITY) l = s == 0.f ? 0.f : s;                 // no other entry (or a NaN among them)
+    else if (t2 >= m) l = log1pf(s * __builtin_amdgcn_exp2f(m - t2));
+    else l = (m - t2) * LN2 + logf(s + __builtin_amdgcn_exp2f(t2 - m));
+    loss[row] = l;
+    if (lse) lse[row] = t + l;
+}
+
+// dh = bf16 of the slabs' sum, slab by slab
+__global__ void __launch_bounds__(256) ce_dh_kernel(const float* __restrict__ slabs, int count, long long slab, bf16* __restrict__ dh, int lddh, int R, int d) {
+    const int d8 = d >> 3;
+    const long long total = (long long)R * d8;
+    for (long long id = (long long)blockIdx.x * 256 + threadIdx.x; id < total; id += (long long)gridDim.x * 256) {
+        const int r = (int)(id / d8), c = (int)(id - (long long)r * d8);
+        f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+        for (int k = 0; k < count; ++k) {
+            const float* src = slabs + (size_t)k * slab + (size_t)r * d + c * 8;
+            a += *reinterpret_cast<const f32x4*>(src);
+            b += *reinterpret_cast<const f32x4*>(src + 4);
+        }
+        bf16x8 o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { o[j] = f2bf(a[j]); o[4 + j] = f2bf(b[j]); }
+        *reinterpret_cast<bf16x8*>(dh + (size_t)r * lddh + c * 8) = o;
+    }
+}
+
+int blocks_for(long long items) {
+    const long long g = (items + 255) / 256;
+    return (int)(g < 1 ? 1 : g > 16384 ? 16384 : g);
+}
+
+size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+// Pieces of the vocabulary, and slices of a piece for dh.  A piece's P takes at most 256 MiB; a launch of dh's product should
+// give every compute unit a tile (256x256 tiles where the output has them, else 64x64), a slice has four K steps or more.
+struct CePlan { int piece, ldp, slabs; };
+CePlan ce_plan(int R, int V, int d) {
+    CePlan pl;
+    long long fit = (256ll << 20) / 2 / (R > 0 ? R : 1) / 256 * 256;
+    if (fit < 256) fit = 256;
+    const int pieces = (int)((V + fit - 1) / fit);
+    long long piece = ((V + pieces - 1) / pieces + 255) / 256 * 256;
+    if (piece > V) piece = V;
+    pl.piece = (int)piece;
+    pl.ldp = (int)((piece + 63) / 64 * 64);
+    const int ksteps = (pl.piece + 63) / 64, cus = paced_cu_count();
+    const long long big = (long long)((R + 255) / 256) * ((d + 255) / 256), tiny = (long long)((R + 63) / 64) * ((d + 63) / 64);
+    long long want = R >= 256 && d >= 256 ? cus / big : 2ll * cus / tiny;
+    if (want > ksteps / 4) want = ksteps / 4;
+    if (want < 1) want = 1;
+    const int per = (int)((ksteps + want - 1) / want);
+    pl.slabs = (ksteps + per - 1) / per;
+    return pl;
+}
+
+GemmParams product(const void* A, int lda, const void* B, int ldb, void* C, int ldc, int M, int N, int K, float alpha) {
+    GemmParams p = {};
+    p.A = (const bf16*)A; p.B = (const bf16*)B; p.C = C;
+    p.M = M; p.N = N; p.K = K; p.lda = lda; p.ldb = ldb; p.ldc = ldc;
+    p.k_per_split = K; p.batch = 1; p.alpha = alpha; p.mask_scale = 1.f; p.drop = make_drop(0.f, 0);
+    return p;
+}
+
+int ce_check(const char* who, const void* h, int ldh, const void* w, int ldw, const long long* labels, int R, int V, int d) {
+    PACED_CHECK_ARG(R >= 0 && V > 0 && d > 0 && d % 64 == 0, "%s: need R >= 0, V > 0 and d a multiple of 64 (R=%d V=%d d=%d)", who, R, V, d);
+    if (R == 0) return PACED_OK;
+    PACED_CHECK_ARG(h && w && labels, "%s: null operand", who);
+    PACED_CHECK_ARG(ldh >= d && ldw >= d && ldh % 8 == 0 && ldw % 8 == 0 && (((uintptr_t)h | (uintptr_t)w) & 15) == 0,
+                    "%s: h and w need 16-byte aligned rows, strides of at least d and multiples of 8 (ldh=%d ldw=%d)", who, ldh, ldw);
+    return PACED_OK;
+}
+
+}  // namespace
+
+extern "C" size_t paced_linear_ce_fwd_workspace_bytes(int R, int V) {
+    if (R <= 0 || V <= 0) return 0;
+    return round256((size_t)((V + 31) / 32) * R * 8) + round256((size_t)R * 4);
+}
+
+extern "C" int paced_linear_ce_fwd(const void* h, int ldh, const void* w, int ldw, const long long* labels, float* loss, float* lse,
+                                   int R, int V, int d, long long ignore_index, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = ce_check("paced_linear_ce_fwd", h, ldh, w, ldw, labels, R, V, d);
+    if (rc != PACED_OK || R == 0) return rc;
+    PACED_CHECK_ARG(loss, "paced_linear_ce_fwd: null operand");
+    const size_t need = paced_linear_ce_fwd_workspace_bytes(R, V);
+    PACED_CHECK_ARG(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
+                    "paced_linear_ce_fwd: a 16-byte aligned workspace of %zu bytes is needed, got %zu", need, workspace_bytes);
+    GemmParams p = product(h, ldh, w, ldw, nullptr, 0, R, V, d, scale);
+    p.ce_part = (f32x2*)workspace;
+    p.ce_target = (float*)((char*)workspace + round256((size_t)((V + 31) / 32) * R * 8));
+    p.ce_labels = labels; p.ce_ignore = ignore_index; p.ce_vocab = V;
+    const int rg = paced_gemm_launch(p, false, false, EPI_CE_STATS, 1, (hipStream_t)stream);
+    if (rg != PACED_OK) return rg;
+    const int width = paced_gemm_last_kernel() < 128 ? 32 : 64;           // columns of a wave in the tiles that were taken
+    hipLaunchKernelGGL(ce_join_kernel, dim3((R + 7) / 8), dim3(256), 0, (hipStream_t)stream, p.ce_part, (V + width - 1) / width, p.ce_target,
+                       labels, ignore_index, V, loss, lse, R);
+    PACED_CHECK_LAUNCH();
+    return PACED_OK;
+}
+
+extern "C" size_t paced_linear_ce_bwd_workspace_bytes(int R, int V, int d) {
+    if (R <= 0 || V <= 0 || d <= 0) return 0;
+    const CePlan pl = ce_plan(R, V, d);
+    return round256((size_t)R * pl.ldp * 2) + (size_t)pl.slabs * R * d * 4;
+}
+
+extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ldw, const long long* labels, const float* lse, const float* gloss,
+                                   void* dh, int lddh, void* dw, int lddw, int dw_f32, int R, int V, int d, long long ignore_index, float scale,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = ce_check("paced_linear_ce_bwd", h, ldh, w, ldw, labels, R, V, d);
+    if (rc != PACED_OK) return rc;
+    hipStream_t s = (hipStream_t)stream;
+    PACED_CHECK_ARG(!dw || (lddw >= d && lddw % 8 == 0 && ((uintptr_t)dw & 15) == 0), "paced_linear_ce_bwd: dw needs 16-byte aligned rows, a stride of at least d and a multiple of 8 (lddw=%d)", lddw);
+    if (R == 0) {                                     // no row: dw's sum is empty
+        if (!dw || dw_f32) return PACED_OK;
+        hipLaunchKernelGGL(ce_dh_kernel, dim3(blocks_for((long long)V * (d >> 3))), dim3(256), 0, s, nullptr, 0, 0LL, (bf16*)dw, lddw, V, d);
+        PACED_CHECK_LAUNCH();
+        return PACED_OK;
+    }
+    PACED_CHECK_ARG(lse && gloss, "paced_linear_ce_bwd: null operand");
+    PACED_CHECK_ARG(!dh || (lddh >= d && lddh % 8 == 0 && ((uintptr_t)dh & 15) == 0), "paced_linear_ce_bwd: dh needs 16-byte aligned rows, a stride of at least d and a multiple of 8 (lddh=%d)", lddh);
+    const CePlan pl = ce_plan(R, V, d);
+    const size_t need = paced_linear_ce_bwd_workspace_bytes(R, V, d);
+    PACED_CHECK_ARG(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
+                    "paced_linear_ce_bwd: a 16-byte aligned workspace of %zu bytes is needed, got %zu", need, workspace_bytes);
+    // a transposed operand is addressed with 32-bit byte offsets from its first row
+    PACED_CHECK_ARG((unsigned long long)R * (ldh > pl.ldp ? ldh : pl.ldp) < (1ull << 31) && (unsigned long long)pl.piece * ldw < (1ull << 31),
+                    "paced_linear_ce_bwd: %d rows of stride %d span more than 4 GiB; pass fewer rows at a time", R, ldh);
+    bf16* P = (bf16*)workspace;
+    float* slabs = (float*)((char*)workspace + round256((size_t)R * pl.ldp * 2));
+    for (int v0 = 0; v0 < V; v0 += pl.piece) {
+        const int n = V - v0 < pl.piece ? V - v0 : pl.piece;
+        const bf16* wp = (const bf16*)w + (size_t)v0 * ldw;
+        GemmParams p = product(h, ldh, wp, ldw, P, pl.ldp, R, n, d, scale);
+        p.ce_labels = labels; p.ce_lse = lse; p.ce_g = gloss;
+        p.ce_ignore = ignore_index; p.ce_vocab = V; p.ce_first = v0;
+        int r = paced_gemm_launch(p, false, false, EPI_CE_GRAD, 1, s);
+        if (r != PACED_OK) return r;
+        if (dh) {
+            p = product(P, pl.ldp, wp, ldw, slabs, d, R, d, n, scale);
+            p.strideC = (long long)R * d;
+            p.accumulate = v0 > 0;
+            if ((r = paced_gemm_launch(p, false, true, EPI_SLAB_F32, pl.slabs, s)) != PACED_OK) return r;
+        }
+        if (dw) {
+            p = product(P, pl.ldp, h, ldh, dw_f32 ? (void*)((float*)dw + (size_t)v0 * lddw) : (void*)((bf16*)dw + (size_t)v0 * lddw), lddw, n, d, R, scale);
+            p.accumulate = 1;
+            if ((r = paced_gemm_launch(p, true, true, dw_f32 ? EPI_SLAB_F32 : EPI_BF16, 1, s)) != PACED_OK) return r;
+        }
+    }
+    if (dh) {
+        hipLaunchKernelGGL(ce_dh_kernel, dim3(blocks_for((long long)R * (d >> 3))), dim3(256), 0, s, slabs, pl.slabs, (long long)R * d, (bf16*)dh, lddh, R, d);
+        PACED_CHECK_LAUNCH();
+    }
+    return PACED_OK;
+}

@@ -529,6 +529,51 @@ def cross_entropy(logits, labels, loss, dlogits=None, *, ignore_index=-100, gsca
     return loss
 
 
+def _head_operands(h, w, labels):
+    if h.dim() != 2 or w.dim() != 2 or h.shape[1] != w.shape[1] or h.shape[1] % 64 or h.shape[1] == 0 or w.shape[0] == 0:
+        raise ValueError(f"h must be [R, d] and w [V, d] with d a multiple of 64, got {tuple(h.shape)} and {tuple(w.shape)}")
+    R, d = h.shape
+    V = w.shape[0]
+    _flat(labels, R, I64, "labels")
+    return R, V, d, _rows_of(h, (R, d), BF16, "h"), _rows_of(w, (V, d), BF16, "w")
+
+
+def linear_ce_fwd(h, w, labels, loss, lse=None, *, ignore_index=-100, scale=1.0, workspace=None):
+    """Cross entropy of a linear head without its logits: loss[r] = logsumexp(z[r]) - z[r, label] for z = scale * h w^T
+    (h bf16 [R, d], w bf16 [V, d], labels int64 [R]); rows whose label is ``ignore_index`` or outside [0, V) give 0.
+    ``lse`` (fp32 [R]) is what ``linear_ce_bwd`` needs."""
+    lib = _lib.load()
+    with _one_device(h=h, w=w, labels=labels, loss=loss, lse=lse):
+        R, V, d, ldh, ldw = _head_operands(h, w, labels)
+        _flat(loss, R, F32, "loss"); _flat(lse, R, F32, "lse")
+        need = lib.paced_linear_ce_fwd_workspace_bytes(R, V)
+        ws = _workspace(workspace, need, h.device)
+        _lib.check(lib.paced_linear_ce_fwd(_p(h), ldh, _p(w), ldw, _p(labels), _p(loss), _p(lse), R, V, d, ignore_index, scale, _p(ws), need,
+                                           _stream()), "paced_linear_ce_fwd")
+    return loss
+
+
+def linear_ce_bwd(h, w, labels, lse, grad_loss, dh=None, dw=None, *, ignore_index=-100, scale=1.0, workspace=None):
+    """Gradients of sum(grad_loss * loss) of ``linear_ce_fwd``: ``dh`` (bf16 [R, d]) is written, ``dw`` [V, d] is written
+    (bf16) or added to (fp32); either may be left out."""
+    lib = _lib.load()
+    with _one_device(h=h, w=w, labels=labels, lse=lse, grad_loss=grad_loss, dh=dh, dw=dw):
+        R, V, d, ldh, ldw = _head_operands(h, w, labels)
+        _flat(lse, R, F32, "lse"); _flat(grad_loss, R, F32, "grad_loss")
+        lddh = _rows_of(dh, (R, d), BF16, "dh")
+        if dw is not None and dw.dtype not in (BF16, F32):
+            raise ValueError(f"dw must be bf16 or fp32, got {dw.dtype}")
+        f32 = dw is not None and dw.dtype == F32
+        lddw = _rows_of(dw, (V, d), F32 if f32 else BF16, "dw")
+        if dh is None and dw is None:
+            return None
+        need = lib.paced_linear_ce_bwd_workspace_bytes(R, V, d)
+        ws = _workspace(workspace, need, h.device)
+        _lib.check(lib.paced_linear_ce_bwd(_p(h), ldh, _p(w), ldw, _p(labels), _p(lse), _p(grad_loss), _p(dh), lddh, _p(dw), lddw, int(f32),
+                                           R, V, d, ignore_index, scale, _p(ws), need, _stream()), "paced_linear_ce_bwd")
+    return dh
+
+
 def lce_group(pce, nce, ce, n, use_mean):
     lib = _lib.load()
     _chk(pce, F32, "pce"); _chk(nce, F32, "nce"); _chk(ce, F32, "ce")
