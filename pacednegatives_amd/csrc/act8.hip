@@ -258,6 +258,197 @@ __global__ void __launch_bounds__(256) act8_dw_kernel(DwParams p, int ntm, int n
     }
 }
 
+// 256x256 tiles: the phased kernel of gemm.hip (same ring order, phases, barriers and A halves) with B halves of codes: 8 KiB
+// instead of 16, one LDS-DMA instruction per wave instead of two, half the fragment reads; a fragment is converted behind its
+// phase's barrier.  Codes of a half: [64 tokens][128] bytes, 16-byte unit u of token k at u ^ (k & 7); half h holds the h-th 32
+// features of every 64.  With each step's first B half every wave fetches the scales of its own 64 features.
+// Instructions in flight behind a phase's wait (the six youngest half-tiles; B half 0 and its scales 2, A halves 2, B half 1 1):
+// 11 after B half 0 and A half 0 were issued, 10 after B half 1 and A half 1.
+// LDS: ring slots 0, 2, .. 8 are B halves (5 x 8 KiB), 1, 3, .. 9 A halves (5 x 16 KiB), three sets of scales (a set is read in
+// its step and overwritten two steps on): 126 KiB.
+constexpr int DP_B = 5 * 16384, DP_S = DP_B + 5 * 8192, DP_LDS = DP_S + 3 * 2048;
+
+struct DwStep {
+    __amdgpu_buffer_rsrc_t rA, rB, rS;
+    uint32_t sA, sB, sS;
+};
+struct DwStream {
+    DwItem it;
+    int k, round;
+    bool live;
+    __device__ __forceinline__ DwStep take(const DwParams& p, int b, int G, int ntm, int ntn, int total, uint32_t strideA) {
+        DwStep s;
+        if (live) {
+            s.rA = it.rA; s.rB = it.rB; s.rS = it.rS;
+            s.sA = (uint32_t)k * strideA; s.sB = (uint32_t)k * (uint32_t)p.N; s.sS = (uint32_t)(k / QBLOCK) * (uint32_t)p.N;
+            k += BK;
+            if (it.kbeg + k >= it.kend) {
+                const int L = item_of(b, ++round, G, total);
+                if (L >= 0) { it = dw_item<256, 256>(p, L, ntm, ntn); k = 0; }
+                else live = false;
+            }
+        } else {                       // past the last item: the same instructions through empty descriptors
+            s.rA = __builtin_amdgcn_make_buffer_rsrc((void*)p.dy, 0, 0, 0x00020000);
+            s.rB = __builtin_amdgcn_make_buffer_rsrc((void*)p.q, 0, 0, 0x00020000);
+            s.rS = __builtin_amdgcn_make_buffer_rsrc((void*)p.scale, 0, 0, 0x00020000);
+            s.sA = s.sB = s.sS = 0;
+        }
+        return s;
+    }
+};
+
+__global__ void __launch_bounds__(512) act8_dw_phased_kernel(DwParams p, int ntm, int ntn, int total) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = w >> 2, wc = w & 3, g = lane >> 4, i16 = lane & 15;
+    const int G = gridDim.x, b = blockIdx.x;
+
+    uint32_t offA[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) offA[i] = stage_offset<true, 128>((i * 8 + w) * 64 + lane, p.lddy, p.heads);
+    const int bk = (w * 64 + lane) >> 3, bc = ((w * 64 + lane) & 7) ^ (bk & 7);
+    const uint32_t offB = (uint32_t)(bk * p.N + (bc >> 1) * 64 + (bc & 1) * 16);
+    // lanes 0-15: the first 32 tokens' scales of the wave's 64 features, 16-31: the second's, the rest outside every descriptor
+    const uint32_t offS = lane < 32 ? (uint32_t)((lane >> 4) * p.N + wc * 64 + (lane & 15) * 4) : 0x80000000u;
+    const uint32_t strideA = (uint32_t)p.lddy * 2u;
+    const uint32_t halfA = p.heads ? (uint32_t)(p.heads * 4) : 256u, halfB = 32u;
+    char* const sw = smem + w * 1024;
+    char* const ssc = smem + DP_S + w * 256;
+#define DP_STAGE_A(st, slot, off) PACED_STAGE_HALF((st).rA, sw + ((slot) >> 1) * 16384, offA, (st).sA + (off))
+#define DP_STAGE_B(st, slot, off) __builtin_amdgcn_raw_ptr_buffer_load_lds((st).rB, LDS_PTR(sw + DP_B + ((slot) >> 1) * 8192), 16, offB, (st).sB + (off), 0, 0)
+#define DP_STAGE_S(st, set) __builtin_amdgcn_raw_ptr_buffer_load_lds((st).rS, LDS_PTR(ssc + (set) * 2048), 4, offS, (st).sS, 0, 0)
+
+    const int L = item_of(b, 0, G, total);
+    if (L < 0) return;
+    DwStream st;
+    st.it = dw_item<256, 256>(p, L, ntm, ntn);
+    st.k = 0; st.round = 0; st.live = true;
+    DwItem cur = st.it;
+    {
+        const DwStep c0 = st.take(p, b, G, ntm, ntn, total, strideA);
+        const DwStep c1 = st.take(p, b, G, ntm, ntn, total, strideA);
+        DP_STAGE_B(c0, 0, 0); DP_STAGE_S(c0, 0);
+        DP_STAGE_A(c0, 1, 0);
+        DP_STAGE_B(c0, 2, halfB);
+        DP_STAGE_A(c0, 3, halfA);
+        DP_STAGE_B(c1, 4, 0); DP_STAGE_S(c1, 1);
+        DP_STAGE_A(c1, 5, 0);
+        DP_STAGE_B(c1, 6, halfB);
+        DP_STAGE_A(c1, 7, halfA);
+    }
+    asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    if (wr == 1) __builtin_amdgcn_s_barrier();       // second wave group runs one barrier behind
+    DwStep c2 = st.take(p, b, G, ntm, ntn, total, strideA);
+
+    f32x4 acc[8][4];
+    bf16x8 fa[4][2], fb0[2][2], fb1[2][2];
+    u32x2 cb[2][2];
+    uint32_t sb[2][2];
+    int base = 0, set = 0;                            // ring slot of this K step's first half-tile, its set of scales
+    // fragment reads of one B half (inline assembly, waited for behind the phase's barrier like A's)
+    auto read_b = [&](int slot, int half) {
+        const uint32_t lb = (uint32_t)(uintptr_t)LDS_PTR(smem + DP_B + (slot >> 1) * 8192);
+        const uint32_t ls = (uint32_t)(uintptr_t)LDS_PTR(ssc + set * 2048) + (uint32_t)(half * 32 + i16);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int k = 8 * g + (i16 >> 1);
+            const uint32_t a = lb + (uint32_t)(k * 128 + (((wc * 2 + j) ^ (k & 7)) << 4) + (i16 & 1) * 8);
+            asm volatile("ds_read_b64_tr_b8 %0, %1" : "=v"(cb[j][0]) : "v"(a));
+            asm volatile("ds_read_b64_tr_b8 %0, %1 offset:%2" : "=v"(cb[j][1]) : "v"(a), "n"(32 * 128));
+            if (j == 0) {
+                asm volatile("ds_read_u8 %0, %1" : "=v"(sb[0][0]) : "v"(ls));
+                asm volatile("ds_read_u8 %0, %1 offset:64" : "=v"(sb[0][1]) : "v"(ls));
+            } else {
+                asm volatile("ds_read_u8 %0, %1 offset:16" : "=v"(sb[1][0]) : "v"(ls));
+                asm volatile("ds_read_u8 %0, %1 offset:80" : "=v"(sb[1][1]) : "v"(ls));
+            }
+        }
+    };
+    auto convert_b = [&](bf16x8 (&fb)[2][2]) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) fb[j][kk] = act8_fragment(cb[j][kk], sb[j][kk]);
+    };
+    for (int round = 0;;) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int nsteps = (cur.kend - cur.kbeg + BK - 1) / BK;
+        for (int t = 0; t < nsteps; ++t) {
+            const int sB0 = base, sA0 = ring_wrap(base + 1), sB1 = ring_wrap(base + 2), sA1 = ring_wrap(base + 3);
+            const int d1 = ring_wrap(base + 8), d2 = ring_wrap(base + 9);      // phases 3 and 4 reuse sB0 and sA0
+            const int next2 = set == 0 ? 2 : set - 1;                            // the set of step t + 2
+            // ---- phase 1
+            read_b(sB0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk) fa[i][kk] = read_frag<true, 128, true>(smem + (sA0 >> 1) * 16384, wr * 64 + i * 16, kk, lane);
+            DP_STAGE_B(c2, d1, 0);
+            DP_STAGE_S(c2, next2);
+            asm volatile("s_waitcnt vmcnt(11)" ::: "memory");
+            PACED_PINNED_BARRIER();
+            PACED_WAIT_LDS_READS();
+            convert_b(fb0);
+            quadrant_mfma<false>(fa, fb0, acc, 0, 0);
+            PACED_PINNED_BARRIER();
+            // ---- phase 2
+            read_b(sB1, 1);
+            DP_STAGE_A(c2, d2, 0);
+            asm volatile("s_waitcnt vmcnt(11)" ::: "memory");
+            PACED_PINNED_BARRIER();
+            PACED_WAIT_LDS_READS();
+            convert_b(fb1);
+            quadrant_mfma<false>(fa, fb1, acc, 0, 1);
+            PACED_PINNED_BARRIER();
+            // ---- phase 3
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk) fa[i][kk] = read_frag<true, 128, true>(smem + (sA1 >> 1) * 16384, wr * 64 + i * 16, kk, lane);
+            DP_STAGE_B(c2, sB0, halfB);
+            asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+            PACED_PINNED_BARRIER();
+            PACED_WAIT_LDS_READS();
+            quadrant_mfma<false>(fa, fb1, acc, 1, 1);
+            PACED_PINNED_BARRIER();
+            // ---- phase 4
+            DP_STAGE_A(c2, sA0, halfA);
+            c2 = st.take(p, b, G, ntm, ntn, total, strideA);
+            base = ring_wrap(base + 4);
+            set = set == 2 ? 0 : set + 1;
+            asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+            PACED_PINNED_BARRIER();
+            quadrant_mfma<false>(fa, fb0, acc, 1, 0);
+            PACED_PINNED_BARRIER();
+        }
+        if (wr == 0) __builtin_amdgcn_s_barrier();       // both groups run their epilogues side by side (see gemm.hip)
+        float* out = p.out + (size_t)cur.split * p.slab;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int m = cur.m0 + CfgPhased::moff(wr, i) + i16;
+            if (m >= p.M) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int n = cur.n0 + CfgPhased::noff(wc, j) + g * 4;
+                if (n < p.N) *reinterpret_cast<f32x4*>(out + (size_t)m * p.ldout + n) = acc[i][j];
+            }
+        }
+        const int Ln = item_of(b, ++round, G, total);
+        if (Ln < 0) break;
+        cur = dw_item<256, 256>(p, Ln, ntm, ntn);
+        if (wr == 1) __builtin_amdgcn_s_barrier();       // fall one barrier behind again
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#undef DP_STAGE_A
+#undef DP_STAGE_B
+#undef DP_STAGE_S
+}
+
 // dw (+)= the slabs' sum, slab by slab
 __global__ void __launch_bounds__(256) slab_sum_kernel(const float* __restrict__ slabs, int count, long long slab, float* dw, int lddw,
                                                        int M, int N, int accumulate) {
@@ -274,15 +465,27 @@ __global__ void __launch_bounds__(256) slab_sum_kernel(const float* __restrict__
     }
 }
 
-struct DwPlan { int ntm, ntn, splits, k_per_split; };
+// Which tiles, and how many slices of the tokens.  256x256 tiles run at about three times the rate of 64x64 ones, so they are
+// taken when they waste less than that at the output's edges and when tiles times slices (of 12 K steps or more) give most
+// compute units one.
+struct DwPlan { int tile, ntm, ntn, splits, k_per_split; };
 DwPlan dw_plan(int T, int M, int N) {
     DwPlan pl;
-    pl.ntm = (M + 63) / 64;
-    pl.ntn = (N + 63) / 64;
-    const int ktiles = (T + BK - 1) / BK;
-    const long long tiles = (long long)pl.ntm * pl.ntn, slots = 3LL * paced_cu_count();
-    long long splits = tiles >= slots ? 1 : slots / tiles;
-    if (splits > (ktiles + 3) / 4) splits = (ktiles + 3) / 4;
+    const int ktiles = (T + BK - 1) / BK, cus = paced_cu_count();
+    const long long t256 = (long long)((M + 255) / 256) * ((N + 255) / 256), t64 = (long long)((M + 63) / 64) * ((N + 63) / 64);
+    long long splits = t256 >= cus ? 1 : cus / t256;
+    if (splits > ktiles / 12) splits = ktiles / 12 > 0 ? ktiles / 12 : 1;
+    if (t256 * splits * 8 >= cus * 5 && t256 * 16 * 2 < t64 * 5) {
+        pl.tile = 256;
+        pl.ntm = (M + 255) / 256;
+        pl.ntn = (N + 255) / 256;
+    } else {
+        pl.tile = 64;
+        pl.ntm = (M + 63) / 64;
+        pl.ntn = (N + 63) / 64;
+        splits = t64 >= 3LL * cus ? 1 : 3LL * cus / t64;
+        if (splits > (ktiles + 3) / 4) splits = (ktiles + 3) / 4;
+    }
     const int per = (int)((ktiles + splits - 1) / splits);
     pl.k_per_split = per * BK;
     pl.splits = (ktiles + per - 1) / per;
@@ -360,7 +563,17 @@ extern "C" int paced_act8_dweight(const void* dy, int lddy, long long dy_heads, 
     p.ldout = need ? N : lddw;
     p.slab = (long long)M * N;
     const int total = pl.ntm * pl.ntn * pl.splits;
-    hipLaunchKernelGGL(act8_dw_kernel, dim3(total), dim3(256), DW_NS * DW_STEP, s, p, pl.ntm, pl.ntn, total);
+    if (pl.tile == 256) {
+        static PerDeviceOnce once;
+        bool& attr_set = once.flag();
+        if (!attr_set) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&act8_dw_phased_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, DP_LDS);
+            if (e != hipSuccess) { paced_set_error("paced_act8_dweight: hipFuncSetAttribute(%d bytes LDS) failed: %s", DP_LDS, hipGetErrorString(e)); return PACED_ERR_HIP; }
+            attr_set = true;
+        }
+        const int cus = paced_cu_count();
+        hipLaunchKernelGGL(act8_dw_phased_kernel, dim3(total < cus ? total : cus), dim3(512), DP_LDS, s, p, pl.ntm, pl.ntn, total);
+    } else hipLaunchKernelGGL(act8_dw_kernel, dim3(total), dim3(256), DW_NS * DW_STEP, s, p, pl.ntm, pl.ntn, total);
     PACED_CHECK_LAUNCH();
     if (need) {
         hipLaunchKernelGGL(slab_sum_kernel, dim3(flat_blocks((long long)M * (N >> 2))), dim3(256), 0, s, p.out, pl.splits, p.slab, dw, lddw, M, N, accumulate);
