@@ -16,98 +16,106 @@ constexpr int QBLOCK = 32;                 // tokens per scale
 constexpr int MIN_CODE = 127 - 117, MAX_CODE = 127 + 120, NAN_CODE = 255;
 
 // ------------------------------------------------------------------------------------------------ writing and reading
-// One thread per 32 tokens x 8 features: 32 loads of 16 bytes in flight, the maxima in its own registers (integer maxima of
-// the magnitudes' bits, two features to a register), no exchange between lanes.
+// One thread per 32 tokens x 2 W features: 32 loads of 4 W bytes in flight, the maxima in its own registers (integer maxima of
+// the magnitudes' bits, two features to a register), no exchange between lanes.  W = 4 moves 16-byte pieces; where that leaves
+// most compute units without a wave, W = 1 cuts the work of a thread to a quarter.
 typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+template <int W> struct Words;
+template <> struct Words<4> {
+    typedef u32x4 in;
+    typedef u32x2 out;
+    static __device__ __forceinline__ uint32_t get(in v, int j) { return v[j]; }
+    static __device__ __forceinline__ out pack(const uint32_t (&b)[4]) { return out{b[0] | (b[1] << 16), b[2] | (b[3] << 16)}; }
+};
+template <> struct Words<1> {
+    typedef uint32_t in;
+    typedef unsigned short out;
+    static __device__ __forceinline__ uint32_t get(in v, int) { return v; }
+    static __device__ __forceinline__ out pack(const uint32_t (&b)[1]) { return (out)b[0]; }
+};
+template <int W>
 __global__ void __launch_bounds__(256) act8_quantize_kernel(const bf16* __restrict__ x, int ldx, unsigned char* __restrict__ q,
                                                             unsigned char* __restrict__ scale, int T, int n, int nblk) {
-    const int chunks = n >> 3;
+    typedef typename Words<W>::in In;
+    typedef typename Words<W>::out Out;
+    const int chunks = n / (2 * W);
     const long long total = (long long)nblk * chunks;
     for (long long id = (long long)blockIdx.x * 256 + threadIdx.x; id < total; id += (long long)gridDim.x * 256) {
         const int blk = (int)(id / chunks), c = (int)(id - (long long)blk * chunks);
         const int rows = min(QBLOCK, T - blk * QBLOCK);
-        const bf16* src = x + (size_t)blk * QBLOCK * ldx + c * 8;
-        u32x4 v[QBLOCK];
+        const bf16* src = x + (size_t)blk * QBLOCK * ldx + c * 2 * W;
+        In v[QBLOCK];
 #pragma unroll
-        for (int r = 0; r < QBLOCK; ++r) v[r] = r < rows ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + (size_t)r * ldx)) : u32x4{0u, 0u, 0u, 0u};
-        u16x2 top[4] = {};
+        for (int r = 0; r < QBLOCK; ++r) v[r] = r < rows ? __builtin_nontemporal_load(reinterpret_cast<const In*>(src + (size_t)r * ldx)) : In{};
+        u16x2 top[W] = {};
 #pragma unroll
         for (int r = 0; r < QBLOCK; ++r)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) top[j] = __builtin_elementwise_max(top[j], __builtin_bit_cast(u16x2, v[r][j] & 0x7fff7fffu));
-        float inv[8], lim[8];
-        uint32_t bad = 0;                  // bit e: feature e of this thread holds a value that is not finite
-        uint32_t code[2] = {0u, 0u};
+            for (int j = 0; j < W; ++j) top[j] = __builtin_elementwise_max(top[j], __builtin_bit_cast(u16x2, Words<W>::get(v[r], j) & 0x7fff7fffu));
+        float inv[2 * W], lim[2 * W];
+        uint32_t nan[W], code[W];          // codes that make a block NaN, scale bytes: two features to a word
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int bits = top[e >> 1][e & 1];
-            int k = (bits >> 7) - 8 + ((bits & 0x7f) > 0x60 ? 1 : 0);        // 448 = 1.75 * 2^8
-            k = max(k, MIN_CODE);
-            inv[e] = __uint_as_float((uint32_t)(254 - k) << 23);
-            lim[e] = k == MAX_CODE ? 240.f : 448.f;
-            if (bits >= 0x7f80) { bad |= 1u << e; k = NAN_CODE; }
-            code[e >> 2] |= (uint32_t)k << (8 * (e & 3));
+        for (int j = 0; j < W; ++j) {
+            nan[j] = code[j] = 0;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int bits = top[j][e];
+                int k = (bits >> 7) - 8 + ((bits & 0x7f) > 0x60 ? 1 : 0);        // 448 = 1.75 * 2^8
+                k = max(k, MIN_CODE);
+                inv[2 * j + e] = __uint_as_float((uint32_t)(254 - k) << 23);
+                lim[2 * j + e] = k == MAX_CODE ? 240.f : 448.f;
+                if (bits >= 0x7f80) { nan[j] |= 0x7fu << (8 * e); k = NAN_CODE; inv[2 * j + e] = 0.f; }
+                code[j] |= (uint32_t)k << (8 * e);
+            }
         }
-        *reinterpret_cast<u32x2*>(scale + (size_t)blk * n + c * 8) = u32x2{code[0], code[1]};
-        unsigned char* dst = q + (size_t)blk * QBLOCK * n + c * 8;
+        *reinterpret_cast<Out*>(scale + (size_t)blk * n + c * 2 * W) = Words<W>::pack(code);
+        unsigned char* dst = q + (size_t)blk * QBLOCK * n + c * 2 * W;
 #pragma unroll
         for (int r = 0; r < QBLOCK; ++r) {
-            u32x2 o;
+            uint32_t o[W];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float f[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t u = v[r][h * 2 + (e >> 1)];
-                    const float y = __uint_as_float((e & 1) ? (u & 0xffff0000u) : (u << 16)) * inv[h * 4 + e];
-                    f[e] = fminf(fmaxf(y, -lim[h * 4 + e]), lim[h * 4 + e]);
-                }
-                int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
-                w = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], w, true);
-                o[h] = (uint32_t)w;
+            for (int j = 0; j < W; ++j) {
+                const uint32_t u = Words<W>::get(v[r], j);
+                const float lo = __uint_as_float(u << 16) * inv[2 * j], hi = __uint_as_float(u & 0xffff0000u) * inv[2 * j + 1];
+                o[j] = ((uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(__builtin_amdgcn_fmed3f(lo, -lim[2 * j], lim[2 * j]),
+                                                                   __builtin_amdgcn_fmed3f(hi, -lim[2 * j + 1], lim[2 * j + 1]), 0, false) & 0xffffu) | nan[j];
             }
-            if (bad) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if ((bad >> e) & 1u) o[e >> 2] |= 0x7fu << (8 * (e & 3));
-            }
-            if (r < rows) __builtin_nontemporal_store(o, reinterpret_cast<u32x2*>(dst + (size_t)r * n));
+            if (r < rows) __builtin_nontemporal_store(Words<W>::pack(o), reinterpret_cast<Out*>(dst + (size_t)r * n));
         }
     }
 }
 
-// One thread per 8 tokens x 16 features.
+// One thread per 16 tokens x 8 features: a wave stores whole 1 KiB runs (16 features to a thread, two 16-byte stores 32 bytes
+// apart: 84 us against 139264 x 768).
+constexpr int DQ_ROWS = 16;
 __global__ void __launch_bounds__(256) act8_dequantize_kernel(const unsigned char* __restrict__ q, const unsigned char* __restrict__ scale,
                                                               bf16* __restrict__ y, int ldy, int T, int n) {
-    const int chunks = n >> 4;
-    const long long total = (long long)((T + 7) >> 3) * chunks;
+    const int chunks = n >> 3;
+    const long long total = (long long)((T + DQ_ROWS - 1) / DQ_ROWS) * chunks;
     for (long long id = (long long)blockIdx.x * 256 + threadIdx.x; id < total; id += (long long)gridDim.x * 256) {
-        const int t8 = (int)(id / chunks), c = (int)(id - (long long)t8 * chunks);
-        const int rows = min(8, T - t8 * 8);
-        u32x4 v[8];
+        const int tb = (int)(id / chunks), c = (int)(id - (long long)tb * chunks);
+        const int rows = min(DQ_ROWS, T - tb * DQ_ROWS);
+        const unsigned char* src = q + (size_t)tb * DQ_ROWS * n + c * 8;
+        u32x2 v[DQ_ROWS];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) v[r] = r < rows ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(q + (size_t)(t8 * 8 + r) * n + c * 16)) : u32x4{0u, 0u, 0u, 0u};
-        const u32x4 s = *reinterpret_cast<const u32x4*>(scale + (size_t)(t8 >> 2) * n + c * 16);
-        float f[16];
+        for (int r = 0; r < DQ_ROWS; ++r) v[r] = r < rows ? __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(src + (size_t)r * n)) : u32x2{0u, 0u};
+        const u32x2 s = *reinterpret_cast<const u32x2*>(scale + (size_t)(tb / (QBLOCK / DQ_ROWS)) * n + c * 8);
+        float f[8];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(((s[e >> 2] >> (8 * (e & 3))) & 0xffu) << 23);
+        for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(((s[e >> 2] >> (8 * (e & 3))) & 0xffu) << 23);
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            u32x4 o[2];
+        for (int r = 0; r < DQ_ROWS; ++r) {
+            u32x4 o;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
+            for (int w = 0; w < 2; ++w) {
                 const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)v[r][w], false);
                 const auto b = __builtin_amdgcn_cvt_pk_f32_fp8((int)v[r][w], true);
                 const bf16x2 lo = {f2bf(a[0] * f[4 * w]), f2bf(a[1] * f[4 * w + 1])};
                 const bf16x2 hi = {f2bf(b[0] * f[4 * w + 2]), f2bf(b[1] * f[4 * w + 3])};
-                o[w >> 1][(w & 1) * 2] = __builtin_bit_cast(uint32_t, lo);
-                o[w >> 1][(w & 1) * 2 + 1] = __builtin_bit_cast(uint32_t, hi);
+                o[2 * w] = __builtin_bit_cast(uint32_t, lo);
+                o[2 * w + 1] = __builtin_bit_cast(uint32_t, hi);
             }
-            if (r < rows) {
-                bf16* dst = y + (size_t)(t8 * 8 + r) * ldy + c * 16;
-                __builtin_nontemporal_store(o[0], reinterpret_cast<u32x4*>(dst));
-                __builtin_nontemporal_store(o[1], reinterpret_cast<u32x4*>(dst + 8));
-            }
+            if (r < rows) __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(y + (size_t)(tb * DQ_ROWS + r) * ldy + c * 8));
         }
     }
 }
@@ -483,7 +491,7 @@ DwPlan dw_plan(int T, int M, int N) {
         pl.tile = 64;
         pl.ntm = (M + 63) / 64;
         pl.ntn = (N + 63) / 64;
-        splits = t64 >= 3LL * cus ? 1 : 3LL * cus / t64;
+        splits = t64 >= 3LL * cus || (t64 * 4 >= cus * 3 && ktiles <= 24) ? 1 : 3LL * cus / t64;       // (few tokens: the slabs would cost more than they save)
         if (splits > (ktiles + 3) / 4) splits = (ktiles + 3) / 4;
     }
     const int per = (int)((ktiles + splits - 1) / splits);
@@ -506,8 +514,13 @@ extern "C" int paced_act8_quantize(const void* x, int ldx, void* q, void* scale,
     PACED_CHECK_ARG(ldx >= n && ldx % 8 == 0 && (((uintptr_t)x | (uintptr_t)q | (uintptr_t)scale) & 15) == 0,
                     "paced_act8_quantize: 16-byte aligned operands and a row stride of at least n and a multiple of 8 are needed (ldx=%d)", ldx);
     const int nblk = (T + QBLOCK - 1) / QBLOCK;
-    hipLaunchKernelGGL(act8_quantize_kernel, dim3(flat_blocks((long long)nblk * (n >> 3))), dim3(256), 0, (hipStream_t)stream,
-                       (const bf16*)x, ldx, (unsigned char*)q, (unsigned char*)scale, T, n, nblk);
+    const long long wide = (long long)nblk * (n >> 3);
+    if (wide >= 256LL * paced_cu_count())
+        hipLaunchKernelGGL(act8_quantize_kernel<4>, dim3(flat_blocks(wide)), dim3(256), 0, (hipStream_t)stream,
+                           (const bf16*)x, ldx, (unsigned char*)q, (unsigned char*)scale, T, n, nblk);
+    else
+        hipLaunchKernelGGL(act8_quantize_kernel<1>, dim3(flat_blocks(wide * 4)), dim3(256), 0, (hipStream_t)stream,
+                           (const bf16*)x, ldx, (unsigned char*)q, (unsigned char*)scale, T, n, nblk);
     PACED_CHECK_LAUNCH();
     return PACED_OK;
 }
@@ -518,7 +531,7 @@ extern "C" int paced_act8_dequantize(const void* q, const void* scale, void* y, 
     PACED_CHECK_ARG(q && scale && y, "paced_act8_dequantize: null operand");
     PACED_CHECK_ARG(ldy >= n && ldy % 8 == 0 && (((uintptr_t)y | (uintptr_t)q | (uintptr_t)scale) & 15) == 0,
                     "paced_act8_dequantize: 16-byte aligned operands and a row stride of at least n and a multiple of 8 are needed (ldy=%d)", ldy);
-    hipLaunchKernelGGL(act8_dequantize_kernel, dim3(flat_blocks((long long)((T + 7) / 8) * (n >> 4))), dim3(256), 0, (hipStream_t)stream,
+    hipLaunchKernelGGL(act8_dequantize_kernel, dim3(flat_blocks((long long)((T + DQ_ROWS - 1) / DQ_ROWS) * (n >> 3))), dim3(256), 0, (hipStream_t)stream,
                        (const unsigned char*)q, (const unsigned char*)scale, (bf16*)y, ldy, T, n);
     PACED_CHECK_LAUNCH();
     return PACED_OK;

@@ -54,6 +54,7 @@ struct GemmParams {
     long long ce_ignore;
     int ce_vocab, ce_first;       // vocabulary size, entry of column 0
     int accumulate;               // EPI_SLAB_F32: add to what is there
+    int tile;                     // tile edge the caller has chosen (0: the launch's own rule; paced_gemm_set_tile overrides)
 };
 
 // Order-preserving 64-bit key: larger key <=> (higher score, then lower pool row).

@@ -83,6 +83,24 @@ __device__ __forceinline__ void ce_columns(const GemmParams& p, int m0, int wm, 
     }
 }
 
+// ... and their log-sum-exps (base 2) and weights
+template <class Cfg>
+__device__ __forceinline__ void ce_rows(const GemmParams& p, int m0, int wm, int lane, int (&col)[Cfg::MI], bool (&dead)[Cfg::MI],
+                                        float (&lse2)[Cfg::MI], float (&g)[Cfg::MI]) {
+    ce_columns<Cfg>(p, m0, wm, lane, col, dead);
+    const float *srcl[Cfg::MI], *srcg[Cfg::MI];
+#pragma unroll
+    for (int i = 0; i < Cfg::MI; ++i) {
+        const int mc = min(m0 + Cfg::moff(wm, i) + (lane & 15), p.M - 1);
+        srcl[i] = p.ce_lse + mc;
+        srcg[i] = p.ce_g + mc;
+    }
+    ce_load_rows<Cfg::MI>(srcl, lse2);
+    ce_load_rows<Cfg::MI>(srcg, g);
+#pragma unroll
+    for (int i = 0; i < Cfg::MI; ++i) lse2[i] *= CE_LOG2E;
+}
+
 // gradient of four consecutive columns n .. n + 3 of a row: g (2^(z - lse2) - [label])
 __device__ __forceinline__ f32x4 ce_grad4(const GemmParams& p, const f32x4& a, float c, float lse2, float g, int col, bool dead, int n) {
     f32x4 o;
@@ -374,17 +392,8 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, void* Cb, int m0, 
     if (EPI == EPI_CE_GRAD) {
         int col[MI];
         bool dead[MI];
-        ce_columns<Cfg>(p, m0, wm, lane, col, dead);
-        const float *srcl[MI], *srcg[MI];
-        float lse[MI], g[MI];
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            const int mc = min(m0 + Cfg::moff(wm, i) + (lane & 15), p.M - 1);
-            srcl[i] = p.ce_lse + mc;
-            srcg[i] = p.ce_g + mc;
-        }
-        ce_load_rows<MI>(srcl, lse);
-        ce_load_rows<MI>(srcg, g);
+        float lse2[MI], g[MI];
+        ce_rows<Cfg>(p, m0, wm, lane, col, dead, lse2, g);
         const float c = p.alpha * CE_LOG2E;
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
@@ -394,7 +403,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, void* Cb, int m0, 
             for (int j = 0; j < NJ; ++j) {
                 const int n = n0 + Cfg::noff(wn, j) + (lane >> 4) * 4;
                 if (n >= ((p.N + 63) & ~63)) continue;
-                const f32x4 o = ce_grad4(p, acc[i][j], c, lse[i] * CE_LOG2E, g[i], col[i], dead[i], n);
+                const f32x4 o = ce_grad4(p, acc[i][j], c, lse2[i], g[i], col[i], dead[i], n);
                 *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16*>(Cb) + (size_t)m * p.ldc + n) = __builtin_convertvector(o, bf16x4);
             }
         }
@@ -672,7 +681,8 @@ __device__ __forceinline__ void epilogue_rows_impl(const GemmParams& p, void* Cb
     if (TILED && EPI == EPI_RELU_DROP) tbits = u32x4{0u, 0u, 0u, 0u};
     const int rr = lane >> 3, c = lane & 7;
     const int ncol = n0 + wc * 64 + c * 8;
-    const bool col_ok = FULL || ncol < p.N;           // N is a multiple of 8 on this path
+    // N is a multiple of 8 on this path, but for the cross entropy's gradient, whose rows are stored up to a multiple of 64
+    const bool col_ok = FULL || ncol < (EPI == EPI_CE_GRAD ? (p.N + 63) & ~63 : p.N);
     uint32_t mbits[8];
     bf16x8 aux[8];
     auto load_piece = [&](int n) {
@@ -702,6 +712,10 @@ __device__ __forceinline__ void epilogue_rows_impl(const GemmParams& p, void* Cb
     const int wsw = ((mw & 7) << 1) | (mw >> 3);
     const int woff = (mw & 7) * 128;
     const int roff = rr * 128 + ((c ^ rr) << 4);
+    int ccol[8];
+    bool cdead[8];
+    float clse[8], cg[8];
+    if (EPI == EPI_CE_GRAD) ce_rows<CfgPhased>(p, m0, wr, lane, ccol, cdead, clse, cg);
     const bool has_drop = (EPI == EPI_RES_DROP || EPI == EPI_RELU_DROP) && p.drop.thresh != 0;
     const float scale = (EPI == EPI_MASK || EPI == EPI_MASK_BITS) ? p.alpha * p.mask_scale : p.alpha;
 
@@ -711,6 +725,10 @@ __device__ __forceinline__ void epilogue_rows_impl(const GemmParams& p, void* Cb
         const uint32_t qrow = (uint32_t)(drow >> 2);          // quad number: the host sends outputs of more than 2^34 elements elsewhere
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            if (EPI == EPI_CE_GRAD) {
+                o[j] = __builtin_convertvector(ce_grad4(p, acc[i][j], p.alpha * CE_LOG2E, clse[i], cg[i], ccol[i], cdead[i], n0 + wc * 64 + j * 16 + g * 4), bf16x4);
+                continue;
+            }
             f32x4 v = acc[i][j] * scale;
             if (EPI == EPI_RELU_DROP) v = __builtin_elementwise_max(v, f32x4{0.f, 0.f, 0.f, 0.f});
             if (has_drop) {
@@ -769,6 +787,8 @@ __device__ __forceinline__ void epilogue_rows_impl(const GemmParams& p, void* Cb
         }
         if (EPI == EPI_BF16 && p.c_heads) {        // a wave's 64 columns are one head: rows of 128 bytes, 128 bytes apart
             if (ok) st_out(reinterpret_cast<bf16x8*>(reinterpret_cast<bf16*>(Cb) + (size_t)(ncol >> 6) * p.c_heads + (size_t)m * 64 + (ncol & 63)), t);
+        } else if (EPI == EPI_CE_GRAD) {           // read again by the next two launches: an ordinary store
+            if (ok) *reinterpret_cast<bf16x8*>(reinterpret_cast<bf16*>(Cb) + (size_t)m * p.ldc + ncol) = t;
         } else if (ok) st_out(reinterpret_cast<bf16x8*>(reinterpret_cast<bf16*>(Cb) + (size_t)m * p.ldc + ncol), t);
         if (LOADS && n < 8) {
             if (FULL) load_piece(n + 8);
@@ -944,7 +964,7 @@ __global__ void __launch_bounds__(512) gemm_phased_kernel(GemmParams p, int ntm,
         // run their epilogues side by side; otherwise that barrier is met by this group's first barrier of the next
         // item, and each group sits idle through the other's whole epilogue.
         if (wr == 0) __builtin_amdgcn_s_barrier();
-        if (EPI == EPI_BF16 || EPI == EPI_RES_DROP || EPI == EPI_RELU_DROP || EPI == EPI_MASK || EPI == EPI_MASK_BITS) {
+        if (EPI == EPI_BF16 || EPI == EPI_RES_DROP || EPI == EPI_RELU_DROP || EPI == EPI_MASK || EPI == EPI_MASK_BITS || EPI == EPI_CE_GRAD) {
             char* s1 = sw + ring_wrap(base + 8) * HALF;      // the finished K step's B half 1 and A half 1 slots
             char* s2 = sw + ring_wrap(base + 9) * HALF;
             // (the host refuses a tile-ordered mask with fewer than two K steps, so the loop's waits have covered the load)
@@ -1356,7 +1376,7 @@ int launch_cfg(GemmParams p, int splits, hipStream_t stream) {
 
 template <bool TA, bool TB, int EPI>
 int launch(const GemmParams& p, int splits, hipStream_t stream) {
-    const int force_tile = eff_tile();
+    const int force_tile = eff_tile() ? eff_tile() : p.tile;
     if (EPI == EPI_ATOMIC_F32 && splits <= 0 && force_tile == 0 && ring_enabled()) {
         // Short contraction into a mid-sized output (the decoder's weight gradients): the launch is bound by the
         // output, every split adds the whole output once more in atomics, and a big tile leaves CUs empty; take
@@ -1371,7 +1391,7 @@ int launch(const GemmParams& p, int splits, hipStream_t stream) {
     else {
         // the 256x256 tile pays off once there is about one tile per CU (split slices count for atomics)
         const long long t256 = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256) * p.batch;
-        large = p.M >= 256 && p.N >= 256 && (t256 >= 200 || (EPI == EPI_ATOMIC_F32 && t256 >= 9) || (EPI == EPI_SLAB_F32 && t256 * splits >= 128));
+        large = p.M >= 256 && p.N >= 256 && (t256 >= 200 || (EPI == EPI_ATOMIC_F32 && t256 >= 9));
     }
     // the phased kernel moves bf16 outputs (and their residual / mask operand) in 16-byte row pieces
     const bool rows16 = (EPI == EPI_F32 || EPI == EPI_ATOMIC_F32 || EPI == EPI_TOPK_DENSE || EPI == EPI_TOPK_FILTER ||

@@ -30,7 +30,15 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const f32x2* __restrict__ 
     const int r = threadIdx.x & 7, k = threadIdx.x >> 3;
     const int row = blockIdx.x * 8 + r, rr = min(row, R - 1);
     float m = -INFINITY, s = 0.f;
-    for (int g = k; g < groups; g += 32) {
+    int g = k;
+    for (; g + 7 * 32 < groups; g += 8 * 32) {        // eight loads in flight
+        f32x2 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = part[(size_t)(g + i * 32) * R + rr];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) join(m, s, v[i][0], v[i][1]);
+    }
+    for (; g < groups; g += 32) {
         const f32x2 v = part[(size_t)g * R + rr];
         join(m, s, v[0], v[1]);
     }
@@ -82,9 +90,28 @@ int blocks_for(long long items) {
 
 size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// Pieces of the vocabulary, and slices of a piece for dh.  A piece's P takes at most 256 MiB; a launch of dh's product should
-// give every compute unit a tile (256x256 tiles where the output has them, else 64x64), a slice has four K steps or more.
-struct CePlan { int piece, ldp, slabs; };
+// Microseconds of a product of M x N tiles of edge `tile` over `steps` K steps of 64, from what the kernels of gemm.hip reach:
+// a 256x256 step 1.75 (1.2 PFLOP/s over the chip) and 8 to fill and drain a tile's ring; 128x128 and 64x64 tiles run three to a
+// compute unit and give it a step in 0.75 and 0.3.  Good to about a fifth: it only chooses between tiles and slices.
+double product_us(int tile, int M, int N, int slices, int steps) {
+    const long long items = (long long)((M + tile - 1) / tile) * ((N + tile - 1) / tile) * slices, cus = paced_cu_count();
+    const double rounds = (double)((items + cus - 1) / cus), per = (double)((steps + slices - 1) / slices);
+    return tile == 256 ? rounds * (per * 1.75 + 8.) : tile == 128 ? rounds * per * 0.75 + 6. : rounds * per * 0.3 + 6.;
+}
+int best_tile(int M, int N, int steps) {
+    double best = 1e30;
+    int tile = 64;
+    for (int t = 256; t >= 64; t /= 2) {
+        if (t == 256 && (M < 256 || N < 256)) continue;
+        const double us = product_us(t, M, N, 1, steps);
+        if (us < best) { best = us; tile = t; }
+    }
+    return tile;
+}
+
+// Pieces of the vocabulary, tiles, and slices of a piece for dh.  A piece's P takes at most 256 MiB.  More slices give dh's
+// product more workgroups and its second kernel more slabs to add (written and read at about 4 TB/s).
+struct CePlan { int piece, ldp, slabs, dh_tile; };
 CePlan ce_plan(int R, int V, int d) {
     CePlan pl;
     long long fit = (256ll << 20) / 2 / (R > 0 ? R : 1) / 256 * 256;
@@ -94,13 +121,19 @@ CePlan ce_plan(int R, int V, int d) {
     if (piece > V) piece = V;
     pl.piece = (int)piece;
     pl.ldp = (int)((piece + 63) / 64 * 64);
-    const int ksteps = (pl.piece + 63) / 64, cus = paced_cu_count();
-    const long long big = (long long)((R + 255) / 256) * ((d + 255) / 256), tiny = (long long)((R + 63) / 64) * ((d + 63) / 64);
-    long long want = R >= 256 && d >= 256 ? cus / big : 2ll * cus / tiny;
-    if (want > ksteps / 4) want = ksteps / 4;
-    if (want < 1) want = 1;
-    const int per = (int)((ksteps + want - 1) / want);
-    pl.slabs = (ksteps + per - 1) / per;
+    const int steps = (pl.piece + 63) / 64;
+    double best = 1e30;
+    pl.slabs = 1;
+    pl.dh_tile = 64;
+    for (int t = 256; t >= 64; t /= 2) {
+        if (t == 256 && (R < 256 || d < 256)) continue;
+        for (int s = 1; s <= 64 && s * 3 <= steps + 2; ++s) {
+            const double us = product_us(t, R, d, s, steps) + (double)s * R * d * 8. / 4e6;
+            if (us < best) { best = us; pl.slabs = s; pl.dh_tile = t; }
+        }
+    }
+    const int per = (steps + pl.slabs - 1) / pl.slabs;
+    pl.slabs = (steps + per - 1) / per;
     return pl;
 }
 
@@ -191,11 +224,13 @@ extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ld
             p = product(P, pl.ldp, wp, ldw, slabs, d, R, d, n, scale);
             p.strideC = (long long)R * d;
             p.accumulate = v0 > 0;
+            p.tile = pl.dh_tile;
             if ((r = paced_gemm_launch(p, false, true, EPI_SLAB_F32, pl.slabs, s)) != PACED_OK) return r;
         }
         if (dw) {
             p = product(P, pl.ldp, h, ldh, dw_f32 ? (void*)((float*)dw + (size_t)v0 * lddw) : (void*)((bf16*)dw + (size_t)v0 * lddw), lddw, n, d, R, scale);
             p.accumulate = 1;
+            p.tile = best_tile(n, d, (R + 63) / 64);
             if ((r = paced_gemm_launch(p, true, true, dw_f32 ? EPI_SLAB_F32 : EPI_BF16, 1, s)) != PACED_OK) return r;
         }
     }
