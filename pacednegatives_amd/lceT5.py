@@ -291,6 +291,11 @@ class LCEModel:
         if self.memory_limit_bytes is None and os.environ.get("PACED_MEMORY_LIMIT"):
             self.memory_limit_bytes = int(os.environ["PACED_MEMORY_LIMIT"])
         self.ran_ahead = False                 # whether the last training_step returned before its backward pass was over
+        # the LM head's cross entropy and its gradients without the [rows, vocabulary] logits (kernels.linear_ce_fwd / _bwd)
+        self.fused_loss = bool(self.hparams.get("fused_loss", os.environ.get("PACED_FUSED_LOSS", "0") != "0"))
+        # 8-bit checkpoints of the encoder's saved activations (T5Engine.act8)
+        if self.hparams.get("act8", None) is not None:
+            self.model.engine.act8 = bool(self.hparams.act8)
         self._side_stream = self._aux_stream = None
         self._host_vals = None                 # pinned: what a step hands to the host (statistics, eta, mean main loss)
         self.difficulty = float(self.weights.eta.item())
@@ -353,22 +358,25 @@ class LCEModel:
 
     # ---- the step
     def _forward_pair(self, p, n, save, call, after_encoder=None, gemm_grid=0):
-        """Run the positive and negative batches; one packed call when their lengths agree."""
+        """Run the positive and negative batches; one packed call when their lengths agree.  Returns the states and the
+        positives' and negatives' logits, or with ``fused_loss`` the LM head's inputs in their place."""
         eng = self.model.engine
+        fused = self.fused_loss
         # every rank draws its own masks, as the independent RNG streams of DDP ranks do in the reference
         seed = (self._base_seed * 0x9E3779B1 + parallel.rank() * 0x632BE5AB + self.global_step * 8 + call) & 0xFFFFFFFF
         B = p["input_ids"].shape[0]
         if p["input_ids"].shape[1] == n["input_ids"].shape[1]:
             ids = torch.cat([p["input_ids"].to(self.device), n["input_ids"].to(self.device)], 0)
             lab = torch.cat([p["labels"].to(self.device), n["labels"].to(self.device)], 0)
-            st = eng.forward(ids, lab, save=save, drop_p=self.dropout, seed=seed, after_encoder=after_encoder,
+            st = eng.forward(ids, lab, save=save, drop_p=self.dropout, seed=seed, after_encoder=after_encoder, want_logits=not fused,
                              gemm_grid=gemm_grid, gemm_grid_layers=self.nograd_grid_layers)
-            return [st], st.logits[:2 * B], st.logits[2 * B:]
-        sp = eng.forward(p["input_ids"], p["labels"], save=save, drop_p=self.dropout, seed=seed,
+            out = st.y if fused else st.logits
+            return [st], out[:2 * B], out[2 * B:]
+        sp = eng.forward(p["input_ids"], p["labels"], save=save, drop_p=self.dropout, seed=seed, want_logits=not fused,
                          gemm_grid=gemm_grid, gemm_grid_layers=self.nograd_grid_layers)
-        sn = eng.forward(n["input_ids"], n["labels"], save=save, drop_p=self.dropout, seed=seed ^ 0x55555555, after_encoder=after_encoder,
+        sn = eng.forward(n["input_ids"], n["labels"], save=save, drop_p=self.dropout, seed=seed ^ 0x55555555, after_encoder=after_encoder, want_logits=not fused,
                          gemm_grid=gemm_grid, gemm_grid_layers=self.nograd_grid_layers)
-        return [sp, sn], sp.logits, sn.logits
+        return [sp, sn], (sp.y if fused else sp.logits), (sn.y if fused else sn.logits)
 
     def training_step(self, batch, batch_nb):
         """Reference ``lceT5.py:125-168``, in the same order."""
@@ -384,6 +392,7 @@ class LCEModel:
         plab = p["labels"].to(self.device, torch.int64).contiguous().view(-1)
         nlab = n["labels"].to(self.device, torch.int64).contiguous().view(-1)
         ign = int(hp.ignore_index)
+        head = self.model.params.w("shared")
 
         # Nothing in (d) -- the forwards that keep state, the main loss, its backward -- depends on (a) or on eta, and
         # (a) only feeds eta's meta update and the log.  So (a) runs on a second stream, started when (d)'s encoder
@@ -412,8 +421,12 @@ class LCEModel:
             states, plog, nlog = self._forward_pair(p, n, save=False, call=0, gemm_grid=gemm_grid)
             pce = torch.empty(2 * B, dtype=F32, device=self.device)
             nce = torch.empty(2 * B * nneg, dtype=F32, device=self.device)
-            K.cross_entropy(plog, plab, pce, None, ignore_index=ign)
-            K.cross_entropy(nlog, nlab, nce, None, ignore_index=ign)
+            if self.fused_loss:
+                K.linear_ce_fwd(plog, head, plab, pce, ignore_index=ign)
+                K.linear_ce_fwd(nlog, head, nlab, nce, ignore_index=ign)
+            else:
+                K.cross_entropy(plog, plab, pce, None, ignore_index=ign)
+                K.cross_entropy(nlog, nlab, nce, None, ignore_index=ign)
             rows = torch.empty(2 * B, dtype=F32, device=self.device)
             K.lce_group(pce, nce, rows, nneg, use_mean)
             return rows
@@ -434,7 +447,25 @@ class LCEModel:
             pce2 = torch.empty(2 * B, dtype=F32, device=self.device)
             nce2 = torch.empty(2 * B * nneg, dtype=F32, device=self.device)
             rows = torch.empty(2 * B, dtype=F32, device=self.device)
-            if len(states) == 1:
+            if self.fused_loss:
+                # each state's rows in one call: the positives' and the negatives' weights differ, not the arithmetic
+                lab = [torch.cat([plab, nlab])] if len(states) == 1 else [plab, nlab]
+                ce, lses = torch.empty(2 * B * (1 + nneg), dtype=F32, device=self.device), []
+                weight = torch.full_like(ce, g_pos)
+                weight[2 * B:] = g_neg
+                cuts = [slice(0, 2 * B * (1 + nneg))] if len(states) == 1 else [slice(0, 2 * B), slice(2 * B, 2 * B * (1 + nneg))]
+                for st, l, c in zip(states, lab, cuts):
+                    lses.append(torch.empty_like(ce[c]))
+                    K.linear_ce_fwd(st.y, head, l, ce[c], lses[-1], ignore_index=ign)
+                K.lce_group(ce[:2 * B], ce[2 * B:], rows, nneg, use_mean)
+                if on_rows is not None:
+                    on_rows(rows)
+                for k, (st, l, c) in enumerate(zip(states, lab, cuts)):
+                    dy = torch.empty_like(st.y)
+                    K.linear_ce_bwd(st.y, head, l, lses[k], weight[c], dy, self.model.params.grad("shared"), ignore_index=ign)
+                    last = k == len(states) - 1                 # the last pass over the gradients
+                    self.model.engine.backward(st, dy=dy, on_segments_done=on_segments_done if last else None)
+            elif len(states) == 1:
                 dl = torch.empty(states[0].logits.shape, dtype=BF16, device=self.device)
                 K.cross_entropy(plog, plab, pce2, dl[:2 * B], ignore_index=ign, gscale=g_pos)
                 K.cross_entropy(nlog, nlab, nce2, dl[2 * B:], ignore_index=ign, gscale=g_neg)

@@ -133,6 +133,9 @@ class T5Engine:
         self.dw_stream = None                  # when set: weight-gradient products of backward() run on this stream
         self.ffn_bit_mask = os.environ.get("PACED_FFN_BITMASK", "1") != "0"   # encoder FFN backward masks by saved sign bits
         self.head_major = os.environ.get("PACED_HEAD_MAJOR", "1") != "0"   # encoder attention operands head-major (see forward)
+        # the encoder's saved normalised states and feed-forward activations, which only weight gradients read, kept as 8-bit
+        # checkpoints (kernels.act8_quantize): 6 of the 24 d_model-wide bf16 rows an encoder layer keeps shrink to half
+        self.act8 = os.environ.get("PACED_ACT8", "0") != "0"
         self._bucket_dec = torch.tensor([0, 1], dtype=torch.int32, device=self.device)   # offsets 0 and -1 (HF:244-249)
         dec_b = relative_position_bucket(torch.tensor([0, -1]), False, dims.num_buckets, dims.max_distance)
         assert dec_b.tolist() == [0, 1]
@@ -177,13 +180,20 @@ class T5Engine:
         return t[:, :I], t[:, I:2 * I], t[:, 2 * I:]
 
     def _dweight(self, dy, x, name, rows: Optional[slice] = None):
-        """grad[name] (+)= dy^T x  -- dy [M, out], x [M, in] -> [out, in], fp32 atomics."""
+        """grad[name] (+)= dy^T x  -- dy [M, out], x [M, in] -> [out, in], fp32 atomics; x may be an 8-bit checkpoint
+        (codes, scales) of [M, in] (fp32 sums in a fixed order)."""
         g = self.params.grad(name)
         if rows is not None:
             g = g[rows]
+
+        def product():
+            if isinstance(x, tuple):
+                K.act8_dweight(dy, x[0], x[1], g)
+            else:
+                K.gemm(dy, x, g, trans_a=True, trans_b=True, epilogue=K.EPI_ATOMIC_F32, splits=0)   # 0: library picks the split
         side = self.dw_stream
         if side is None:
-            K.gemm(dy, x, g, trans_a=True, trans_b=True, epilogue=K.EPI_ATOMIC_F32, splits=0)   # 0: library picks the split
+            product()
             return
         # Nothing in the backward chain reads a weight gradient, so the product runs on a second stream and its
         # workgroups fill the CUs that the chain's kernel tails leave idle.  Both operands are complete once the
@@ -192,9 +202,10 @@ class T5Engine:
         main = torch.cuda.current_stream()
         side.wait_stream(main)
         with torch.cuda.stream(side):
-            K.gemm(dy, x, g, trans_a=True, trans_b=True, epilogue=K.EPI_ATOMIC_F32, splits=0)
+            product()
         dy.record_stream(side)
-        x.record_stream(side)
+        for t in x if isinstance(x, tuple) else (x,):
+            t.record_stream(side)
 
     # ------------------------------------------------------------------ forward
     def forward(self, input_ids: torch.Tensor, labels: torch.Tensor, *, save: bool, drop_p: float = 0.0, seed: int = 0,
@@ -260,6 +271,10 @@ class T5Engine:
             if save:
                 sv.h_in, sv.xn, sv.rstd1, sv.qkv, sv.ctx, sv.lse = h, xn, rstd1, qkv, ctx, lse
                 sv.h_mid, sv.xn2, sv.rstd2, sv.act, sv.actbits = h_mid, xn2, rstd2, act, actbits
+                if self.act8:
+                    sv.xn, sv.xn2 = K.act8_quantize(xn), K.act8_quantize(xn2)
+                    if actbits is not None:        # (without the sign bits the backward pass masks by the activations themselves)
+                        sv.act = K.act8_quantize(act)
                 st.enc_layers.append(sv)
             h = h_out
         enc = self._empty(M, d)
@@ -338,9 +353,10 @@ class T5Engine:
         return st
 
     # ------------------------------------------------------------------ backward
-    def backward(self, st: ForwardState, dlogits: torch.Tensor, on_segments_done=None) -> None:
+    def backward(self, st: ForwardState, dlogits: torch.Tensor = None, on_segments_done=None, dy: torch.Tensor = None) -> None:
         """Accumulate parameter gradients of one forward call into ``params.g32`` given d loss / d logits
-        (bf16 [N*2, V]).  The forward must have been run with ``save=True``.
+        (bf16 [N*2, V]), or given d loss / d y (bf16 [N*2, d_model], y = the head's input ``st.y``) when the caller has
+        done the LM head's backward itself (``kernels.linear_ce_bwd``).  The forward must have been run with ``save=True``.
 
         ``on_segments_done(first, last)``, if given, is called when every kernel that writes the gradients of the
         layout segments first .. last, or reads their weights, has been enqueued (on the calling stream and on
@@ -353,13 +369,18 @@ class T5Engine:
         d, I, ff, H = dims.d_model, dims.inner, dims.d_ff, dims.num_heads
         M, Md = N * S, N * 2
         scale = 1.0 / (1.0 - p) if p > 0 else 1.0
-        if tuple(dlogits.shape) != (Md, dims.vocab_size):
+        if (dlogits is None) == (dy is None):
+            raise ValueError("backward takes either dlogits or dy")
+        if dlogits is not None and tuple(dlogits.shape) != (Md, dims.vocab_size):
             raise ValueError("dlogits has the wrong shape")
+        if dy is not None and tuple(dy.shape) != (Md, d):
+            raise ValueError("dy has the wrong shape")
 
         # ---- LM head (tied with the embedding)
-        self._dweight(dlogits, st.y, "shared")
-        dy = self._empty(Md, d)
-        K.gemm(dlogits, P.w("shared"), dy, trans_b=True)
+        if dy is None:
+            self._dweight(dlogits, st.y, "shared")
+            dy = self._empty(Md, d)
+            K.gemm(dlogits, P.w("shared"), dy, trans_b=True)
 
         # ---- decoder
         nd = dims.num_decoder_layers

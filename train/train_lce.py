@@ -5,7 +5,8 @@ hyper-parameter arithmetic (``total_steps//batch_size``, ``warmup_steps//batch_s
 same sequence (model, data module, trainer with ChangeDifficulty, fit, save to out_dir/finalmodel;
 ``:66-103``).  Additions: ``--model_name`` (a size name or a local Hugging Face checkpoint directory;
 names cannot be downloaded here) and ``--synthetic N`` (build an N-record synthetic corpus and
-negatives file in out_dir instead of reading ``--data`` / ``--dataset_name``).
+negatives file in out_dir instead of reading ``--data`` / ``--dataset_name``), ``--fused_loss`` and ``--act8`` (memory
+for time: no [rows, vocabulary] logits, and 8-bit copies of what the weight gradients read).
 
 Multi-GPU: ``--num_gpus N`` alone is enough, as for the reference (whose Lightning trainer starts one process per
 device, ``train_lce.py:89-94``): run without a torchrun environment, the script starts N rank processes of itself
@@ -29,7 +30,8 @@ def _bool(v):
 def main(data: str, dataset_name: str, out_dir: str, total_steps: int = 100000, eta: float = 0.0, batch_size: int = 16,
          lr: float = 0.001, meta_lr=None, var: float = 0.01, n: int = 2, use_max: bool = False, warmup_steps: int = 10000,
          sample: bool = False, use_mean: bool = False, num_gpus: int = 1, wandb_project: str = None, num_workers: int = 8,
-         max_steps: int = None, model_name: str = "t5-base", synthetic: int = 0, dropout: float = None, seed: int = 0):
+         max_steps: int = None, model_name: str = "t5-base", synthetic: int = 0, dropout: float = None, seed: int = 0,
+         fused_loss: bool = False, act8: bool = False):
     from pacednegatives_amd.lceT5 import ChangeDifficulty, LCEDataModule, LCEModel
     from pacednegatives_amd.trainer import JSONLLogger, Trainer, init_distributed
     from pacednegatives_amd import synthetic as syn
@@ -53,6 +55,10 @@ def main(data: str, dataset_name: str, out_dir: str, total_steps: int = 100000, 
         "dropout": dropout,
         "seed": seed,
     }
+    if fused_loss:
+        args["fused_loss"] = True
+    if act8:
+        args["act8"] = True
     model = LCEModel(args)
     corpus = dataset_name
     if synthetic:
@@ -108,6 +114,8 @@ if __name__ == "__main__":
     ap.add_argument("--synthetic", type=int, default=0)
     ap.add_argument("--dropout", type=float, default=None)
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--fused_loss", action="store_true", help="LM-head loss and gradients without storing the logits")
+    ap.add_argument("--act8", action="store_true", help="keep the encoder's weight-gradient inputs as 8-bit checkpoints")
     a = ap.parse_args()
     if not a.synthetic and not (a.data and a.dataset_name):
         ap.error("--data and --dataset_name are required unless --synthetic N is given")
