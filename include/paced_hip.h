@@ -157,8 +157,7 @@ int paced_rmsnorm_bwd(const void* dy, const void* x, const void* w, const float*
 /* ---- layer norm (mean and variance), with a residual sum in front of it ---------------------------
  * No counterpart in the reference's T5; the norm of the encoders that dense retrieval and BERT-like rankers use.
  * f32 = 0: x, res, xsum, w, b, y, dy, dres, dx are bf16; f32 = 1: fp32.  Rows of d elements, row strides in elements, any
- * alignment of the element type (16-byte aligned rows with d * size % 16 == 0 are moved in 16-byte pieces); 1 <= d <=
- * paced_layernorm_max_width() (8192); M = 0 does nothing.
+ * alignment of the element type; 1 <= d <= paced_layernorm_max_width() (8192); M = 0 does nothing.
  * fwd: s = x, or s = round(x + res) written to xsum (res and xsum are both given or both NULL);
  *      y = (s - mean) rstd w + b;  mean[M], rstd[M] fp32 saved (each may be NULL).
  * bwd: x is what was normalised (xsum where there was a residual);  g = dy w,  xh = (x - mean) rstd,

@@ -14,7 +14,7 @@ enum Epi : int {
     EPI_TOPK_DENSE = 7,  // cand[n][m] = key(acc, row_base + m)
     EPI_TOPK_FILTER = 8, // if acc >= thr[n]: cand[n][cnt[n]++] = key(acc, row_base + m)
     // ---- internal to the linear-head cross entropy (linear_ce.hip); rows m are tokens, columns n vocabulary entries
-    EPI_CE_STATS = 9,    // part[n / W][m] = (max, sum of 2^(z - max)) of z = acc * alpha * log2 e over W columns but the label's
+    EPI_CE_STATS = 9,    // part[n / W * ce_rows + m] = (max, sum of 2^(z - max)) of z = acc * alpha * log2 e over W columns but the label's
                          // (W = 64; 32 for the 64x64 tiles); target[m] = the label's acc * alpha
     EPI_CE_GRAD = 10,    // C(bf16) = g[m] (2^(z - lse[m] log2 e) - [n is m's label]); columns N .. next multiple of 64 are zeros
     EPI_SLAB_F32 = 11    // C(f32) + split * strideC elements (+)= acc * alpha: one owner per element, no atomics
@@ -53,6 +53,7 @@ struct GemmParams {
     float* ce_target;
     long long ce_ignore;
     int ce_vocab, ce_first;       // vocabulary size, entry of column 0
+    int ce_rows;                  // rows of part (a launch may cover some of them)
     int accumulate;               // EPI_SLAB_F32: add to what is there
     int tile;                     // tile edge the caller has chosen (0: the launch's own rule; paced_gemm_set_tile overrides)
 };

@@ -348,7 +348,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, void* Cb, int m0, 
         const int nw = n0 + Cfg::noff(wn, 0), nl = (lane >> 4) * 4;        // the wave's first column; this lane's within 16
         if (nw >= p.N) return;
         const bool edge = nw + NJ * 16 > p.N;
-        f32x2* part = p.ce_part + (size_t)(nw / (NJ * 16)) * p.M;
+        f32x2* part = p.ce_part + (size_t)(nw / (NJ * 16)) * p.ce_rows;
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
             const int m = m0 + Cfg::moff(wm, i) + (lane & 15);

@@ -15,9 +15,13 @@ namespace {
 constexpr int LN_BLOCK = 256;
 constexpr int LN_MAX_D = 8192;
 
-// V elements of type T as they are loaded: 16 bytes where rows allow it, single elements otherwise
-template <class T, int V> struct Piece;
-template <> struct Piece<bf16, 8> {
+// 16 bytes of a row in a register quad.  The vector types carry the element's alignment only: gfx950 loads and stores 16 bytes
+// at any element address, so rows of odd width or stride take the same path (single elements instead: 23 us for the backward
+// pass of 5001 x 1023 fp32).  The last piece of a row that ends inside it (TAIL) is moved element by element.
+template <class T> struct Piece;
+template <> struct Piece<bf16> {
+    static constexpr int V = 8;
+    typedef u32x4 __attribute__((aligned(2))) At;
     u32x4 r;
     __device__ __forceinline__ float get(int j) const { return __uint_as_float((j & 1) ? (r[j >> 1] & 0xffff0000u) : (r[j >> 1] << 16)); }
     __device__ __forceinline__ void put(const float (&f)[8]) {
@@ -27,29 +31,43 @@ template <> struct Piece<bf16, 8> {
             r[j] = __builtin_bit_cast(uint32_t, v);
         }
     }
-    __device__ __forceinline__ void load(const bf16* p) { r = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)); }
-    __device__ __forceinline__ void load_kept(const bf16* p) { r = *reinterpret_cast<const u32x4*>(p); }
-    __device__ __forceinline__ void store(bf16* p) const { __builtin_nontemporal_store(r, reinterpret_cast<u32x4*>(p)); }
-    __device__ __forceinline__ void clear() { r = u32x4{0u, 0u, 0u, 0u}; }
+    __device__ __forceinline__ void put_one(int j, bf16 x) {
+        const uint32_t u = __builtin_bit_cast(unsigned short, x);
+        r[j >> 1] = (j & 1) ? (r[j >> 1] & 0xffffu) | (u << 16) : (r[j >> 1] & 0xffff0000u) | u;
+    }
+    __device__ __forceinline__ bf16 one(int j) const { return __builtin_bit_cast(bf16, (unsigned short)(r[j >> 1] >> (16 * (j & 1)))); }
 };
-template <> struct Piece<float, 4> {
+template <> struct Piece<float> {
+    static constexpr int V = 4;
+    typedef f32x4 __attribute__((aligned(4))) At;
     f32x4 r;
     __device__ __forceinline__ float get(int j) const { return r[j]; }
     __device__ __forceinline__ void put(const float (&f)[4]) { r = f32x4{f[0], f[1], f[2], f[3]}; }
-    __device__ __forceinline__ void load(const float* p) { r = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p)); }
-    __device__ __forceinline__ void load_kept(const float* p) { r = *reinterpret_cast<const f32x4*>(p); }
-    __device__ __forceinline__ void store(float* p) const { __builtin_nontemporal_store(r, reinterpret_cast<f32x4*>(p)); }
-    __device__ __forceinline__ void clear() { r = f32x4{0.f, 0.f, 0.f, 0.f}; }
+    __device__ __forceinline__ void put_one(int j, float x) { r[j] = x; }
+    __device__ __forceinline__ float one(int j) const { return r[j]; }
 };
-template <class T> struct Piece<T, 1> {
-    T r;
-    __device__ __forceinline__ float get(int) const { return (float)r; }
-    __device__ __forceinline__ void put(const float (&f)[1]) { r = (T)f[0]; }
-    __device__ __forceinline__ void load(const T* p) { r = *p; }
-    __device__ __forceinline__ void load_kept(const T* p) { r = *p; }
-    __device__ __forceinline__ void store(T* p) const { *p = r; }
-    __device__ __forceinline__ void clear() { r = (T)0.f; }
-};
+// elements c .. c + V - 1 of a row of d (zeros past its end); STREAM: read once, past the caches
+template <bool STREAM, bool TAIL, class T>
+__device__ __forceinline__ void load_piece(Piece<T>& p, const T* row, int c, int d) {
+    typedef typename Piece<T>::At At;
+    p.r = decltype(p.r){};
+    if (!TAIL || c + Piece<T>::V <= d) {
+        if (c < d) p.r = STREAM ? __builtin_nontemporal_load(reinterpret_cast<const At*>(row + c)) : *reinterpret_cast<const At*>(row + c);
+    } else if (c < d) {
+#pragma unroll
+        for (int j = 0; j < Piece<T>::V; ++j) if (c + j < d) p.put_one(j, row[c + j]);
+    }
+}
+template <bool TAIL, class T>
+__device__ __forceinline__ void store_piece(const Piece<T>& p, T* row, int c, int d) {
+    typedef typename Piece<T>::At At;
+    if (!TAIL || c + Piece<T>::V <= d) {
+        if (c < d) __builtin_nontemporal_store(p.r, reinterpret_cast<At*>(row + c));
+    } else if (c < d) {
+#pragma unroll
+        for (int j = 0; j < Piece<T>::V; ++j) if (c + j < d) row[c + j] = p.one(j);
+    }
+}
 
 // sum over the TEAM threads of a row (16 or 64 lanes of a wave, or the whole workgroup through `sh`, two sets of four slots)
 template <int TEAM>
@@ -74,28 +92,22 @@ template <class T> struct LnFwd {
 
 // EARLY: w and b are requested together with the row (a launch that is over in one row's latency); else behind the row's sums,
 // from the caches (fewer registers, more rows in flight)
-template <class T, int V, int TEAM, int PER, bool EARLY>
+template <class T, int TEAM, int PER, bool TAIL, bool EARLY>
 __global__ void __launch_bounds__(LN_BLOCK) ln_fwd_kernel(LnFwd<T> a) {
-    constexpr int RPB = LN_BLOCK / TEAM;
+    constexpr int V = Piece<T>::V, RPB = LN_BLOCK / TEAM;
     __shared__ float sh[4][4];
     const int l = threadIdx.x % TEAM, t = threadIdx.x / TEAM;
     const float inv_d = 1.f / (float)a.d;
     for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.M; row0 += (long long)gridDim.x * RPB) {
         const bool ok = row0 + t < a.M;
         const size_t row = ok ? row0 + t : a.M - 1;         // a team past the end repeats the last row and stores nothing
-        Piece<T, V> p[PER], q[PER], w[PER], b[PER];
+        Piece<T> p[PER], q[PER], w[PER], b[PER];
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int c = (l + i * TEAM) * V;
-            p[i].clear();
-            q[i].clear();
-            w[i].clear();
-            b[i].clear();
-            if (c < a.d) {
-                p[i].load(a.x + row * a.ldx + c);
-                if (a.res) q[i].load(a.res + row * a.ldr + c);
-                if (EARLY) { w[i].load_kept(a.w + c); b[i].load_kept(a.b + c); }
-            }
+            load_piece<true, TAIL>(p[i], a.x + row * a.ldx, c, a.d);
+            if (a.res) load_piece<true, TAIL>(q[i], a.res + row * a.ldr, c, a.d);
+            if (EARLY) { load_piece<false, TAIL>(w[i], a.w, c, a.d); load_piece<false, TAIL>(b[i], a.b, c, a.d); }
         }
         float sum = 0.f;
 #pragma unroll
@@ -106,7 +118,7 @@ __global__ void __launch_bounds__(LN_BLOCK) ln_fwd_kernel(LnFwd<T> a) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) f[j] = p[i].get(j) + q[i].get(j);
                 p[i].put(f);
-                if (ok && c < a.d) p[i].store(a.xsum + row * a.lds + c);
+                if (ok) store_piece<TAIL>(p[i], a.xsum + row * a.lds, c, a.d);
             }
 #pragma unroll
             for (int j = 0; j < V; ++j) sum += p[i].get(j);
@@ -114,11 +126,16 @@ __global__ void __launch_bounds__(LN_BLOCK) ln_fwd_kernel(LnFwd<T> a) {
         const float mean = team_sum<TEAM>(sum, sh[0]) * inv_d;
         float sq = 0.f;
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if ((l + i * TEAM) * V < a.d) {
+        for (int i = 0; i < PER; ++i) {
+            const int c = (l + i * TEAM) * V;
+            if (c < a.d) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) { const float f = p[i].get(j) - mean; sq += f * f; }
+                for (int j = 0; j < V; ++j) {
+                    const float f = TAIL && c + j >= a.d ? 0.f : p[i].get(j) - mean;
+                    sq += f * f;
+                }
             }
+        }
         const float rstd = 1.f / sqrtf(team_sum<TEAM>(sq, sh[1]) * inv_d + a.eps);
         if (l == 0 && ok) {
             if (a.mean) a.mean[row] = mean;
@@ -127,15 +144,13 @@ __global__ void __launch_bounds__(LN_BLOCK) ln_fwd_kernel(LnFwd<T> a) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int c = (l + i * TEAM) * V;
-            if (ok && c < a.d) {
-                Piece<T, V> o;
-                if (!EARLY) { w[i].load_kept(a.w + c); b[i].load_kept(a.b + c); }
-                float f[V];
+            if (!EARLY) { load_piece<false, TAIL>(w[i], a.w, c, a.d); load_piece<false, TAIL>(b[i], a.b, c, a.d); }
+            Piece<T> o;
+            float f[V];
 #pragma unroll
-                for (int j = 0; j < V; ++j) f[j] = (p[i].get(j) - mean) * rstd * w[i].get(j) + b[i].get(j);
-                o.put(f);
-                o.store(a.y + row * a.ldy + c);
-            }
+            for (int j = 0; j < V; ++j) f[j] = (p[i].get(j) - mean) * rstd * w[i].get(j) + b[i].get(j);
+            o.put(f);
+            if (ok) store_piece<TAIL>(o, a.y + row * a.ldy, c, a.d);
         }
         if (TEAM > 64) __syncthreads();                     // the next row's sums reuse `sh`
     }
@@ -149,11 +164,12 @@ template <class T> struct LnBwd {
     int lddy, ldx, ldr, lddx, M, d;
 };
 
-// two waves per SIMD: a thread carries its pieces of three rows and two column sums in up to 256 registers
-template <class T, int V, int TEAM, int PER>
-__global__ void __launch_bounds__(LN_BLOCK) __attribute__((amdgpu_waves_per_eu(2)))
+// two waves per SIMD: a thread carries its pieces of three rows and two column sums in up to 256 registers (one wave and 512
+// for fp32 rows of more than 4096)
+template <class T, int TEAM, int PER, bool TAIL>
+__global__ void __launch_bounds__(LN_BLOCK) __attribute__((amdgpu_waves_per_eu(PER < 8 ? 2 : 1)))
 ln_bwd_kernel(LnBwd<T> a) {
-    constexpr int RPB = LN_BLOCK / TEAM;
+    constexpr int V = Piece<T>::V, RPB = LN_BLOCK / TEAM;
     __shared__ float sh[4][4];
     extern __shared__ float cols[];                         // [4 waves][d]
     const int l = threadIdx.x % TEAM, t = threadIdx.x / TEAM;
@@ -166,27 +182,23 @@ ln_bwd_kernel(LnBwd<T> a) {
     for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.M; row0 += (long long)gridDim.x * RPB) {
         const bool ok = row0 + t < a.M;
         const size_t row = ok ? row0 + t : a.M - 1;
-        Piece<T, V> p[PER], q[PER], r[PER];
+        Piece<T> p[PER], q[PER], r[PER];
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int c = (l + i * TEAM) * V;
-            p[i].clear();
-            q[i].clear();
-            r[i].clear();
-            if (c < a.d) {
-                p[i].load(a.dy + row * a.lddy + c);
-                q[i].load(a.x + row * a.ldx + c);
-                if (a.dres) r[i].load(a.dres + row * a.ldr + c);
-            }
+            load_piece<true, TAIL>(p[i], a.dy + row * a.lddy, c, a.d);
+            load_piece<true, TAIL>(q[i], a.x + row * a.ldx, c, a.d);
+            r[i].r = decltype(r[i].r){};
+            if (a.dres) load_piece<true, TAIL>(r[i], a.dres + row * a.ldr, c, a.d);
         }
         const float mean = a.mean[row], rstd = a.rstd[row];
         float sg = 0.f, sgx = 0.f;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int c = (l + i * TEAM) * V;
-            if (c < a.d) {
-                Piece<T, V> w;
-                w.load_kept(a.w + c);
+            if (c < a.d) {                                  // (past the end of a row dy and w are zeros)
+                Piece<T> w;
+                load_piece<false, TAIL>(w, a.w, c, a.d);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const float dy = p[i].get(j), xh = (q[i].get(j) - mean) * rstd, g = dy * w.get(j);
@@ -201,18 +213,16 @@ ln_bwd_kernel(LnBwd<T> a) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int c = (l + i * TEAM) * V;
-            if (ok && c < a.d) {
-                Piece<T, V> w, o;
-                w.load_kept(a.w + c);
-                float f[V];
+            Piece<T> w, o;
+            load_piece<false, TAIL>(w, a.w, c, a.d);
+            float f[V];
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float xh = (q[i].get(j) - mean) * rstd;
-                    f[j] = rstd * (p[i].get(j) * w.get(j) - sg - xh * sgx) + r[i].get(j);
-                }
-                o.put(f);
-                o.store(a.dx + row * a.lddx + c);
+            for (int j = 0; j < V; ++j) {
+                const float xh = (q[i].get(j) - mean) * rstd;
+                f[j] = rstd * (p[i].get(j) * w.get(j) - sg - xh * sgx) + r[i].get(j);
             }
+            o.put(f);
+            if (ok) store_piece<TAIL>(o, a.dx + row * a.lddx, c, a.d);
         }
         if (TEAM > 64) __syncthreads();
     }
@@ -288,80 +298,53 @@ int ln_bwd_grid(int M) {
     return M < most ? M : most;
 }
 
-template <class T, int V, int TEAM, int PER>
-int ln_fwd_go(const LnFwd<T>& a, hipStream_t s) {
+template <class T, int TEAM, int PER, bool TAIL>
+int ln_go(const LnFwd<T>& a, int, hipStream_t s) {
     const long long blocks = ((long long)a.M + LN_BLOCK / TEAM - 1) / (LN_BLOCK / TEAM);
     const int grid = (int)(blocks < 8192 ? blocks : 8192);
-    if (blocks <= paced_cu_count()) hipLaunchKernelGGL((ln_fwd_kernel<T, V, TEAM, PER, true>), dim3(grid), dim3(LN_BLOCK), 0, s, a);
-    else hipLaunchKernelGGL((ln_fwd_kernel<T, V, TEAM, PER, false>), dim3(grid), dim3(LN_BLOCK), 0, s, a);
+    if (blocks <= paced_cu_count()) hipLaunchKernelGGL((ln_fwd_kernel<T, TEAM, PER, TAIL, true>), dim3(grid), dim3(LN_BLOCK), 0, s, a);
+    else hipLaunchKernelGGL((ln_fwd_kernel<T, TEAM, PER, TAIL, false>), dim3(grid), dim3(LN_BLOCK), 0, s, a);
     PACED_CHECK_LAUNCH();
     return PACED_OK;
 }
-template <class T, int V, int TEAM, int PER>
-int ln_bwd_go(const LnBwd<T>& a, int grid, hipStream_t s) {
+template <class T, int TEAM, int PER, bool TAIL>
+int ln_go(const LnBwd<T>& a, int grid, hipStream_t s) {
     const int smem = TEAM < LN_BLOCK && a.part ? 4 * a.d * 4 : 0;              // 32 KiB at most: these teams take d <= 2048
-    hipLaunchKernelGGL((ln_bwd_kernel<T, V, TEAM, PER>), dim3(grid), dim3(LN_BLOCK), smem, s, a);
+    hipLaunchKernelGGL((ln_bwd_kernel<T, TEAM, PER, TAIL>), dim3(grid), dim3(LN_BLOCK), smem, s, a);
     PACED_CHECK_LAUNCH();
     return PACED_OK;
 }
 
 // the narrowest team whose registers hold a row of d elements
-#define LN_TEAM(T, V, TEAM, PER, ...) if (d <= V * TEAM * PER) return GO(T, V, TEAM, PER);
-#define LN_PICK_BF16 LN_TEAM(bf16, 8, 16, 1) LN_TEAM(bf16, 8, 16, 2) LN_TEAM(bf16, 8, 16, 4) LN_TEAM(bf16, 8, 16, 6) \
-                     LN_TEAM(bf16, 8, 64, 2) LN_TEAM(bf16, 8, 64, 4) LN_TEAM(bf16, 8, 256, 2) LN_TEAM(bf16, 8, 256, 4)
-#define LN_PICK_F32 LN_TEAM(float, 4, 16, 2) LN_TEAM(float, 4, 16, 8) LN_TEAM(float, 4, 64, 3) LN_TEAM(float, 4, 64, 4) LN_TEAM(float, 4, 64, 8) \
-                    LN_TEAM(float, 4, 256, 4) LN_TEAM(float, 4, 256, 8)
-#define LN_PICK_ONE(T) LN_TEAM(T, 1, 16, 4) LN_TEAM(T, 1, 64, 4) LN_TEAM(T, 1, 64, 16) LN_TEAM(T, 1, 256, 8) LN_TEAM(T, 1, 256, 32)
-
-template <class T> int ln_fwd_pick(const LnFwd<T>& a, bool vec, hipStream_t s);
-template <class T> int ln_bwd_pick(const LnBwd<T>& a, bool vec, int grid, hipStream_t s);
-#define GO(T, V, TEAM, PER) ln_fwd_go<T, V, TEAM, PER>(a, s)
-template <> int ln_fwd_pick<bf16>(const LnFwd<bf16>& a, bool vec, hipStream_t s) {
-    const int d = a.d;
-    if (vec) { LN_PICK_BF16 }
-    LN_PICK_ONE(bf16)
-    return PACED_ERR_ARG;
+template <class T, bool TAIL, class Args>
+int ln_team(const Args& a, int grid, hipStream_t s) {
+    const int n = (a.d + Piece<T>::V - 1) / Piece<T>::V;     // pieces of a row
+    if (n <= 16) return ln_go<T, 16, 1, TAIL>(a, grid, s);
+    if (n <= 32) return ln_go<T, 16, 2, TAIL>(a, grid, s);
+    if (n <= 64) return ln_go<T, 16, 4, TAIL>(a, grid, s);
+    if (n <= 96) return ln_go<T, 16, 6, TAIL>(a, grid, s);
+    if (n <= 128) return ln_go<T, 64, 2, TAIL>(a, grid, s);
+    if (n <= 256) return ln_go<T, 64, 4, TAIL>(a, grid, s);
+    if (n <= 512) return ln_go<T, 256, 2, TAIL>(a, grid, s);
+    if (n <= 1024) return ln_go<T, 256, 4, TAIL>(a, grid, s);
+    if constexpr (Piece<T>::V * 1024 < LN_MAX_D) return ln_go<T, 256, 8, TAIL>(a, grid, s);
+    return PACED_ERR_ARG;                                    // (d <= LN_MAX_D was checked)
 }
-template <> int ln_fwd_pick<float>(const LnFwd<float>& a, bool vec, hipStream_t s) {
-    const int d = a.d;
-    if (vec) { LN_PICK_F32 }
-    LN_PICK_ONE(float)
-    return PACED_ERR_ARG;
+template <class T, class Args>
+int ln_launch(const Args& a, int grid, hipStream_t s) {
+    static_assert(1024 * Piece<bf16>::V >= LN_MAX_D && 2048 * Piece<float>::V >= LN_MAX_D, "the widest teams hold the widest row");
+    return a.d % Piece<T>::V ? ln_team<T, true>(a, grid, s) : ln_team<T, false>(a, grid, s);
 }
-#undef GO
-#define GO(T, V, TEAM, PER) ln_bwd_go<T, V, TEAM, PER>(a, grid, s)
-template <> int ln_bwd_pick<bf16>(const LnBwd<bf16>& a, bool vec, int grid, hipStream_t s) {
-    const int d = a.d;
-    if (vec) { LN_PICK_BF16 }
-    LN_PICK_ONE(bf16)
-    return PACED_ERR_ARG;
-}
-template <> int ln_bwd_pick<float>(const LnBwd<float>& a, bool vec, int grid, hipStream_t s) {
-    const int d = a.d;
-    if (vec) { LN_PICK_F32 }
-    LN_PICK_ONE(float)
-    return PACED_ERR_ARG;
-}
-#undef GO
-
-// whether rows at p, ld elements apart, can be moved in 16-byte pieces
-bool vec_ok(const void* p, int ld, int size) { return !p || (((uintptr_t)p & 15) == 0 && (long long)ld * size % 16 == 0); }
 
 template <class T>
 int ln_fwd(const void* x, int ldx, const void* res, int ldr, void* xsum, int lds, const void* w, const void* b, void* y, int ldy,
            float* mean, float* rstd, int M, int d, float eps, hipStream_t s) {
-    const int size = (int)sizeof(T);
-    const bool vec = (long long)d * size % 16 == 0 && vec_ok(x, ldx, size) && vec_ok(res, ldr, size) && vec_ok(xsum, lds, size) &&
-                     vec_ok(y, ldy, size) && vec_ok(w, 0, size) && vec_ok(b, 0, size);
-    return ln_fwd_pick<T>(LnFwd<T>{(const T*)x, (const T*)res, (const T*)w, (const T*)b, (T*)xsum, (T*)y, mean, rstd, ldx, ldr, lds, ldy, M, d, eps}, vec, s);
+    return ln_launch<T>(LnFwd<T>{(const T*)x, (const T*)res, (const T*)w, (const T*)b, (T*)xsum, (T*)y, mean, rstd, ldx, ldr, lds, ldy, M, d, eps}, 0, s);
 }
 template <class T>
 int ln_bwd(const void* dy, int lddy, const void* x, int ldx, const void* w, const float* mean, const float* rstd, const void* dres, int ldr,
            void* dx, int lddx, float* part, int grid, int M, int d, hipStream_t s) {
-    const int size = (int)sizeof(T);
-    const bool vec = (long long)d * size % 16 == 0 && vec_ok(dy, lddy, size) && vec_ok(x, ldx, size) && vec_ok(dres, ldr, size) &&
-                     vec_ok(dx, lddx, size) && vec_ok(w, 0, size);
-    return ln_bwd_pick<T>(LnBwd<T>{(const T*)dy, (const T*)x, (const T*)w, (const T*)dres, mean, rstd, (T*)dx, part, lddy, ldx, ldr, lddx, M, d}, vec, grid, s);
+    return ln_launch<T>(LnBwd<T>{(const T*)dy, (const T*)x, (const T*)w, (const T*)dres, mean, rstd, (T*)dx, part, lddy, ldx, ldr, lddx, M, d}, grid, s);
 }
 
 }  // namespace

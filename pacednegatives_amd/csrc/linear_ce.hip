@@ -22,40 +22,44 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
     m = mx;
 }
 
-// 8 rows of a workgroup, 32 threads over the column groups of each
+// RPB rows of a workgroup, 256 / RPB threads over the column groups of each: 8 (64-byte runs of a group's row statistics), or
+// 1 where there are too few rows to fill the chip
+template <int RPB>
 __global__ void __launch_bounds__(256) ce_join_kernel(const f32x2* __restrict__ part, int groups, const float* __restrict__ target,
                                                       const long long* __restrict__ labels, long long ignore, int V,
                                                       float* __restrict__ loss, float* __restrict__ lse, int R) {
-    __shared__ f32x2 sh[4][8];
-    const int r = threadIdx.x & 7, k = threadIdx.x >> 3;
-    const int row = blockIdx.x * 8 + r, rr = min(row, R - 1);
+    constexpr int K = 256 / RPB, AHEAD = RPB == 1 ? 4 : 8;
+    __shared__ f32x2 sh[4][RPB];
+    const int r = threadIdx.x % RPB, k = threadIdx.x / RPB;
+    const int row = blockIdx.x * RPB + r, rr = min(row, R - 1);
+    const long long label = labels[rr];
+    const float t = target[rr];
     float m = -INFINITY, s = 0.f;
     int g = k;
-    for (; g + 7 * 32 < groups; g += 8 * 32) {        // eight loads in flight
-        f32x2 v[8];
+    for (; g + (AHEAD - 1) * K < groups; g += AHEAD * K) {        // that many loads in flight
+        f32x2 v[AHEAD];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = part[(size_t)(g + i * 32) * R + rr];
+        for (int i = 0; i < AHEAD; ++i) v[i] = part[(size_t)(g + i * K) * R + rr];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) join(m, s, v[i][0], v[i][1]);
+        for (int i = 0; i < AHEAD; ++i) join(m, s, v[i][0], v[i][1]);
     }
-    for (; g < groups; g += 32) {
+    for (; g < groups; g += K) {
         const f32x2 v = part[(size_t)g * R + rr];
         join(m, s, v[0], v[1]);
     }
 #pragma unroll
-    for (int o = 8; o < 64; o <<= 1) join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
-    if ((threadIdx.x & 63) < 8) sh[threadIdx.x >> 6][r] = f32x2{m, s};
+    for (int o = RPB; o < 64; o <<= 1) join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+    if ((threadIdx.x & 63) < RPB) sh[threadIdx.x >> 6][r] = f32x2{m, s};
     __syncthreads();
-    if (threadIdx.x >= 8 || row >= R) return;
+    if (threadIdx.x >= RPB || row >= R) return;
 #pragma unroll
     for (int w = 1; w < 4; ++w) join(m, s, sh[w][r][0], sh[w][r][1]);
-    const long long label = labels[row];
     if (label == ignore || label < 0 || label >= V) {
         loss[row] = 0.f;
         if (lse) lse[row] = m * LN2 + logf(s);
         return;
     }
-    const float t = target[row], t2 = t * LOG2E;
+    const float t2 = t * LOG2E;                                 // (written for a label that counts; garbage otherwise)
     float l;
     if (m == -INFINITY) l = s == 0.f ? 0.f : s;                 // no other entry (or a NaN among them)
     else if (t2 >= m) l = log1pf(s * __builtin_amdgcn_exp2f(m - t2));
@@ -109,29 +113,52 @@ int best_tile(int M, int N, int steps) {
     return tile;
 }
 
-// Pieces of the vocabulary, tiles, and slices of a piece for dh.  A piece's P takes at most 256 MiB.  More slices give dh's
-// product more workgroups and its second kernel more slabs to add (written and read at about 4 TB/s).
-struct CePlan { int piece, ldp, slabs, dh_tile; };
-CePlan ce_plan(int R, int V, int d) {
-    CePlan pl;
-    long long fit = (256ll << 20) / 2 / (R > 0 ? R : 1) / 256 * 256;
-    if (fit < 256) fit = 256;
-    const int pieces = (int)((V + fit - 1) / fit);
-    long long piece = ((V + pieces - 1) / pieces + 255) / 256 * 256;
-    if (piece > V) piece = V;
-    pl.piece = (int)piece;
-    pl.ldp = (int)((piece + 63) / 64 * 64);
-    const int steps = (pl.piece + 63) / 64;
+// Tile and slices of dh's product over a piece: more slices give it more workgroups and its second kernel more slabs to add
+// (written and read at about 4 TB/s).
+double dh_us(int R, int d, int steps, int* tile, int* slices) {
     double best = 1e30;
-    pl.slabs = 1;
-    pl.dh_tile = 64;
     for (int t = 256; t >= 64; t /= 2) {
         if (t == 256 && (R < 256 || d < 256)) continue;
         for (int s = 1; s <= 64 && s * 3 <= steps + 2; ++s) {
             const double us = product_us(t, R, d, s, steps) + (double)s * R * d * 8. / 4e6;
-            if (us < best) { best = us; pl.slabs = s; pl.dh_tile = t; }
+            if (us < best) { best = us; *slices = s; *tile = t; }
+            if (t != 64 && (long long)((R + t - 1) / t) * ((d + t - 1) / t) * s > 4ll * paced_cu_count()) break;
         }
     }
+    return best;
+}
+
+// Pieces of the vocabulary: P takes at most 256 MiB (256 columns at least).  Where it takes several, sixteen widths between
+// half and all of that are compared by the rounds of tiles that they come to.
+struct CePlan { int piece, ldp, slabs, dh_tile; };
+CePlan ce_plan(int R, int V, int d) {
+    CePlan pl;
+    long long fit = (256ll << 20) / 2 / (R > 0 ? R : 1) / 256;       // in tiles of 256 columns
+    if (fit < 1) fit = 1;
+    long long piece = fit * 256;
+    if (piece >= V) piece = V;
+    else {
+        double best = 1e30;
+        const long long down = fit / 32 > 0 ? fit / 32 : 1;
+        for (long long c = fit; c >= 1 && c * 2 >= fit && c > fit - 16 * down; c -= down) {
+            double us = 0.;
+            const int full = (int)(V / (c * 256)), rest = (int)(V - full * c * 256), k = (R + 63) / 64;
+            for (int part = 0; part < 2; ++part) {
+                const int n = part ? rest : (int)c * 256;
+                if (n == 0 || (!part && !full)) continue;
+                int tile = 64, slices = 1;
+                us += (part ? 1 : full) * (product_us(best_tile(R, n, d / 64), R, n, 1, d / 64) + dh_us(R, d, (n + 63) / 64, &tile, &slices) +
+                                           product_us(best_tile(n, d, k), n, d, 1, k));
+            }
+            if (us < best) { best = us; piece = c * 256; }
+        }
+    }
+    pl.piece = (int)piece;
+    pl.ldp = (int)((piece + 63) / 64 * 64);
+    const int steps = (pl.piece + 63) / 64;
+    pl.slabs = 1;
+    pl.dh_tile = 64;
+    dh_us(R, d, steps, &pl.dh_tile, &pl.slabs);
     const int per = (steps + pl.slabs - 1) / pl.slabs;
     pl.slabs = (steps + per - 1) / per;
     return pl;
@@ -143,6 +170,34 @@ GemmParams product(const void* A, int lda, const void* B, int ldb, void* C, int 
     p.M = M; p.N = N; p.K = K; p.lda = lda; p.ldb = ldb; p.ldc = ldc;
     p.k_per_split = K; p.batch = 1; p.alpha = alpha; p.mask_scale = 1.f; p.drop = make_drop(0.f, 0);
     return p;
+}
+
+// One product of the logits (EPI_CE_STATS or EPI_CE_GRAD) of all rows: in one launch, or the rows that fill 256x256 tiles and
+// the rest in 128x128 tiles where that saves a round of tiles (1088 rows x 32128 entries: 3 rounds for 4.25 tiles of rows, 2 for
+// 4).  Up to 64 rows 64x64 tiles read the weights fastest (16 rows: 16.6 us against 18.4 with 128x128).
+int ce_logits(GemmParams p, int epilogue, hipStream_t s) {
+    const int steps = (p.K + 63) / 64, R = p.M, full = R / 256 * 256;
+    if (R <= 64) p.tile = 64;
+    else p.tile = best_tile(R, p.N, steps);
+    if (p.tile < 128 && R > 64) p.tile = 128;
+    if (full > 0 && full < R && p.N >= 256) {
+        const double split = product_us(256, full, p.N, 1, steps) + product_us(128, R - full, p.N, 1, steps);
+        if (split < product_us(p.tile, R, p.N, 1, steps)) {
+            GemmParams rest = p;
+            p.M = full;
+            p.tile = 256;
+            const int rc = paced_gemm_launch(p, false, false, epilogue, 1, s);
+            if (rc != PACED_OK) return rc;
+            rest.M = R - full;
+            rest.tile = 128;
+            rest.A += (size_t)full * p.lda;
+            rest.ce_labels += full;
+            if (epilogue == EPI_CE_STATS) { rest.ce_part += full; rest.ce_target += full; }
+            else { rest.ce_lse += full; rest.ce_g += full; rest.C = (bf16*)rest.C + (size_t)full * p.ldc; }
+            return paced_gemm_launch(rest, false, false, epilogue, 1, s);
+        }
+    }
+    return paced_gemm_launch(p, false, false, epilogue, 1, s);
 }
 
 int ce_check(const char* who, const void* h, int ldh, const void* w, int ldw, const long long* labels, int R, int V, int d) {
@@ -173,11 +228,15 @@ extern "C" int paced_linear_ce_fwd(const void* h, int ldh, const void* w, int ld
     p.ce_part = (f32x2*)workspace;
     p.ce_target = (float*)((char*)workspace + round256((size_t)((V + 31) / 32) * R * 8));
     p.ce_labels = labels; p.ce_ignore = ignore_index; p.ce_vocab = V;
-    const int rg = paced_gemm_launch(p, false, false, EPI_CE_STATS, 1, (hipStream_t)stream);
+    p.ce_rows = R;
+    const int rg = ce_logits(p, EPI_CE_STATS, (hipStream_t)stream);
     if (rg != PACED_OK) return rg;
     const int width = paced_gemm_last_kernel() < 128 ? 32 : 64;           // columns of a wave in the tiles that were taken
-    hipLaunchKernelGGL(ce_join_kernel, dim3((R + 7) / 8), dim3(256), 0, (hipStream_t)stream, p.ce_part, (V + width - 1) / width, p.ce_target,
-                       labels, ignore_index, V, loss, lse, R);
+    const int groups = (V + width - 1) / width;
+    if (R >= 2 * paced_cu_count())
+        hipLaunchKernelGGL(ce_join_kernel<8>, dim3((R + 7) / 8), dim3(256), 0, (hipStream_t)stream, p.ce_part, groups, p.ce_target, labels, ignore_index, V, loss, lse, R);
+    else
+        hipLaunchKernelGGL(ce_join_kernel<1>, dim3(R), dim3(256), 0, (hipStream_t)stream, p.ce_part, groups, p.ce_target, labels, ignore_index, V, loss, lse, R);
     PACED_CHECK_LAUNCH();
     return PACED_OK;
 }
@@ -218,7 +277,7 @@ extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ld
         GemmParams p = product(h, ldh, wp, ldw, P, pl.ldp, R, n, d, scale);
         p.ce_labels = labels; p.ce_lse = lse; p.ce_g = gloss;
         p.ce_ignore = ignore_index; p.ce_vocab = V; p.ce_first = v0;
-        int r = paced_gemm_launch(p, false, false, EPI_CE_GRAD, 1, s);
+        int r = ce_logits(p, EPI_CE_GRAD, s);
         if (r != PACED_OK) return r;
         if (dh) {
             p = product(P, pl.ldp, wp, ldw, slabs, d, R, d, n, scale);

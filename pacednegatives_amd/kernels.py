@@ -23,7 +23,8 @@ PROFILE = None
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    # (the raw handle: torch.cuda.current_stream() builds a Stream object, 2.5 us for each of a step's launches)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _p(t):
