@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(Cfg::WGM * Cfg::WGN * 64) gemm_ring_kernel(Gem
     constexpr bool NATURAL = (EPI == EPI_ATOMIC_F32 || EPI == EPI_TOPK_DENSE || EPI == EPI_TOPK_FILTER);
     using Ops = TileOps<Cfg, TA, TB>;
     constexpr int PER = Ops::IA + Ops::IB;           // LDS-DMA instructions per wave and K step
-    static_assert(NS >= 3 && (NS - 2) * PER <= 63, "the pending count must fit the vmcnt field");
+    static_assert(NS >= 2 && (NS - 2) * PER <= 63, "the pending count must fit the vmcnt field");
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1352,6 +1352,10 @@ int launch_cfg(GemmParams p, int splits, hipStream_t stream) {
                 if (per_cu == 3) return launch_ring<Cfg, TA, TB, EPI, 3>(p, ntm, ntn, total, stream);
             } else {
                 if (per_cu == 1) return launch_ring<Cfg, TA, TB, EPI, 4>(p, ntm, ntn, total, stream);
+                // linear_ce.hip's products with one to two tiles per CU: two buffers a workgroup, two workgroups a CU (the
+                // single buffer's full wait per K step has nobody to hide it here: 272 tiles of 12 steps, 20.6 us)
+                if constexpr (EPI == EPI_CE_STATS || EPI == EPI_CE_GRAD || EPI == EPI_SLAB_F32 || (EPI == EPI_BF16 && TA && TB))
+                    if (per_cu == 2 && p.tile == 128) return launch_ring<Cfg, TA, TB, EPI, 2>(p, ntm, ntn, total, stream);
             }
         }
     }

@@ -161,6 +161,7 @@ template <class T> struct LnBwd {
     const float *mean, *rstd;
     T* dx;
     float* part;                    // [gridDim.x][2][d]: sums of dy xh, then of dy; NULL: no column sums
+    float *dw, *db;
     int lddy, ldx, ldr, lddx, M, d;
 };
 
@@ -292,14 +293,10 @@ __global__ void __launch_bounds__(32 * COLS_LANES) ln_cols_kernel(const float* _
     }
 }
 
-// workgroups of the backward kernel: two to a compute unit, none without a row
-int ln_bwd_grid(int M) {
-    const int most = 2 * paced_cu_count();
-    return M < most ? M : most;
-}
+constexpr int LN_BWD_PER_CU = 4;           // most workgroups of the backward kernel for a compute unit (the workspace's rows)
 
 template <class T, int TEAM, int PER, bool TAIL>
-int ln_go(const LnFwd<T>& a, int, hipStream_t s) {
+int ln_go(const LnFwd<T>& a, hipStream_t s) {
     const long long blocks = ((long long)a.M + LN_BLOCK / TEAM - 1) / (LN_BLOCK / TEAM);
     const int grid = (int)(blocks < 8192 ? blocks : 8192);
     if (blocks <= paced_cu_count()) hipLaunchKernelGGL((ln_fwd_kernel<T, TEAM, PER, TAIL, true>), dim3(grid), dim3(LN_BLOCK), 0, s, a);
@@ -308,43 +305,50 @@ int ln_go(const LnFwd<T>& a, int, hipStream_t s) {
     return PACED_OK;
 }
 template <class T, int TEAM, int PER, bool TAIL>
-int ln_go(const LnBwd<T>& a, int grid, hipStream_t s) {
+int ln_go(const LnBwd<T>& a, hipStream_t s) {
+    // resident workgroups: up to 16 elements a thread need at most 128 registers, four to a compute unit; more need up to 256
+    const int most = (PER * Piece<T>::V <= 16 ? LN_BWD_PER_CU : 2) * paced_cu_count();
+    const long long rounds_of = ((long long)a.M + LN_BLOCK / TEAM - 1) / (LN_BLOCK / TEAM), rounds = (rounds_of + most - 1) / most;
+    const int grid = (int)((rounds_of + rounds - 1) / rounds);          // every workgroup the same number of row groups
     const int smem = TEAM < LN_BLOCK && a.part ? 4 * a.d * 4 : 0;              // 32 KiB at most: these teams take d <= 2048
     hipLaunchKernelGGL((ln_bwd_kernel<T, TEAM, PER, TAIL>), dim3(grid), dim3(LN_BLOCK), smem, s, a);
+    PACED_CHECK_LAUNCH();
+    if (!a.part) return PACED_OK;
+    hipLaunchKernelGGL(ln_cols_kernel, dim3((2 * a.d + 31) / 32), dim3(32 * COLS_LANES), 0, s, a.part, grid, a.d, a.dw, a.db);
     PACED_CHECK_LAUNCH();
     return PACED_OK;
 }
 
 // the narrowest team whose registers hold a row of d elements
 template <class T, bool TAIL, class Args>
-int ln_team(const Args& a, int grid, hipStream_t s) {
+int ln_team(const Args& a, hipStream_t s) {
     const int n = (a.d + Piece<T>::V - 1) / Piece<T>::V;     // pieces of a row
-    if (n <= 16) return ln_go<T, 16, 1, TAIL>(a, grid, s);
-    if (n <= 32) return ln_go<T, 16, 2, TAIL>(a, grid, s);
-    if (n <= 64) return ln_go<T, 16, 4, TAIL>(a, grid, s);
-    if (n <= 96) return ln_go<T, 16, 6, TAIL>(a, grid, s);
-    if (n <= 128) return ln_go<T, 64, 2, TAIL>(a, grid, s);
-    if (n <= 256) return ln_go<T, 64, 4, TAIL>(a, grid, s);
-    if (n <= 512) return ln_go<T, 256, 2, TAIL>(a, grid, s);
-    if (n <= 1024) return ln_go<T, 256, 4, TAIL>(a, grid, s);
-    if constexpr (Piece<T>::V * 1024 < LN_MAX_D) return ln_go<T, 256, 8, TAIL>(a, grid, s);
+    if (n <= 16) return ln_go<T, 16, 1, TAIL>(a, s);
+    if (n <= 32) return ln_go<T, 16, 2, TAIL>(a, s);
+    if (n <= 64) return ln_go<T, 16, 4, TAIL>(a, s);
+    if (n <= 96) return ln_go<T, 16, 6, TAIL>(a, s);
+    if (n <= 128) return ln_go<T, 64, 2, TAIL>(a, s);
+    if (n <= 256) return ln_go<T, 64, 4, TAIL>(a, s);
+    if (n <= 512) return ln_go<T, 256, 2, TAIL>(a, s);
+    if (n <= 1024) return ln_go<T, 256, 4, TAIL>(a, s);
+    if constexpr (Piece<T>::V * 1024 < LN_MAX_D) return ln_go<T, 256, 8, TAIL>(a, s);
     return PACED_ERR_ARG;                                    // (d <= LN_MAX_D was checked)
 }
 template <class T, class Args>
-int ln_launch(const Args& a, int grid, hipStream_t s) {
+int ln_launch(const Args& a, hipStream_t s) {
     static_assert(1024 * Piece<bf16>::V >= LN_MAX_D && 2048 * Piece<float>::V >= LN_MAX_D, "the widest teams hold the widest row");
-    return a.d % Piece<T>::V ? ln_team<T, true>(a, grid, s) : ln_team<T, false>(a, grid, s);
+    return a.d % Piece<T>::V ? ln_team<T, true>(a, s) : ln_team<T, false>(a, s);
 }
 
 template <class T>
 int ln_fwd(const void* x, int ldx, const void* res, int ldr, void* xsum, int lds, const void* w, const void* b, void* y, int ldy,
            float* mean, float* rstd, int M, int d, float eps, hipStream_t s) {
-    return ln_launch<T>(LnFwd<T>{(const T*)x, (const T*)res, (const T*)w, (const T*)b, (T*)xsum, (T*)y, mean, rstd, ldx, ldr, lds, ldy, M, d, eps}, 0, s);
+    return ln_launch<T>(LnFwd<T>{(const T*)x, (const T*)res, (const T*)w, (const T*)b, (T*)xsum, (T*)y, mean, rstd, ldx, ldr, lds, ldy, M, d, eps}, s);
 }
 template <class T>
 int ln_bwd(const void* dy, int lddy, const void* x, int ldx, const void* w, const float* mean, const float* rstd, const void* dres, int ldr,
-           void* dx, int lddx, float* part, int grid, int M, int d, hipStream_t s) {
-    return ln_launch<T>(LnBwd<T>{(const T*)dy, (const T*)x, (const T*)w, (const T*)dres, mean, rstd, (T*)dx, part, lddy, ldx, ldr, lddx, M, d}, grid, s);
+           void* dx, int lddx, float* dw, float* db, float* part, int M, int d, hipStream_t s) {
+    return ln_launch<T>(LnBwd<T>{(const T*)dy, (const T*)x, (const T*)w, (const T*)dres, mean, rstd, (T*)dx, part, dw, db, lddy, ldx, ldr, lddx, M, d}, s);
 }
 
 }  // namespace
@@ -365,7 +369,8 @@ extern "C" int paced_layernorm_fwd(const void* x, int ldx, const void* res, int 
 
 extern "C" size_t paced_layernorm_workspace_bytes(int M, int d) {
     if (M <= 0 || d <= 0) return 0;
-    return (size_t)ln_bwd_grid(M) * 2 * (size_t)d * 4;
+    const size_t most = (size_t)LN_BWD_PER_CU * paced_cu_count();
+    return ((size_t)M < most ? (size_t)M : most) * 2 * (size_t)d * 4;
 }
 
 extern "C" int paced_layernorm_bwd(const void* dy, int lddy, const void* x, int ldx, const void* w, const float* mean, const float* rstd,
@@ -379,12 +384,7 @@ extern "C" int paced_layernorm_bwd(const void* dy, int lddy, const void* x, int 
     const size_t need = sums ? paced_layernorm_workspace_bytes(M, d) : 0;
     PACED_CHECK_ARG(!sums || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 3) == 0),
                     "paced_layernorm_bwd: the column sums need a workspace of %zu bytes, got %zu", need, workspace_bytes);
-    const int grid = ln_bwd_grid(M);
     float* part = sums ? (float*)workspace : nullptr;
-    const int rc = f32 ? ln_bwd<float>(dy, lddy, x, ldx, w, mean, rstd, dres, ldr, dx, lddx, part, grid, M, d, (hipStream_t)stream)
-                       : ln_bwd<bf16>(dy, lddy, x, ldx, w, mean, rstd, dres, ldr, dx, lddx, part, grid, M, d, (hipStream_t)stream);
-    if (rc != PACED_OK || !sums) return rc;
-    hipLaunchKernelGGL(ln_cols_kernel, dim3((2 * d + 31) / 32), dim3(32 * COLS_LANES), 0, (hipStream_t)stream, part, grid, d, dw, db);
-    PACED_CHECK_LAUNCH();
-    return PACED_OK;
+    return f32 ? ln_bwd<float>(dy, lddy, x, ldx, w, mean, rstd, dres, ldr, dx, lddx, dw, db, part, M, d, (hipStream_t)stream)
+               : ln_bwd<bf16>(dy, lddy, x, ldx, w, mean, rstd, dres, ldr, dx, lddx, dw, db, part, M, d, (hipStream_t)stream);
 }
