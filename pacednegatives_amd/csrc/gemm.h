@@ -15,7 +15,7 @@ enum Epi : int {
     EPI_TOPK_FILTER = 8, // if acc >= thr[n]: cand[n][cnt[n]++] = key(acc, row_base + m)
     // ---- internal to the linear-head cross entropy (linear_ce.hip); rows m are tokens, columns n vocabulary entries
     EPI_CE_STATS = 9,    // part[n / W * ce_rows + m] = (max, sum of 2^(z - max)) of z = acc * alpha * log2 e over W columns but the label's
-                         // (W = 64; 32 for the 64x64 tiles); target[m] = the label's acc * alpha
+                         // (W = paced_gemm_stat_width(), 32 or 64); target[m] = the label's acc * alpha
     EPI_CE_GRAD = 10,    // C(bf16) = g[m] (2^(z - lse[m] log2 e) - [n is m's label]); columns N .. next multiple of 64 are zeros
     EPI_SLAB_F32 = 11    // C(f32) + split * strideC elements (+)= acc * alpha: one owner per element, no atomics
 };
@@ -73,7 +73,8 @@ __host__ __device__ __forceinline__ float topk_key_score(unsigned long long key)
 __host__ __device__ __forceinline__ unsigned int topk_key_row(unsigned long long key) { return ~(unsigned int)key; }
 
 // Launches the tiled kernel for (trans_a, trans_b, epilogue); arguments are already validated.
-extern "C" int paced_gemm_last_kernel(void);
+// columns per statistics group of the calling thread's most recent EPI_CE_STATS launch
+int paced_gemm_stat_width();
 int paced_gemm_launch(const GemmParams& p, bool trans_a, bool trans_b, int epilogue, int splits, hipStream_t stream);
 
 

@@ -1275,6 +1275,7 @@ int g_grid_limit = 0;    // 0 = one phased workgroup per CU; n > 0: at most n (p
 bool g_grid_env_read = false;
 struct CallOpts { int grid_limit = -1, tile = -1, ring = -1; };
 thread_local CallOpts t_call;
+thread_local int t_stat_width = 0;    // columns of a wave in this thread's most recent EPI_CE_STATS launch
 thread_local int t_last_kernel = 0;   // tile of this thread's most recent launch (64, 128, 256), +1 when the ring variant took it
 
 int eff_tile() { return t_call.tile >= 0 ? t_call.tile : g_force_tile; }
@@ -1307,6 +1308,7 @@ int launch_ring(const GemmParams& p, int ntm, int ntn, int total, hipStream_t st
     }
     hipLaunchKernelGGL((gemm_ring_kernel<Cfg, TA, TB, EPI, NS>), dim3(total), dim3(Cfg::WGM * Cfg::WGN * 64), smem, stream, p, ntm, ntn, total);
     t_last_kernel = Cfg::BM + 1;
+    t_stat_width = Cfg::NJ * 16;
     PACED_CHECK_LAUNCH();
     return PACED_OK;
 }
@@ -1351,11 +1353,15 @@ int launch_cfg(GemmParams p, int splits, hipStream_t stream) {
                 if (per_cu == 2) return launch_ring<Cfg, TA, TB, EPI, 4>(p, ntm, ntn, total, stream);
                 if (per_cu == 3) return launch_ring<Cfg, TA, TB, EPI, 3>(p, ntm, ntn, total, stream);
             } else {
-                if (per_cu == 1) return launch_ring<Cfg, TA, TB, EPI, 4>(p, ntm, ntn, total, stream);
-                // linear_ce.hip's products with one to two tiles per CU: two buffers a workgroup, two workgroups a CU (the
-                // single buffer's full wait per K step has nobody to hide it here: 272 tiles of 12 steps, 20.6 us)
-                if constexpr (EPI == EPI_CE_STATS || EPI == EPI_CE_GRAD || EPI == EPI_SLAB_F32 || (EPI == EPI_BF16 && TA && TB))
+                // linear_ce.hip's products.  One tile per CU: eight waves (64 of 1088 rows x 32128 entries 12.6 us, with four
+                // 14.4).  Up to two: four waves and two buffers, two workgroups a CU (272 tiles of 12 steps 16.0 us, with
+                // eight waves 16.0 to 20 with the gradient's epilogue; the single buffer's full wait per K step, which
+                // nobody hides here, 20.6).
+                if constexpr (EPI == EPI_CE_STATS || EPI == EPI_CE_GRAD || EPI == EPI_SLAB_F32 || (EPI == EPI_BF16 && TA && TB)) {
+                    if (per_cu == 1 && p.tile == 128) return launch_ring<CfgSmall8, TA, TB, EPI, 4>(p, ntm, ntn, total, stream);
                     if (per_cu == 2 && p.tile == 128) return launch_ring<Cfg, TA, TB, EPI, 2>(p, ntm, ntn, total, stream);
+                }
+                if (per_cu == 1) return launch_ring<Cfg, TA, TB, EPI, 4>(p, ntm, ntn, total, stream);
             }
         }
     }
@@ -1374,6 +1380,7 @@ int launch_cfg(GemmParams p, int splits, hipStream_t stream) {
     if constexpr (PHASED) hipLaunchKernelGGL((gemm_phased_kernel<TA, TB, EPI>), dim3(grid), dim3(512), smem, stream, p, ntm, ntn, total);
     else hipLaunchKernelGGL((gemm_bf16_kernel<Cfg, TA, TB, EPI>), dim3(grid), dim3(Cfg::WGM * Cfg::WGN * 64), smem, stream, p, ntm, ntn, total);
     t_last_kernel = Cfg::BM;
+    t_stat_width = Cfg::NJ * 16;
     PACED_CHECK_LAUNCH();
     return PACED_OK;
 }
@@ -1445,6 +1452,7 @@ extern "C" int paced_gemm_set_tile(int tile) {
     return PACED_OK;
 }
 
+int paced_gemm_stat_width() { return t_stat_width; }
 extern "C" int paced_gemm_last_kernel(void) { return t_last_kernel; }
 
 extern "C" long long paced_gemm_tile_bits_bytes(int M, int N) {

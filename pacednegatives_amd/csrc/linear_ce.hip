@@ -231,7 +231,7 @@ extern "C" int paced_linear_ce_fwd(const void* h, int ldh, const void* w, int ld
     p.ce_rows = R;
     const int rg = ce_logits(p, EPI_CE_STATS, (hipStream_t)stream);
     if (rg != PACED_OK) return rg;
-    const int width = paced_gemm_last_kernel() < 128 ? 32 : 64;           // columns of a wave in the tiles that were taken
+    const int width = paced_gemm_stat_width();
     const int groups = (V + width - 1) / width;
     if (R >= 2 * paced_cu_count())
         hipLaunchKernelGGL(ce_join_kernel<8>, dim3((R + 7) / 8), dim3(256), 0, (hipStream_t)stream, p.ce_part, groups, p.ce_target, labels, ignore_index, V, loss, lse, R);
