@@ -6,7 +6,6 @@ not match what its grid assumes.
 """
 from __future__ import annotations
 
-import contextlib
 import os
 
 import torch
@@ -46,19 +45,21 @@ def _rows2d(t, name):
     return t.stride(0)
 
 
-def _one_device(**tensors):
-    """The device that all given tensors (None: absent) live on, as a context for the launch: the current device, or a
-    switch to theirs.  Work then goes to that device's current stream."""
+def _elsewhere(**tensors):
+    """Checks that all given tensors (None: absent) live on one device; that device if it is not the current one, else None
+    (the caller then launches under ``torch.cuda.device``: work goes to that device's current stream)."""
     dev = None
     for name, t in tensors.items():
         if t is None:
             continue
-        if not t.is_cuda:
+        d = t.device
+        if d.type != "cuda":
             raise ValueError(f"{name} must be a device tensor")
-        if dev is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, the tensors before it on {dev}")
-        dev = t.device
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+        if dev is None:
+            dev = d
+        elif d != dev:
+            raise ValueError(f"{name} is on {d}, the tensors before it on {dev}")
+    return None if dev.index == torch.cuda.current_device() else dev
 
 
 def _rows_of(t, shape, dtype, name):
@@ -67,15 +68,17 @@ def _rows_of(t, shape, dtype, name):
         return 0
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if shape[1] > 1 and t.stride(1) != 1:
+    rows, d = shape
+    ld, inner = t.stride()
+    if d > 1 and inner != 1:
         raise ValueError(f"{name} must have unit inner stride, got strides {t.stride()}")
-    if shape[0] <= 1:
-        return shape[1]
-    if not shape[1] <= t.stride(0) < 2 ** 31:
+    if rows <= 1:
+        return d
+    if not d <= ld < 2 ** 31:
         raise ValueError(f"{name}: rows overlap or lie too far apart (strides {t.stride()})")
-    return t.stride(0)
+    return ld
 
 
 def _flat(t, n, dtype, name):
@@ -245,17 +248,20 @@ def layernorm_fwd(x, w, b, y, mean=None, rstd=None, *, eps=1e-5, res=None, xsum=
     """y = layer norm of x, or of x + res (written to ``xsum`` in the tensors' type: the backward pass's ``x``), weighted by w
     and b; bf16 or fp32 [M, d] rows.  ``mean`` and ``rstd`` (fp32 [M]) are what ``layernorm_bwd`` needs."""
     lib = _lib.load()
-    with _one_device(x=x, w=w, b=b, y=y, mean=mean, rstd=rstd, res=res, xsum=xsum):
-        if x.dim() != 2 or x.dtype not in (BF16, F32):
-            raise ValueError(f"x must be a bf16 or fp32 matrix, got {x.dtype} {tuple(x.shape)}")
-        if (res is None) != (xsum is None):
-            raise ValueError("res and xsum go together")
-        M, d = x.shape
-        ldx, ldy = _rows_of(x, (M, d), x.dtype, "x"), _rows_of(y, (M, d), x.dtype, "y")
-        ldr, lds = _rows_of(res, (M, d), x.dtype, "res"), _rows_of(xsum, (M, d), x.dtype, "xsum")
-        _flat(w, d, x.dtype, "w"); _flat(b, d, x.dtype, "b"); _flat(mean, M, F32, "mean"); _flat(rstd, M, F32, "rstd")
-        _lib.check(lib.paced_layernorm_fwd(_p(x), ldx, _p(res), ldr, _p(xsum), lds, _p(w), _p(b), _p(y), ldy, _p(mean), _p(rstd), M, d,
-                                           int(x.dtype == F32), eps, _stream()), "paced_layernorm_fwd")
+    other = _elsewhere(x=x, w=w, b=b, y=y, mean=mean, rstd=rstd, res=res, xsum=xsum)
+    if other is not None:
+        with torch.cuda.device(other):
+            return layernorm_fwd(x, w, b, y, mean, rstd, eps=eps, res=res, xsum=xsum)
+    if x.dim() != 2 or x.dtype not in (BF16, F32):
+        raise ValueError(f"x must be a bf16 or fp32 matrix, got {x.dtype} {tuple(x.shape)}")
+    if (res is None) != (xsum is None):
+        raise ValueError("res and xsum go together")
+    M, d = x.shape
+    ldx, ldy = _rows_of(x, (M, d), x.dtype, "x"), _rows_of(y, (M, d), x.dtype, "y")
+    ldr, lds = _rows_of(res, (M, d), x.dtype, "res"), _rows_of(xsum, (M, d), x.dtype, "xsum")
+    _flat(w, d, x.dtype, "w"); _flat(b, d, x.dtype, "b"); _flat(mean, M, F32, "mean"); _flat(rstd, M, F32, "rstd")
+    _lib.check(lib.paced_layernorm_fwd(_p(x), ldx, _p(res), ldr, _p(xsum), lds, _p(w), _p(b), _p(y), ldy, _p(mean), _p(rstd), M, d,
+                                       int(x.dtype == F32), eps, _stream()), "paced_layernorm_fwd")
     return y
 
 
@@ -263,17 +269,20 @@ def layernorm_bwd(dy, x, w, mean, rstd, dx, *, dres=None, dw=None, db=None, work
     """Backward of ``layernorm_fwd``; x is what was normalised.  dx = gradient through the norm (+ ``dres``); ``dw`` and ``db``
     (fp32 [d]) are added to, in a fixed order."""
     lib = _lib.load()
-    with _one_device(dy=dy, x=x, w=w, mean=mean, rstd=rstd, dx=dx, dres=dres, dw=dw, db=db):
-        if x.dim() != 2 or x.dtype not in (BF16, F32):
-            raise ValueError(f"x must be a bf16 or fp32 matrix, got {x.dtype} {tuple(x.shape)}")
-        M, d = x.shape
-        lddy, ldx, lddx = _rows_of(dy, (M, d), x.dtype, "dy"), _rows_of(x, (M, d), x.dtype, "x"), _rows_of(dx, (M, d), x.dtype, "dx")
-        ldr = _rows_of(dres, (M, d), x.dtype, "dres")
-        _flat(w, d, x.dtype, "w"); _flat(mean, M, F32, "mean"); _flat(rstd, M, F32, "rstd"); _flat(dw, d, F32, "dw"); _flat(db, d, F32, "db")
-        need = lib.paced_layernorm_workspace_bytes(M, d) if dw is not None or db is not None else 0
-        ws = _workspace(workspace, need, x.device)
-        _lib.check(lib.paced_layernorm_bwd(_p(dy), lddy, _p(x), ldx, _p(w), _p(mean), _p(rstd), _p(dres), ldr, _p(dx), lddx, _p(dw), _p(db),
-                                           M, d, int(x.dtype == F32), _p(ws), need, _stream()), "paced_layernorm_bwd")
+    other = _elsewhere(dy=dy, x=x, w=w, mean=mean, rstd=rstd, dx=dx, dres=dres, dw=dw, db=db)
+    if other is not None:
+        with torch.cuda.device(other):
+            return layernorm_bwd(dy, x, w, mean, rstd, dx, dres=dres, dw=dw, db=db, workspace=workspace)
+    if x.dim() != 2 or x.dtype not in (BF16, F32):
+        raise ValueError(f"x must be a bf16 or fp32 matrix, got {x.dtype} {tuple(x.shape)}")
+    M, d = x.shape
+    lddy, ldx, lddx = _rows_of(dy, (M, d), x.dtype, "dy"), _rows_of(x, (M, d), x.dtype, "x"), _rows_of(dx, (M, d), x.dtype, "dx")
+    ldr = _rows_of(dres, (M, d), x.dtype, "dres")
+    _flat(w, d, x.dtype, "w"); _flat(mean, M, F32, "mean"); _flat(rstd, M, F32, "rstd"); _flat(dw, d, F32, "dw"); _flat(db, d, F32, "db")
+    need = lib.paced_layernorm_workspace_bytes(M, d) if dw is not None or db is not None else 0
+    ws = _workspace(workspace, need, x.device)
+    _lib.check(lib.paced_layernorm_bwd(_p(dy), lddy, _p(x), ldx, _p(w), _p(mean), _p(rstd), _p(dres), ldr, _p(dx), lddx, _p(dw), _p(db),
+                                       M, d, int(x.dtype == F32), _p(ws), need, _stream()), "paced_layernorm_bwd")
     return dx
 
 
@@ -289,10 +298,15 @@ def act8_quantize(x, q=None, scale=None):
         q = torch.empty(T, n, dtype=U8, device=x.device)
     if scale is None:
         scale = torch.empty(blocks, n, dtype=U8, device=x.device)
-    with _one_device(x=x, q=q, scale=scale):
-        ldx = _rows_of(x, (T, n), BF16, "x")
-        _flat(q, T * n, U8, "q"); _flat(scale, blocks * n, U8, "scale")
-        _lib.check(lib.paced_act8_quantize(_p(x), ldx, _p(q), _p(scale), T, n, _stream()), "paced_act8_quantize")
+    other = _elsewhere(x=x, q=q, scale=scale)
+    if other is not None:
+        with torch.cuda.device(other):
+            return act8_quantize(x, q, scale)
+    ldx = _rows_of(x, (T, n), BF16, "x")
+    if q.shape != (T, n) or scale.shape != (blocks, n):
+        raise ValueError(f"q must hold the codes {(T, n)} and scale {(blocks, n)}, got {tuple(q.shape)} and {tuple(scale.shape)}")
+    _flat(q, T * n, U8, "q"); _flat(scale, blocks * n, U8, "scale")
+    _lib.check(lib.paced_act8_quantize(_p(x), ldx, _p(q), _p(scale), T, n, _stream()), "paced_act8_quantize")
     return q, scale
 
 
@@ -300,7 +314,7 @@ def _checkpoint(q, scale):
     if q.dim() != 2 or q.shape[1] % 16 or q.shape[1] == 0:
         raise ValueError(f"q must be [T, n] with n a multiple of 16, got {tuple(q.shape)}")
     T, n = q.shape
-    if tuple(scale.shape) != ((T + 31) // 32, n):
+    if scale.shape != ((T + 31) // 32, n):
         raise ValueError(f"scale must be [ceil(T/32), n] = {((T + 31) // 32, n)}, got {tuple(scale.shape)}")
     _flat(q, T * n, U8, "q"); _flat(scale, scale.numel(), U8, "scale")
     return T, n
@@ -309,9 +323,12 @@ def _checkpoint(q, scale):
 def act8_dequantize(q, scale, y):
     """The values of a checkpoint (bf16 [T, n]); nothing is rounded."""
     lib = _lib.load()
-    with _one_device(q=q, scale=scale, y=y):
-        T, n = _checkpoint(q, scale)
-        _lib.check(lib.paced_act8_dequantize(_p(q), _p(scale), _p(y), _rows_of(y, (T, n), BF16, "y"), T, n, _stream()), "paced_act8_dequantize")
+    other = _elsewhere(q=q, scale=scale, y=y)
+    if other is not None:
+        with torch.cuda.device(other):
+            return act8_dequantize(q, scale, y)
+    T, n = _checkpoint(q, scale)
+    _lib.check(lib.paced_act8_dequantize(_p(q), _p(scale), _p(y), _rows_of(y, (T, n), BF16, "y"), T, n, _stream()), "paced_act8_dequantize")
     return y
 
 
@@ -319,26 +336,29 @@ def act8_dweight(dy, q, scale, dw, *, accumulate=True, workspace=None):
     """dw (fp32 [out, in]) += dy^T x for the checkpoint x = (q, scale) of [T, in] and dy bf16 [T, out] (or head-major, see
     _operand); ``accumulate=False`` writes dw."""
     lib = _lib.load()
-    with _one_device(dy=dy, q=q, scale=scale, dw=dw):
-        T, N = _checkpoint(q, scale)
-        if dy.dtype != BF16:
-            raise ValueError(f"dy must be {BF16}, got {dy.dtype}")
-        if dy.dim() == 3:
-            rows, M, lddy, heads = _operand(dy, "dy")
-            if rows != T:
-                raise ValueError(f"dy has {rows} rows, the checkpoint {T}")
-            if dy.shape[0] == 1:
-                heads = T * 64                               # a single head may have any stride
-        else:
-            if dy.dim() != 2:
-                raise ValueError(f"dy must be [T, out] or head-major, got {tuple(dy.shape)}")
-            M, heads = dy.shape[1], 0
-            lddy = _rows_of(dy, (T, M), BF16, "dy")
-        lddw = _rows_of(dw, (M, N), F32, "dw")
-        need = lib.paced_act8_dweight_workspace_bytes(T, M, N, int(bool(accumulate)))
-        ws = _workspace(workspace, need, dy.device)
-        _lib.check(lib.paced_act8_dweight(_p(dy), lddy, heads, _p(q), _p(scale), _p(dw), lddw, T, M, N, int(bool(accumulate)), _p(ws), need,
-                                          _stream()), "paced_act8_dweight")
+    other = _elsewhere(dy=dy, q=q, scale=scale, dw=dw)
+    if other is not None:
+        with torch.cuda.device(other):
+            return act8_dweight(dy, q, scale, dw, accumulate=accumulate, workspace=workspace)
+    T, N = _checkpoint(q, scale)
+    if dy.dtype != BF16:
+        raise ValueError(f"dy must be {BF16}, got {dy.dtype}")
+    if dy.dim() == 3:
+        rows, M, lddy, heads = _operand(dy, "dy")
+        if rows != T:
+            raise ValueError(f"dy has {rows} rows, the checkpoint {T}")
+        if dy.shape[0] == 1:
+            heads = T * 64                               # a single head may have any stride
+    else:
+        if dy.dim() != 2:
+            raise ValueError(f"dy must be [T, out] or head-major, got {tuple(dy.shape)}")
+        M, heads = dy.shape[1], 0
+        lddy = _rows_of(dy, (T, M), BF16, "dy")
+    lddw = _rows_of(dw, (M, N), F32, "dw")
+    need = lib.paced_act8_dweight_workspace_bytes(T, M, N, int(bool(accumulate)))
+    ws = _workspace(workspace, need, dy.device)
+    _lib.check(lib.paced_act8_dweight(_p(dy), lddy, heads, _p(q), _p(scale), _p(dw), lddw, T, M, N, int(bool(accumulate)), _p(ws), need,
+                                      _stream()), "paced_act8_dweight")
     return dw
 
 
@@ -544,13 +564,16 @@ def linear_ce_fwd(h, w, labels, loss, lse=None, *, ignore_index=-100, scale=1.0,
     (h bf16 [R, d], w bf16 [V, d], labels int64 [R]); rows whose label is ``ignore_index`` or outside [0, V) give 0.
     ``lse`` (fp32 [R]) is what ``linear_ce_bwd`` needs."""
     lib = _lib.load()
-    with _one_device(h=h, w=w, labels=labels, loss=loss, lse=lse):
-        R, V, d, ldh, ldw = _head_operands(h, w, labels)
-        _flat(loss, R, F32, "loss"); _flat(lse, R, F32, "lse")
-        need = lib.paced_linear_ce_fwd_workspace_bytes(R, V)
-        ws = _workspace(workspace, need, h.device)
-        _lib.check(lib.paced_linear_ce_fwd(_p(h), ldh, _p(w), ldw, _p(labels), _p(loss), _p(lse), R, V, d, ignore_index, scale, _p(ws), need,
-                                           _stream()), "paced_linear_ce_fwd")
+    other = _elsewhere(h=h, w=w, labels=labels, loss=loss, lse=lse)
+    if other is not None:
+        with torch.cuda.device(other):
+            return linear_ce_fwd(h, w, labels, loss, lse, ignore_index=ignore_index, scale=scale, workspace=workspace)
+    R, V, d, ldh, ldw = _head_operands(h, w, labels)
+    _flat(loss, R, F32, "loss"); _flat(lse, R, F32, "lse")
+    need = lib.paced_linear_ce_fwd_workspace_bytes(R, V)
+    ws = _workspace(workspace, need, h.device)
+    _lib.check(lib.paced_linear_ce_fwd(_p(h), ldh, _p(w), ldw, _p(labels), _p(loss), _p(lse), R, V, d, ignore_index, scale, _p(ws), need,
+                                       _stream()), "paced_linear_ce_fwd")
     return loss
 
 
@@ -558,20 +581,23 @@ def linear_ce_bwd(h, w, labels, lse, grad_loss, dh=None, dw=None, *, ignore_inde
     """Gradients of sum(grad_loss * loss) of ``linear_ce_fwd``: ``dh`` (bf16 [R, d]) is written, ``dw`` [V, d] is written
     (bf16) or added to (fp32); either may be left out."""
     lib = _lib.load()
-    with _one_device(h=h, w=w, labels=labels, lse=lse, grad_loss=grad_loss, dh=dh, dw=dw):
-        R, V, d, ldh, ldw = _head_operands(h, w, labels)
-        _flat(lse, R, F32, "lse"); _flat(grad_loss, R, F32, "grad_loss")
-        lddh = _rows_of(dh, (R, d), BF16, "dh")
-        if dw is not None and dw.dtype not in (BF16, F32):
-            raise ValueError(f"dw must be bf16 or fp32, got {dw.dtype}")
-        f32 = dw is not None and dw.dtype == F32
-        lddw = _rows_of(dw, (V, d), F32 if f32 else BF16, "dw")
-        if dh is None and dw is None:
-            return None
-        need = lib.paced_linear_ce_bwd_workspace_bytes(R, V, d)
-        ws = _workspace(workspace, need, h.device)
-        _lib.check(lib.paced_linear_ce_bwd(_p(h), ldh, _p(w), ldw, _p(labels), _p(lse), _p(grad_loss), _p(dh), lddh, _p(dw), lddw, int(f32),
-                                           R, V, d, ignore_index, scale, _p(ws), need, _stream()), "paced_linear_ce_bwd")
+    other = _elsewhere(h=h, w=w, labels=labels, lse=lse, grad_loss=grad_loss, dh=dh, dw=dw)
+    if other is not None:
+        with torch.cuda.device(other):
+            return linear_ce_bwd(h, w, labels, lse, grad_loss, dh, dw, ignore_index=ignore_index, scale=scale, workspace=workspace)
+    R, V, d, ldh, ldw = _head_operands(h, w, labels)
+    _flat(lse, R, F32, "lse"); _flat(grad_loss, R, F32, "grad_loss")
+    lddh = _rows_of(dh, (R, d), BF16, "dh")
+    if dw is not None and dw.dtype not in (BF16, F32):
+        raise ValueError(f"dw must be bf16 or fp32, got {dw.dtype}")
+    f32 = dw is not None and dw.dtype == F32
+    lddw = _rows_of(dw, (V, d), F32 if f32 else BF16, "dw")
+    if dh is None and dw is None:
+        return None
+    need = lib.paced_linear_ce_bwd_workspace_bytes(R, V, d)
+    ws = _workspace(workspace, need, h.device)
+    _lib.check(lib.paced_linear_ce_bwd(_p(h), ldh, _p(w), ldw, _p(labels), _p(lse), _p(grad_loss), _p(dh), lddh, _p(dw), lddw, int(f32),
+                                       R, V, d, ignore_index, scale, _p(ws), need, _stream()), "paced_linear_ce_bwd")
     return dh
 
 
