@@ -268,8 +268,8 @@ __global__ void __launch_bounds__(256) act8_dw_kernel(DwParams p, int ntm, int n
 
 // 256x256 tiles: the phased kernel of gemm.hip (same ring order, phases, barriers and A halves) with B halves of codes: 8 KiB
 // instead of 16, one LDS-DMA instruction per wave instead of two, half the fragment reads; a fragment is converted behind its
-// phase's barrier.  Codes of a half: [64 tokens][128] bytes, 16-byte unit u of token k at u ^ (k & 7); half h holds the h-th 32
-// features of every 64.  With each step's first B half every wave fetches the scales of its own 64 features.
+// phase's barrier.  Codes of a half: [64 tokens][128] bytes, 16-byte unit u of token k at u ^ (k & 7) ^ ((k >> 3) & 1) (the
+// sixteen tokens that two lane groups gather lie on different banks); half h holds the h-th 32 features of every 64.  With each step's first B half every wave fetches the scales of its own 64 features.
 // Instructions in flight behind a phase's wait (the six youngest half-tiles; B half 0 and its scales 2, A halves 2, B half 1 1):
 // 11 after B half 0 and A half 0 were issued, 10 after B half 1 and A half 1.
 // LDS: ring slots 0, 2, .. 8 are B halves (5 x 8 KiB), 1, 3, .. 9 A halves (5 x 16 KiB), three sets of scales (a set is read in
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(512) act8_dw_phased_kernel(DwParams p, int ntm
     uint32_t offA[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) offA[i] = stage_offset<true, 128>((i * 8 + w) * 64 + lane, p.lddy, p.heads);
-    const int bk = (w * 64 + lane) >> 3, bc = ((w * 64 + lane) & 7) ^ (bk & 7);
+    const int bk = (w * 64 + lane) >> 3, bc = ((w * 64 + lane) & 7) ^ (bk & 7) ^ ((bk >> 3) & 1);
     const uint32_t offB = (uint32_t)(bk * p.N + (bc >> 1) * 64 + (bc & 1) * 16);
     // lanes 0-15: the first 32 tokens' scales of the wave's 64 features, 16-31: the second's, the rest outside every descriptor
     const uint32_t offS = lane < 32 ? (uint32_t)((lane >> 4) * p.N + wc * 64 + (lane & 15) * 4) : 0x80000000u;
@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(512) act8_dw_phased_kernel(DwParams p, int ntm
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int k = 8 * g + (i16 >> 1);
-            const uint32_t a = lb + (uint32_t)(k * 128 + (((wc * 2 + j) ^ (k & 7)) << 4) + (i16 & 1) * 8);
+            const uint32_t a = lb + (uint32_t)(k * 128 + (((wc * 2 + j) ^ (k & 7) ^ (g & 1)) << 4) + (i16 & 1) * 8);
             asm volatile("ds_read_b64_tr_b8 %0, %1" : "=v"(cb[j][0]) : "v"(a));
             asm volatile("ds_read_b64_tr_b8 %0, %1 offset:%2" : "=v"(cb[j][1]) : "v"(a), "n"(32 * 128));
             if (j == 0) {

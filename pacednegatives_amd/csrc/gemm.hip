@@ -32,38 +32,26 @@ __device__ __forceinline__ void* batch_c(const GemmParams& p, int b) {
 // by inline assembly that waits for itself: a load the compiler can see would drain the K loop's LDS-DMA (epilogue_rows_impl).
 constexpr float CE_LOG2E = 1.4426950408889634f;
 
-template <int MI, class T>
-__device__ __forceinline__ void ce_load_rows(const T* const (&src)[MI], T (&v)[MI]) {
+// A row's label goes through ce_columns; its log-sum-exp and weight, where wanted, are requested ahead of the labels' own block
+// and have arrived when that block's wait is over.
+__device__ __forceinline__ void ce_request(float& v, const float* src) { asm volatile("global_load_dword %0, %1, off" : "=v"(v) : "v"(src) : "memory"); }
+
+template <int MI>
+__device__ __forceinline__ void ce_load_labels(const u32x2* const (&src)[MI], u32x2 (&v)[MI]) {
     static_assert(MI == 2 || MI == 4 || MI == 8, "row blocks of a wave");
-    if constexpr (sizeof(T) == 8) {
-        if constexpr (MI == 8)
-            asm volatile("global_load_dwordx2 %0, %8, off\n\tglobal_load_dwordx2 %1, %9, off\n\tglobal_load_dwordx2 %2, %10, off\n\tglobal_load_dwordx2 %3, %11, off\n\t"
-                         "global_load_dwordx2 %4, %12, off\n\tglobal_load_dwordx2 %5, %13, off\n\tglobal_load_dwordx2 %6, %14, off\n\tglobal_load_dwordx2 %7, %15, off\n\t"
-                         "s_waitcnt vmcnt(0) ; hidden-load wait"
-                         : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
-                         : "v"(src[0]), "v"(src[1]), "v"(src[2]), "v"(src[3]), "v"(src[4]), "v"(src[5]), "v"(src[6]), "v"(src[7]) : "memory");
-        else if constexpr (MI == 4)
-            asm volatile("global_load_dwordx2 %0, %4, off\n\tglobal_load_dwordx2 %1, %5, off\n\tglobal_load_dwordx2 %2, %6, off\n\tglobal_load_dwordx2 %3, %7, off\n\t"
-                         "s_waitcnt vmcnt(0) ; hidden-load wait"
-                         : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]) : "v"(src[0]), "v"(src[1]), "v"(src[2]), "v"(src[3]) : "memory");
-        else
-            asm volatile("global_load_dwordx2 %0, %2, off\n\tglobal_load_dwordx2 %1, %3, off\n\ts_waitcnt vmcnt(0) ; hidden-load wait"
-                         : "=&v"(v[0]), "=&v"(v[1]) : "v"(src[0]), "v"(src[1]) : "memory");
-    } else {
-        if constexpr (MI == 8)
-            asm volatile("global_load_dword %0, %8, off\n\tglobal_load_dword %1, %9, off\n\tglobal_load_dword %2, %10, off\n\tglobal_load_dword %3, %11, off\n\t"
-                         "global_load_dword %4, %12, off\n\tglobal_load_dword %5, %13, off\n\tglobal_load_dword %6, %14, off\n\tglobal_load_dword %7, %15, off\n\t"
-                         "s_waitcnt vmcnt(0) ; hidden-load wait"
-                         : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
-                         : "v"(src[0]), "v"(src[1]), "v"(src[2]), "v"(src[3]), "v"(src[4]), "v"(src[5]), "v"(src[6]), "v"(src[7]) : "memory");
-        else if constexpr (MI == 4)
-            asm volatile("global_load_dword %0, %4, off\n\tglobal_load_dword %1, %5, off\n\tglobal_load_dword %2, %6, off\n\tglobal_load_dword %3, %7, off\n\t"
-                         "s_waitcnt vmcnt(0) ; hidden-load wait"
-                         : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]) : "v"(src[0]), "v"(src[1]), "v"(src[2]), "v"(src[3]) : "memory");
-        else
-            asm volatile("global_load_dword %0, %2, off\n\tglobal_load_dword %1, %3, off\n\ts_waitcnt vmcnt(0) ; hidden-load wait"
-                         : "=&v"(v[0]), "=&v"(v[1]) : "v"(src[0]), "v"(src[1]) : "memory");
-    }
+    if constexpr (MI == 8)
+        asm volatile("global_load_dwordx2 %0, %8, off\n\tglobal_load_dwordx2 %1, %9, off\n\tglobal_load_dwordx2 %2, %10, off\n\tglobal_load_dwordx2 %3, %11, off\n\t"
+                     "global_load_dwordx2 %4, %12, off\n\tglobal_load_dwordx2 %5, %13, off\n\tglobal_load_dwordx2 %6, %14, off\n\tglobal_load_dwordx2 %7, %15, off\n\t"
+                     "s_waitcnt vmcnt(0) ; hidden-load wait"
+                     : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+                     : "v"(src[0]), "v"(src[1]), "v"(src[2]), "v"(src[3]), "v"(src[4]), "v"(src[5]), "v"(src[6]), "v"(src[7]) : "memory");
+    else if constexpr (MI == 4)
+        asm volatile("global_load_dwordx2 %0, %4, off\n\tglobal_load_dwordx2 %1, %5, off\n\tglobal_load_dwordx2 %2, %6, off\n\tglobal_load_dwordx2 %3, %7, off\n\t"
+                     "s_waitcnt vmcnt(0) ; hidden-load wait"
+                     : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]) : "v"(src[0]), "v"(src[1]), "v"(src[2]), "v"(src[3]) : "memory");
+    else
+        asm volatile("global_load_dwordx2 %0, %2, off\n\tglobal_load_dwordx2 %1, %3, off\n\ts_waitcnt vmcnt(0) ; hidden-load wait"
+                     : "=&v"(v[0]), "=&v"(v[1]) : "v"(src[0]), "v"(src[1]) : "memory");
 }
 
 // labels of this lane's rows, as columns of the launch (ignored, or of another piece: outside [0, N))
@@ -74,7 +62,7 @@ __device__ __forceinline__ void ce_columns(const GemmParams& p, int m0, int wm, 
 #pragma unroll
     for (int i = 0; i < Cfg::MI; ++i)
         src[i] = reinterpret_cast<const u32x2*>(p.ce_labels + min(m0 + Cfg::moff(wm, i) + (lane & 15), p.M - 1));
-    ce_load_rows<Cfg::MI>(src, v);
+    ce_load_labels<Cfg::MI>(src, v);
 #pragma unroll
     for (int i = 0; i < Cfg::MI; ++i) {
         const long long label = (long long)(((unsigned long long)v[i][1] << 32) | v[i][0]);
@@ -87,30 +75,40 @@ __device__ __forceinline__ void ce_columns(const GemmParams& p, int m0, int wm, 
 template <class Cfg>
 __device__ __forceinline__ void ce_rows(const GemmParams& p, int m0, int wm, int lane, int (&col)[Cfg::MI], bool (&dead)[Cfg::MI],
                                         float (&lse2)[Cfg::MI], float (&g)[Cfg::MI]) {
-    ce_columns<Cfg>(p, m0, wm, lane, col, dead);
-    const float *srcl[Cfg::MI], *srcg[Cfg::MI];
 #pragma unroll
     for (int i = 0; i < Cfg::MI; ++i) {
         const int mc = min(m0 + Cfg::moff(wm, i) + (lane & 15), p.M - 1);
-        srcl[i] = p.ce_lse + mc;
-        srcg[i] = p.ce_g + mc;
+        ce_request(lse2[i], p.ce_lse + mc);
+        ce_request(g[i], p.ce_g + mc);
     }
-    ce_load_rows<Cfg::MI>(srcl, lse2);
-    ce_load_rows<Cfg::MI>(srcg, g);
+    ce_columns<Cfg>(p, m0, wm, lane, col, dead);
 #pragma unroll
-    for (int i = 0; i < Cfg::MI; ++i) lse2[i] *= CE_LOG2E;
+    for (int i = 0; i < Cfg::MI; ++i) {
+        asm volatile("" : "+v"(lse2[i]), "+v"(g[i]) :: "memory");          // arrived: not read before this point
+        lse2[i] *= CE_LOG2E;
+    }
 }
 
-// gradient of four consecutive columns n .. n + 3 of a row: g (2^(z - lse2) - [label])
+// gradient of four consecutive columns n .. n + 3 of a row: g (2^(z - lse2) - [label]).  SPECIAL: the label may be among the
+// wave's columns, the row ignored (its logits may be anything) or the columns past the vocabulary's end; without it a value
+// takes three instructions instead of eight (the caller asks once for a wave's 16 x 64 block).
+template <bool SPECIAL>
 __device__ __forceinline__ f32x4 ce_grad4(const GemmParams& p, const f32x4& a, float c, float lse2, float g, int col, bool dead, int n) {
     f32x4 o;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         float v = __builtin_amdgcn_exp2f(__builtin_fmaf(a[r], c, -lse2)) * g;
-        if (n + r == col) v -= g;
-        o[r] = dead || n + r >= p.N ? 0.f : v;       // (an ignored row's logits may be anything)
+        if (SPECIAL) {
+            if (n + r == col) v -= g;
+            v = dead || n + r >= p.N ? 0.f : v;
+        }
+        o[r] = v;
     }
     return o;
+}
+// whether a wave's block of columns nw .. nw + width - 1 needs SPECIAL
+__device__ __forceinline__ bool ce_special(const GemmParams& p, int col, bool dead, int nw, int width) {
+    return nw + width > p.N || __ballot(dead || (col >= nw && col < nw + width)) != 0;
 }
 
 template <int EPI>
@@ -398,12 +396,14 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, void* Cb, int m0, 
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
             const int m = m0 + Cfg::moff(wm, i) + (lane & 15);
+            const bool special = ce_special(p, col[i], dead[i], n0 + Cfg::noff(wn, 0), NJ * 16);
             if (m >= p.M) continue;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 const int n = n0 + Cfg::noff(wn, j) + (lane >> 4) * 4;
                 if (n >= ((p.N + 63) & ~63)) continue;
-                const f32x4 o = ce_grad4(p, acc[i][j], c, lse2[i], g[i], col[i], dead[i], n);
+                const f32x4 o = special ? ce_grad4<true>(p, acc[i][j], c, lse2[i], g[i], col[i], dead[i], n)
+                                        : ce_grad4<false>(p, acc[i][j], c, lse2[i], g[i], col[i], dead[i], n);
                 *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16*>(Cb) + (size_t)m * p.ldc + n) = __builtin_convertvector(o, bf16x4);
             }
         }
@@ -722,11 +722,15 @@ __device__ __forceinline__ void epilogue_rows_impl(const GemmParams& p, void* Cb
     // 16-row block i as bf16 in the MFMA layout (4 consecutive columns of one row per lane and 16-column group)
     auto convert = [&](int i, bf16x4 (&o)[4]) {
         const uint64_t drow = (uint64_t)(m0 + CfgPhased::moff(wr, i) + mw) * (uint64_t)p.N + (uint64_t)(n0 + wc * 64 + g * 4);
+        const bool special = EPI == EPI_CE_GRAD && ce_special(p, ccol[i], cdead[i], n0 + wc * 64, 64);
         const uint32_t qrow = (uint32_t)(drow >> 2);          // quad number: the host sends outputs of more than 2^34 elements elsewhere
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (EPI == EPI_CE_GRAD) {
-                o[j] = __builtin_convertvector(ce_grad4(p, acc[i][j], p.alpha * CE_LOG2E, clse[i], cg[i], ccol[i], cdead[i], n0 + wc * 64 + j * 16 + g * 4), bf16x4);
+                const int n = n0 + wc * 64 + j * 16 + g * 4;
+                const f32x4 v = special ? ce_grad4<true>(p, acc[i][j], p.alpha * CE_LOG2E, clse[i], cg[i], ccol[i], cdead[i], n)
+                                        : ce_grad4<false>(p, acc[i][j], p.alpha * CE_LOG2E, clse[i], cg[i], ccol[i], cdead[i], n);
+                o[j] = __builtin_convertvector(v, bf16x4);
                 continue;
             }
             f32x4 v = acc[i][j] * scale;
