@@ -128,12 +128,15 @@ double dh_us(int R, int d, int steps, int* tile, int* slices) {
     return best;
 }
 
-// Pieces of the vocabulary: P takes at most 256 MiB (256 columns at least).  Where it takes several, sixteen widths between
+// Pieces of the vocabulary: P takes at most 256 MiB (256 columns at least), a piece of the weights 2 GiB (the products address
+// a transposed operand with 32-bit byte offsets).  Where it takes several, sixteen widths between
 // half and all of that are compared by the rounds of tiles that they come to.
 struct CePlan { int piece, ldp, slabs, dh_tile; };
 CePlan ce_plan(int R, int V, int d) {
     CePlan pl;
     long long fit = (256ll << 20) / 2 / (R > 0 ? R : 1) / 256;       // in tiles of 256 columns
+    const long long reach = (1ll << 30) / d / 256;
+    if (fit > reach) fit = reach;
     if (fit < 1) fit = 1;
     long long piece = fit * 256;
     if (piece >= V) piece = V;
@@ -206,6 +209,7 @@ int ce_check(const char* who, const void* h, int ldh, const void* w, int ldw, co
     PACED_CHECK_ARG(h && w && labels, "%s: null operand", who);
     PACED_CHECK_ARG(ldh >= d && ldw >= d && ldh % 8 == 0 && ldw % 8 == 0 && (((uintptr_t)h | (uintptr_t)w) & 15) == 0,
                     "%s: h and w need 16-byte aligned rows, strides of at least d and multiples of 8 (ldh=%d ldw=%d)", who, ldh, ldw);
+    PACED_CHECK_ARG(ldh <= 1 << 22 && ldw <= 1 << 22, "%s: a tile of 256 rows must span less than 4 GiB: row strides up to 2^22 (ldh=%d ldw=%d)", who, ldh, ldw);
     return PACED_OK;
 }
 
@@ -267,8 +271,8 @@ extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ld
     PACED_CHECK_ARG(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
                     "paced_linear_ce_bwd: a 16-byte aligned workspace of %zu bytes is needed, got %zu", need, workspace_bytes);
     // a transposed operand is addressed with 32-bit byte offsets from its first row
-    PACED_CHECK_ARG((unsigned long long)R * (ldh > pl.ldp ? ldh : pl.ldp) < (1ull << 31) && (unsigned long long)pl.piece * ldw < (1ull << 31),
-                    "paced_linear_ce_bwd: %d rows of stride %d span more than 4 GiB; pass fewer rows at a time", R, ldh);
+    PACED_CHECK_ARG((unsigned long long)R * (ldh > pl.ldp ? ldh : pl.ldp) < (1ull << 31), "paced_linear_ce_bwd: %d rows of h with a stride of %d span 4 GiB or more; pass fewer at a time", R, ldh);
+    PACED_CHECK_ARG((unsigned long long)pl.piece * ldw < (1ull << 31), "paced_linear_ce_bwd: %d rows of w with a stride of %d span 4 GiB or more; pass w with a smaller stride", pl.piece, ldw);
     bf16* P = (bf16*)workspace;
     float* slabs = (float*)((char*)workspace + round256((size_t)R * pl.ldp * 2));
     for (int v0 = 0; v0 < V; v0 += pl.piece) {

@@ -74,7 +74,8 @@ def ce_bwd(lib, **kw):
 
 
 @pytest.mark.parametrize("kw,words", [(dict(d=96), "multiple of 64"), (dict(d=0), "multiple of 64"), (dict(V=0), "V > 0"), (dict(R=-1), "R >= 0"), (dict(h=0), "null"), (dict(labels=0), "null"),
-                                      (dict(h=ODD), "aligned"), (dict(ldw=68), "multiples of 8"), (dict(ldh=56), "at least d")])
+                                      (dict(h=ODD), "aligned"), (dict(ldw=68), "multiples of 8"), (dict(ldh=56), "at least d"), (dict(ldh=1 << 23), "2^22"),
+                                      (dict(ldw=1 << 23), "2^22")])
 def test_linear_ce(lib, kw, words):
     refused(lib, ce_fwd(lib, **kw), words)
     refused(lib, ce_bwd(lib, **kw), words)
