@@ -8,6 +8,9 @@
 // is a bf16 value and reading back rounds nothing.
 // Blocks run along the tokens because a weight gradient contracts over tokens: all eight values of a lane's MFMA fragment
 // (eight tokens of one feature) share one scale, and v_cvt_scalef32_pk_bf16_fp8 applies it while it converts.
+// Writing and reading are bound by memory: 139264 x 768 in 51.5 us (6.3 TB/s) and 55 us (5.9 TB/s).  The gradient is bound by the
+// matrix cores where tokens are many: 2304 x 768 from 139264 tokens in 411 us with the slabs' sum, 1.20 PFLOP/s (the bf16
+// products of gemm.hip reach 1.25 to 1.35 on large squares, the vendor's 1.39); 512 x 2048 from 1001 tokens in 10.4 us, by latency.
 #include "gemm_tiles.h"
 
 namespace {
@@ -16,71 +19,44 @@ constexpr int QBLOCK = 32;                 // tokens per scale
 constexpr int MIN_CODE = 127 - 117, MAX_CODE = 127 + 120, NAN_CODE = 255;
 
 // ------------------------------------------------------------------------------------------------ writing and reading
-// One thread per 32 tokens x 2 W features: 32 loads of 4 W bytes in flight, the maxima in its own registers (integer maxima of
-// the magnitudes' bits, two features to a register), no exchange between lanes.  W = 4 moves 16-byte pieces; where that leaves
-// most compute units without a wave, W = 1 cuts the work of a thread to a quarter.
+// One thread per 32 tokens x 2 features: 32 loads of 4 bytes in flight (256-byte runs of a wave), the maxima in its own
+// registers (integer maxima of the magnitudes' bits), no exchange between lanes.  Wider pieces measured slower at every size:
+// 139264 x 768 in 51.5 us with 2 features a thread, 54 with 4, 57 with 8; 300 x 512 in 5.2, 5.8 and 7.0 (fewer waves).
 typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
-template <int W> struct Words;
-template <> struct Words<4> {
-    typedef u32x4 in;
-    typedef u32x2 out;
-    static __device__ __forceinline__ uint32_t get(in v, int j) { return v[j]; }
-    static __device__ __forceinline__ out pack(const uint32_t (&b)[4]) { return out{b[0] | (b[1] << 16), b[2] | (b[3] << 16)}; }
-};
-template <> struct Words<1> {
-    typedef uint32_t in;
-    typedef unsigned short out;
-    static __device__ __forceinline__ uint32_t get(in v, int) { return v; }
-    static __device__ __forceinline__ out pack(const uint32_t (&b)[1]) { return (out)b[0]; }
-};
-template <int W>
 __global__ void __launch_bounds__(256) act8_quantize_kernel(const bf16* __restrict__ x, int ldx, unsigned char* __restrict__ q,
                                                             unsigned char* __restrict__ scale, int T, int n, int nblk) {
-    typedef typename Words<W>::in In;
-    typedef typename Words<W>::out Out;
-    const int chunks = n / (2 * W);
+    const int chunks = n >> 1;
     const long long total = (long long)nblk * chunks;
     for (long long id = (long long)blockIdx.x * 256 + threadIdx.x; id < total; id += (long long)gridDim.x * 256) {
         const int blk = (int)(id / chunks), c = (int)(id - (long long)blk * chunks);
         const int rows = min(QBLOCK, T - blk * QBLOCK);
-        const bf16* src = x + (size_t)blk * QBLOCK * ldx + c * 2 * W;
-        In v[QBLOCK];
+        const bf16* src = x + (size_t)blk * QBLOCK * ldx + c * 2;
+        uint32_t v[QBLOCK];
 #pragma unroll
-        for (int r = 0; r < QBLOCK; ++r) v[r] = r < rows ? __builtin_nontemporal_load(reinterpret_cast<const In*>(src + (size_t)r * ldx)) : In{};
-        u16x2 top[W] = {};
+        for (int r = 0; r < QBLOCK; ++r) v[r] = r < rows ? __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(src + (size_t)r * ldx)) : 0u;
+        u16x2 top = {};
 #pragma unroll
-        for (int r = 0; r < QBLOCK; ++r)
+        for (int r = 0; r < QBLOCK; ++r) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v[r] & 0x7fff7fffu));
+        float inv[2], lim[2];
+        uint32_t nan = 0, code = 0;        // codes that make a block NaN, scale bytes
 #pragma unroll
-            for (int j = 0; j < W; ++j) top[j] = __builtin_elementwise_max(top[j], __builtin_bit_cast(u16x2, Words<W>::get(v[r], j) & 0x7fff7fffu));
-        float inv[2 * W], lim[2 * W];
-        uint32_t nan[W], code[W];          // codes that make a block NaN, scale bytes: two features to a word
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-            nan[j] = code[j] = 0;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int bits = top[j][e];
-                int k = (bits >> 7) - 8 + ((bits & 0x7f) > 0x60 ? 1 : 0);        // 448 = 1.75 * 2^8
-                k = max(k, MIN_CODE);
-                inv[2 * j + e] = __uint_as_float((uint32_t)(254 - k) << 23);
-                lim[2 * j + e] = k == MAX_CODE ? 240.f : 448.f;
-                if (bits >= 0x7f80) { nan[j] |= 0x7fu << (8 * e); k = NAN_CODE; inv[2 * j + e] = 0.f; }
-                code[j] |= (uint32_t)k << (8 * e);
-            }
+        for (int e = 0; e < 2; ++e) {
+            const int bits = top[e];
+            int k = (bits >> 7) - 8 + ((bits & 0x7f) > 0x60 ? 1 : 0);        // 448 = 1.75 * 2^8
+            k = max(k, MIN_CODE);
+            inv[e] = __uint_as_float((uint32_t)(254 - k) << 23);
+            lim[e] = k == MAX_CODE ? 240.f : 448.f;
+            if (bits >= 0x7f80) { nan |= 0x7fu << (8 * e); k = NAN_CODE; inv[e] = 0.f; }
+            code |= (uint32_t)k << (8 * e);
         }
-        *reinterpret_cast<Out*>(scale + (size_t)blk * n + c * 2 * W) = Words<W>::pack(code);
-        unsigned char* dst = q + (size_t)blk * QBLOCK * n + c * 2 * W;
+        *reinterpret_cast<unsigned short*>(scale + (size_t)blk * n + c * 2) = (unsigned short)code;
+        unsigned char* dst = q + (size_t)blk * QBLOCK * n + c * 2;
 #pragma unroll
         for (int r = 0; r < QBLOCK; ++r) {
-            uint32_t o[W];
-#pragma unroll
-            for (int j = 0; j < W; ++j) {
-                const uint32_t u = Words<W>::get(v[r], j);
-                const float lo = __uint_as_float(u << 16) * inv[2 * j], hi = __uint_as_float(u & 0xffff0000u) * inv[2 * j + 1];
-                o[j] = ((uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(__builtin_amdgcn_fmed3f(lo, -lim[2 * j], lim[2 * j]),
-                                                                   __builtin_amdgcn_fmed3f(hi, -lim[2 * j + 1], lim[2 * j + 1]), 0, false) & 0xffffu) | nan[j];
-            }
-            if (r < rows) __builtin_nontemporal_store(Words<W>::pack(o), reinterpret_cast<Out*>(dst + (size_t)r * n));
+            const float lo = __uint_as_float(v[r] << 16) * inv[0], hi = __uint_as_float(v[r] & 0xffff0000u) * inv[1];
+            const uint32_t o = ((uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(__builtin_amdgcn_fmed3f(lo, -lim[0], lim[0]),
+                                                                           __builtin_amdgcn_fmed3f(hi, -lim[1], lim[1]), 0, false) & 0xffffu) | nan;
+            if (r < rows) __builtin_nontemporal_store((unsigned short)o, reinterpret_cast<unsigned short*>(dst + (size_t)r * n));
         }
     }
 }
@@ -473,9 +449,10 @@ __global__ void __launch_bounds__(256) slab_sum_kernel(const float* __restrict__
     }
 }
 
-// Which tiles, and how many slices of the tokens.  256x256 tiles run at about three times the rate of 64x64 ones, so they are
+// Which tiles, and how many slices of the tokens.  256x256 tiles run at almost three times the rate of 64x64 ones, so they are
 // taken when they waste less than that at the output's edges and when tiles times slices (of 12 K steps or more) give most
-// compute units one.
+// compute units one.  Both sides, slabs' sum apart: 139264 tokens, 2304 x 768 in 468 us against 1160, 17408, 768 x 2048 in 61
+// against 89, 4352, 2304 x 768 in 36.6 against 36.8; but 8704, 768 x 768 in 34 against 23, 1001, 512 x 2048 in 35 against 10.5.
 struct DwPlan { int tile, ntm, ntn, splits, k_per_split; };
 DwPlan dw_plan(int T, int M, int N) {
     DwPlan pl;
@@ -514,13 +491,8 @@ extern "C" int paced_act8_quantize(const void* x, int ldx, void* q, void* scale,
     PACED_CHECK_ARG(ldx >= n && ldx % 8 == 0 && (((uintptr_t)x | (uintptr_t)q | (uintptr_t)scale) & 15) == 0,
                     "paced_act8_quantize: 16-byte aligned operands and a row stride of at least n and a multiple of 8 are needed (ldx=%d)", ldx);
     const int nblk = (T + QBLOCK - 1) / QBLOCK;
-    const long long wide = (long long)nblk * (n >> 3);
-    if (wide >= 256LL * paced_cu_count())
-        hipLaunchKernelGGL(act8_quantize_kernel<4>, dim3(flat_blocks(wide)), dim3(256), 0, (hipStream_t)stream,
-                           (const bf16*)x, ldx, (unsigned char*)q, (unsigned char*)scale, T, n, nblk);
-    else
-        hipLaunchKernelGGL(act8_quantize_kernel<1>, dim3(flat_blocks(wide * 4)), dim3(256), 0, (hipStream_t)stream,
-                           (const bf16*)x, ldx, (unsigned char*)q, (unsigned char*)scale, T, n, nblk);
+    hipLaunchKernelGGL(act8_quantize_kernel, dim3(flat_blocks((long long)nblk * (n >> 1))), dim3(256), 0, (hipStream_t)stream,
+                       (const bf16*)x, ldx, (unsigned char*)q, (unsigned char*)scale, T, n, nblk);
     PACED_CHECK_LAUNCH();
     return PACED_OK;
 }

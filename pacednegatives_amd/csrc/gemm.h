@@ -49,6 +49,8 @@ struct GemmParams {
     const long long* ce_labels;   // [M]; a label counts when it is not ce_ignore and lies in [0, ce_vocab)
     const float* ce_lse;          // [M]
     const float* ce_g;            // [M]
+    float* ce_err;                // [M] EPI_CE_GRAD: what the label's entry lost in its rounding (rows with a label among the columns)
+    bf16* ce_lo;                  // EPI_CE_GRAD, small tiles: what every entry lost, in bf16, laid out as C (NULL: not wanted)
     f32x2* ce_part;
     float* ce_target;
     long long ce_ignore;
@@ -73,6 +75,8 @@ __host__ __device__ __forceinline__ float topk_key_score(unsigned long long key)
 __host__ __device__ __forceinline__ unsigned int topk_key_row(unsigned long long key) { return ~(unsigned int)key; }
 
 // Launches the tiled kernel for (trans_a, trans_b, epilogue); arguments are already validated.
+// tile edge that paced_gemm_set_tile has forced (0: none)
+int paced_gemm_forced_tile();
 // columns per statistics group of the calling thread's most recent EPI_CE_STATS launch
 int paced_gemm_stat_width();
 int paced_gemm_launch(const GemmParams& p, bool trans_a, bool trans_b, int epilogue, int splits, hipStream_t stream);

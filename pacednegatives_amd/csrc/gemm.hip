@@ -92,14 +92,18 @@ __device__ __forceinline__ void ce_rows(const GemmParams& p, int m0, int wm, int
 // gradient of four consecutive columns n .. n + 3 of a row: g (2^(z - lse2) - [label]).  SPECIAL: the label may be among the
 // wave's columns, the row ignored (its logits may be anything) or the columns past the vocabulary's end; without it a value
 // takes three instructions instead of eight (the caller asks once for a wave's 16 x 64 block).
+// The label's entry, nearly -g for most rows, dominates dh: what its rounding to bf16 loses is kept for the kernel that finishes dh.
 template <bool SPECIAL>
-__device__ __forceinline__ f32x4 ce_grad4(const GemmParams& p, const f32x4& a, float c, float lse2, float g, int col, bool dead, int n) {
+__device__ __forceinline__ f32x4 ce_grad4(const GemmParams& p, const f32x4& a, float c, float lse2, float g, int col, bool dead, int m, int n) {
     f32x4 o;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         float v = __builtin_amdgcn_exp2f(__builtin_fmaf(a[r], c, -lse2)) * g;
         if (SPECIAL) {
-            if (n + r == col) v -= g;
+            if (n + r == col) {
+                v -= g;
+                if (m < p.M && col < p.N) p.ce_err[m] = v - bf2f(f2bf(v));
+            }
             v = dead || n + r >= p.N ? 0.f : v;
         }
         o[r] = v;
@@ -402,9 +406,11 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, void* Cb, int m0, 
             for (int j = 0; j < NJ; ++j) {
                 const int n = n0 + Cfg::noff(wn, j) + (lane >> 4) * 4;
                 if (n >= ((p.N + 63) & ~63)) continue;
-                const f32x4 o = special ? ce_grad4<true>(p, acc[i][j], c, lse2[i], g[i], col[i], dead[i], n)
-                                        : ce_grad4<false>(p, acc[i][j], c, lse2[i], g[i], col[i], dead[i], n);
-                *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16*>(Cb) + (size_t)m * p.ldc + n) = __builtin_convertvector(o, bf16x4);
+                const f32x4 o = special ? ce_grad4<true>(p, acc[i][j], c, lse2[i], g[i], col[i], dead[i], m, n)
+                                        : ce_grad4<false>(p, acc[i][j], c, lse2[i], g[i], col[i], dead[i], m, n);
+                const bf16x4 hi = __builtin_convertvector(o, bf16x4);
+                *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16*>(Cb) + (size_t)m * p.ldc + n) = hi;
+                if (p.ce_lo) *reinterpret_cast<bf16x4*>(p.ce_lo + (size_t)m * p.ldc + n) = __builtin_convertvector(o - __builtin_convertvector(hi, f32x4), bf16x4);
             }
         }
         return;
@@ -727,9 +733,9 @@ __device__ __forceinline__ void epilogue_rows_impl(const GemmParams& p, void* Cb
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (EPI == EPI_CE_GRAD) {
-                const int n = n0 + wc * 64 + j * 16 + g * 4;
-                const f32x4 v = special ? ce_grad4<true>(p, acc[i][j], p.alpha * CE_LOG2E, clse[i], cg[i], ccol[i], cdead[i], n)
-                                        : ce_grad4<false>(p, acc[i][j], p.alpha * CE_LOG2E, clse[i], cg[i], ccol[i], cdead[i], n);
+                const int m = m0 + CfgPhased::moff(wr, i) + mw, n = n0 + wc * 64 + j * 16 + g * 4;
+                const f32x4 v = special ? ce_grad4<true>(p, acc[i][j], p.alpha * CE_LOG2E, clse[i], cg[i], ccol[i], cdead[i], m, n)
+                                        : ce_grad4<false>(p, acc[i][j], p.alpha * CE_LOG2E, clse[i], cg[i], ccol[i], cdead[i], m, n);
                 o[j] = __builtin_convertvector(v, bf16x4);
                 continue;
             }
@@ -1456,6 +1462,7 @@ extern "C" int paced_gemm_set_tile(int tile) {
     return PACED_OK;
 }
 
+int paced_gemm_forced_tile() { return eff_tile(); }
 int paced_gemm_stat_width() { return t_stat_width; }
 extern "C" int paced_gemm_last_kernel(void) { return t_last_kernel; }
 

@@ -5,11 +5,17 @@
 // a second kernel that joins them; the logits never leave the registers.  The label's term is kept out of the sums, so that
 // a confident row's loss log(1 + sum of the others / its own) keeps its relative precision.
 // Backward: the vocabulary goes by in pieces.  A piece's logits are computed again and leave as P in bf16 (the MFMA operand
-// type; half a step of 2^-8 relative to each entry, as paced_cross_entropy's dlogits), which feeds the two other products.
+// type; half a step of 2^-8 relative to each entry, as paced_cross_entropy's dlogits), which feeds the two other products.  What
+// the label's entry, the largest of a row, loses in that rounding is given back where dh is finished; up to 64 rows, where
+// few addends average the loss in dw, P's low part is kept too (ce_dw_few_kernel).
 // dh is summed over pieces and slices of a piece in fp32 slabs with one owner per element, dw is complete with its piece:
 // nothing is added atomically, equal inputs give equal bits.
-// Matrix-core bound: 2 R V d operations forward, three times that backward.
+// Matrix-core bound: 2 R V d operations forward, three times that backward.  Measured, loss and both gradients: 8192 rows x
+// 50001 entries x 1024 in 3.0 ms (1.12 PFLOP/s over the four products, the statistics alone 1.1), 1088 x 32128 x 768 in 254 us
+// (0.85 PFLOP/s: 4.25 x 125.5 tiles of 256 do not fill whole rounds of 256 compute units); the loss of 16 rows 15 us, of which
+// the weights' 49 MB take 11.
 #include "gemm.h"
+#include "gemm_tiles.h"
 #include <cmath>
 
 namespace {
@@ -68,8 +74,11 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const f32x2* __restrict__ 
     if (lse) lse[row] = t + l;
 }
 
-// dh = bf16 of the slabs' sum, slab by slab
-__global__ void __launch_bounds__(256) ce_dh_kernel(const float* __restrict__ slabs, int count, long long slab, bf16* __restrict__ dh, int lddh, int R, int d) {
+// dh = bf16 of the slabs' sum, slab by slab, and of scale err[r] w[label], the label's entry's share that P's rounding lost
+// (labels NULL: the sum alone)
+__global__ void __launch_bounds__(256) ce_dh_kernel(const float* __restrict__ slabs, int count, long long slab, bf16* __restrict__ dh, int lddh, int R, int d,
+                                                    const long long* __restrict__ labels, long long ignore, int V, const float* __restrict__ err,
+                                                    const bf16* __restrict__ w, int ldw, float scale) {
     const int d8 = d >> 3;
     const long long total = (long long)R * d8;
     for (long long id = (long long)blockIdx.x * 256 + threadIdx.x; id < total; id += (long long)gridDim.x * 256) {
@@ -80,10 +89,81 @@ __global__ void __launch_bounds__(256) ce_dh_kernel(const float* __restrict__ sl
             a += *reinterpret_cast<const f32x4*>(src);
             b += *reinterpret_cast<const f32x4*>(src + 4);
         }
+        if (labels) {
+            const long long label = labels[r];
+            if (label != ignore && label >= 0 && label < V) {
+                const bf16x8 x = *reinterpret_cast<const bf16x8*>(w + (size_t)label * ldw + c * 8);
+                const float e = scale * err[r];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { a[j] += e * bf2f(x[j]); b[j] += e * bf2f(x[4 + j]); }
+            }
+        }
         bf16x8 o;
 #pragma unroll
         for (int j = 0; j < 4; ++j) { o[j] = f2bf(a[j]); o[4 + j] = f2bf(b[j]); }
         *reinterpret_cast<bf16x8*>(dh + (size_t)r * lddh + c * 8) = o;
+    }
+}
+
+// dw (+)= scale (hi + lo)^T h for R <= 64 rows: hi, lo [R][ldp] bf16, the two parts of P.  A workgroup makes 64 entries x 256
+// features: P's parts and h come into LDS whole (LDS-DMA; rows past R read as zeros), a wave takes 16 entries, and an MFMA's 64
+// rows are all there is to contract, so the kernel is bound by writing dw.  The MFMA's sixteen columns are taken as four
+// fours, eight apart, so that two products leave a lane eight consecutive features of one entry: 16-byte stores.
+constexpr int FEW = 64, FEW_P = 8192, FEW_H = 32768;
+template <bool F32>
+__global__ void __launch_bounds__(256) ce_dw_few_kernel(const bf16* __restrict__ hi, const bf16* __restrict__ lo, int ldp, const bf16* __restrict__ h, int ldh,
+                                                        void* __restrict__ dw, int lddw, int R, int n, int d, float scale) {
+    __shared__ __attribute__((aligned(16))) char smem[2 * FEW_P + FEW_H];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int v0 = blockIdx.x * 64, d0 = blockIdx.y * 256;
+    const int cols = min(256, d - d0);                           // a multiple of 64
+    const auto rh = __builtin_amdgcn_make_buffer_rsrc((void*)(hi + v0), 0, (uint32_t)(((size_t)(R - 1) * ldp + 64) * 2), 0x00020000);
+    const auto rl = __builtin_amdgcn_make_buffer_rsrc((void*)(lo + v0), 0, (uint32_t)(((size_t)(R - 1) * ldp + 64) * 2), 0x00020000);
+    const auto rx = __builtin_amdgcn_make_buffer_rsrc((void*)(h + d0), 0, (uint32_t)(((size_t)(R - 1) * ldh + cols) * 2), 0x00020000);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t off = stage_offset<true, 64>((i * 4 + w) * 64 + lane, ldp);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rh, LDS_PTR(smem + (i * 4 + w) * 1024), 16, off, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rl, LDS_PTR(smem + FEW_P + (i * 4 + w) * 1024), 16, off, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)                                  // (columns past d: a neighbour's values, not stored)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, LDS_PTR(smem + 2 * FEW_P + (i * 4 + w) * 1024), 16, stage_offset<true, 256>((i * 4 + w) * 64 + lane, ldh), 0, 0, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    bf16x8 a[2][2];                                              // [part][32 rows]
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+        a[0][kk] = read_frag<true, 64>(smem, w * 16, kk, lane);
+        a[1][kk] = read_frag<true, 64>(smem + FEW_P, w * 16, kk, lane);
+    }
+    const int g = lane >> 4, i16 = lane & 15, q = i16 >> 2, piece = i16 & 3;
+    const int hk = q | ((g & 1) << 2);
+    const int v = v0 + w * 16 + i16;
+    for (int nb = 0; nb < cols / 32; ++nb) {
+        f32x4 acc[2] = {};
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                // fragment of features nb * 32 + 8 piece + 4 b ..: rows kk * 32 + 8 g ..+7 (image of gemm_tiles.h, 256 columns)
+                const char* at = smem + 2 * FEW_P + (kk * 32 + 8 * g + q) * 512 + (((nb * 2 + (piece >> 1)) ^ hk) << 5) + ((piece & 1) * 8 + b * 4) * 2;
+                const bf16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)at);
+                const bf16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(at + 4 * 512));
+                const bf16x8 x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+                acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, a[1][kk], acc[b], 0, 0, 0);
+                acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, a[0][kk], acc[b], 0, 0, 0);
+            }
+        if (v >= n) continue;
+        const int c = d0 + nb * 32 + g * 8;
+        if (F32) {
+            float* out = (float*)dw + (size_t)v * lddw + c;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) *reinterpret_cast<f32x4*>(out + 4 * b) += acc[b] * scale;
+        } else {
+            const bf16x4 o0 = __builtin_convertvector(acc[0] * scale, bf16x4), o1 = __builtin_convertvector(acc[1] * scale, bf16x4);
+            __builtin_nontemporal_store(__builtin_shufflevector(o0, o1, 0, 1, 2, 3, 4, 5, 6, 7), reinterpret_cast<bf16x8*>((bf16*)dw + (size_t)v * lddw + c));
+        }
     }
 }
 
@@ -196,7 +276,7 @@ int ce_logits(GemmParams p, int epilogue, hipStream_t s) {
             rest.A += (size_t)full * p.lda;
             rest.ce_labels += full;
             if (epilogue == EPI_CE_STATS) { rest.ce_part += full; rest.ce_target += full; }
-            else { rest.ce_lse += full; rest.ce_g += full; rest.C = (bf16*)rest.C + (size_t)full * p.ldc; }
+            else { rest.ce_lse += full; rest.ce_g += full; rest.ce_err += full; rest.C = (bf16*)rest.C + (size_t)full * p.ldc; }
             return paced_gemm_launch(rest, false, false, epilogue, 1, s);
         }
     }
@@ -248,7 +328,7 @@ extern "C" int paced_linear_ce_fwd(const void* h, int ldh, const void* w, int ld
 extern "C" size_t paced_linear_ce_bwd_workspace_bytes(int R, int V, int d) {
     if (R <= 0 || V <= 0 || d <= 0) return 0;
     const CePlan pl = ce_plan(R, V, d);
-    return round256((size_t)R * pl.ldp * 2) + (size_t)pl.slabs * R * d * 4;
+    return (R <= FEW ? 2 : 1) * round256((size_t)R * pl.ldp * 2) + round256((size_t)R * 4) + (size_t)pl.slabs * R * d * 4;
 }
 
 extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ldw, const long long* labels, const float* lse, const float* gloss,
@@ -260,7 +340,8 @@ extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ld
     PACED_CHECK_ARG(!dw || (lddw >= d && lddw % 8 == 0 && ((uintptr_t)dw & 15) == 0), "paced_linear_ce_bwd: dw needs 16-byte aligned rows, a stride of at least d and a multiple of 8 (lddw=%d)", lddw);
     if (R == 0) {                                     // no row: dw's sum is empty
         if (!dw || dw_f32) return PACED_OK;
-        hipLaunchKernelGGL(ce_dh_kernel, dim3(blocks_for((long long)V * (d >> 3))), dim3(256), 0, s, nullptr, 0, 0LL, (bf16*)dw, lddw, V, d);
+        hipLaunchKernelGGL(ce_dh_kernel, dim3(blocks_for((long long)V * (d >> 3))), dim3(256), 0, s, nullptr, 0, 0LL, (bf16*)dw, lddw, V, d,
+                           nullptr, 0LL, 0, nullptr, nullptr, 0, 0.f);
         PACED_CHECK_LAUNCH();
         return PACED_OK;
     }
@@ -274,13 +355,18 @@ extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ld
     PACED_CHECK_ARG((unsigned long long)R * (ldh > pl.ldp ? ldh : pl.ldp) < (1ull << 31), "paced_linear_ce_bwd: %d rows of h with a stride of %d span 4 GiB or more; pass fewer at a time", R, ldh);
     PACED_CHECK_ARG((unsigned long long)pl.piece * ldw < (1ull << 31), "paced_linear_ce_bwd: %d rows of w with a stride of %d span 4 GiB or more; pass w with a smaller stride", pl.piece, ldw);
     bf16* P = (bf16*)workspace;
-    float* slabs = (float*)((char*)workspace + round256((size_t)R * pl.ldp * 2));
+    const size_t part = round256((size_t)R * pl.ldp * 2);
+    const int forced = paced_gemm_forced_tile();                  // (the low part is written by the 64x64 tiles' epilogue)
+    bf16* low = dw && R <= FEW && (forced == 0 || forced == 64) ? (bf16*)((char*)workspace + part) : nullptr;
+    float* err = (float*)((char*)workspace + (R <= FEW ? 2 : 1) * part);
+    float* slabs = (float*)((char*)err + round256((size_t)R * 4));
     for (int v0 = 0; v0 < V; v0 += pl.piece) {
         const int n = V - v0 < pl.piece ? V - v0 : pl.piece;
         const bf16* wp = (const bf16*)w + (size_t)v0 * ldw;
         GemmParams p = product(h, ldh, wp, ldw, P, pl.ldp, R, n, d, scale);
         p.ce_labels = labels; p.ce_lse = lse; p.ce_g = gloss;
         p.ce_ignore = ignore_index; p.ce_vocab = V; p.ce_first = v0;
+        p.ce_err = err; p.ce_lo = low;
         int r = ce_logits(p, EPI_CE_GRAD, s);
         if (r != PACED_OK) return r;
         if (dh) {
@@ -290,7 +376,12 @@ extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ld
             p.tile = pl.dh_tile;
             if ((r = paced_gemm_launch(p, false, true, EPI_SLAB_F32, pl.slabs, s)) != PACED_OK) return r;
         }
-        if (dw) {
+        if (dw && low) {
+            const dim3 grid((n + 63) / 64, (d + 255) / 256);
+            if (dw_f32) hipLaunchKernelGGL(ce_dw_few_kernel<true>, grid, dim3(256), 0, s, P, low, pl.ldp, (const bf16*)h, ldh, (void*)((float*)dw + (size_t)v0 * lddw), lddw, R, n, d, scale);
+            else hipLaunchKernelGGL(ce_dw_few_kernel<false>, grid, dim3(256), 0, s, P, low, pl.ldp, (const bf16*)h, ldh, (void*)((bf16*)dw + (size_t)v0 * lddw), lddw, R, n, d, scale);
+            PACED_CHECK_LAUNCH();
+        } else if (dw) {
             p = product(P, pl.ldp, h, ldh, dw_f32 ? (void*)((float*)dw + (size_t)v0 * lddw) : (void*)((bf16*)dw + (size_t)v0 * lddw), lddw, n, d, R, scale);
             p.accumulate = 1;
             p.tile = best_tile(n, d, (R + 63) / 64);
@@ -298,7 +389,8 @@ extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ld
         }
     }
     if (dh) {
-        hipLaunchKernelGGL(ce_dh_kernel, dim3(blocks_for((long long)R * (d >> 3))), dim3(256), 0, s, slabs, pl.slabs, (long long)R * d, (bf16*)dh, lddh, R, d);
+        hipLaunchKernelGGL(ce_dh_kernel, dim3(blocks_for((long long)R * (d >> 3))), dim3(256), 0, s, slabs, pl.slabs, (long long)R * d, (bf16*)dh, lddh, R, d,
+                           labels, ignore_index, V, err, (const bf16*)w, ldw, scale);
         PACED_CHECK_LAUNCH();
     }
     return PACED_OK;

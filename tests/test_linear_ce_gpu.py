@@ -252,3 +252,22 @@ def test_refusals():
     buf = torch.zeros(8, 70, device="cuda", dtype=BF16)
     with pytest.raises(PacedHipError, match="multiples of 8"):
         K.linear_ce_fwd(buf[:, :64], w, labels, loss)
+
+
+@pytest.mark.parametrize("R,V,d", [(1, 8000, 448), (9, 433, 384), (64, 5000, 256), (65, 5000, 256)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_few_rows_lose_nothing_to_the_rounding_between_the_products(R, V, d, f32):
+    """dh gets back what the label's entry lost; up to 64 rows dw is made of both parts of P.  What is left is the result's own
+    rounding, half a step 2^-8 at most and uniform: 2^-8 / sqrt(3) of the norm; with fp32 sums dw has P's low part's, 2^-16.
+    (dh's other entries, each off by 2^-8 / sqrt(3) of itself, weigh sqrt(sum p^2) against 1 - p: under a third here.)"""
+    h, w, labels, gl = make(R, V, d, 77 + R, ignored=0.0, size=1.0)
+    o = oracle(h, w, labels, gl, 1.0)
+    _, _, dh, dw = run(h, w, labels, gl, f32=f32)
+    rel = lambda got, want: ((got.double() - want).norm() / want.norm()).item()  # noqa: E731
+    assert rel(dh, o["P"] @ o["w"]) < 1.1 * HALF / 3 ** 0.5
+    want = o["P"].t() @ o["h"]
+    if R <= 64:
+        if f32:       # the sum with 1/4 rounds to 2^-24 of it
+            assert (dw.double() - 0.25 - want).norm() <= 2.0 ** -15 * want.norm() + 2.0 ** -25 * dw.numel() ** 0.5
+        else:
+            assert rel(dw, want) < HALF / 3 ** 0.5
