@@ -89,28 +89,30 @@ __device__ __forceinline__ void ce_rows(const GemmParams& p, int m0, int wm, int
     }
 }
 
-// gradient of four consecutive columns n .. n + 3 of a row: g (2^(z - lse2) - [label]).  SPECIAL: the label may be among the
-// wave's columns, the row ignored (its logits may be anything) or the columns past the vocabulary's end; without it a value
-// takes three instructions instead of eight (the caller asks once for a wave's 16 x 64 block).
-// The label's entry, nearly -g for most rows, dominates dh: what its rounding to bf16 loses is kept for the kernel that finishes dh.
-template <bool SPECIAL>
-__device__ __forceinline__ f32x4 ce_grad4(const GemmParams& p, const f32x4& a, float c, float lse2, float g, int col, bool dead, int m, int n) {
+// gradient of four consecutive columns of a row whose label is none of them: g 2^(z - lse2)
+__device__ __forceinline__ f32x4 ce_grad4(const f32x4& a, float c, float lse2, float g) {
     f32x4 o;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        float v = __builtin_amdgcn_exp2f(__builtin_fmaf(a[r], c, -lse2)) * g;
-        if (SPECIAL) {
-            if (n + r == col) {
-                v -= g;
-                if (m < p.M && col < p.N) p.ce_err[m] = v - bf2f(f2bf(v));
-            }
-            v = dead || n + r >= p.N ? 0.f : v;
-        }
-        o[r] = v;
-    }
+    for (int r = 0; r < 4; ++r) o[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(a[r], c, -lse2)) * g;
     return o;
 }
-// whether a wave's block of columns nw .. nw + width - 1 needs SPECIAL
+// ... and what a block of 16 rows x 64 columns needs where a label is among its columns, a row is ignored (its logits may be
+// anything) or the vocabulary ends in it.  The label's entry, nearly -g for most rows, dominates dh: what its rounding to bf16
+// loses is kept for the kernel that finishes dh.
+__device__ __forceinline__ void ce_mend4(const GemmParams& p, f32x4& v, float g, int col, bool dead, int m, int n) {
+    const int at = col - n;
+    if (at >= 0 && at < 4) {
+        const float x = (at == 0 ? v[0] : at == 1 ? v[1] : at == 2 ? v[2] : v[3]) - g;
+        if (at == 0) v[0] = x;
+        if (at == 1) v[1] = x;
+        if (at == 2) v[2] = x;
+        if (at == 3) v[3] = x;
+        if (m < p.M && col < p.N) p.ce_err[m] = x - bf2f(f2bf(x));
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = dead || n + r >= p.N ? 0.f : v[r];
+}
+// whether a wave's block of columns nw .. nw + width - 1 needs that (asked once for all of it)
 __device__ __forceinline__ bool ce_special(const GemmParams& p, int col, bool dead, int nw, int width) {
     return nw + width > p.N || __ballot(dead || (col >= nw && col < nw + width)) != 0;
 }
@@ -367,14 +369,15 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, void* Cb, int m0, 
                     for (int r = 0; r < 4; ++r) if (nw + j * 16 + nl + r >= p.N) z[j * 4 + r] = -INFINITY;
             }
             if (__ballot(rel >= 0 && rel < NJ * 16)) {
+                const int mine = rel - nl;                     // j * 16 + r where the label is this lane's
+                float t = 0.f;
+                bool hit = false;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        if (rel == j * 16 + nl + r) {
-                            if (m < p.M) p.ce_target[m] = acc[i][j][r] * p.alpha;
-                            z[j * 4 + r] = -INFINITY;
-                        }
+                        if (mine == j * 16 + r) { t = acc[i][j][r]; hit = true; z[j * 4 + r] = -INFINITY; }
+                if (hit && m < p.M) p.ce_target[m] = t * p.alpha;
             }
             float mx = z[0];
 #pragma unroll
@@ -406,8 +409,8 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, void* Cb, int m0, 
             for (int j = 0; j < NJ; ++j) {
                 const int n = n0 + Cfg::noff(wn, j) + (lane >> 4) * 4;
                 if (n >= ((p.N + 63) & ~63)) continue;
-                const f32x4 o = special ? ce_grad4<true>(p, acc[i][j], c, lse2[i], g[i], col[i], dead[i], m, n)
-                                        : ce_grad4<false>(p, acc[i][j], c, lse2[i], g[i], col[i], dead[i], m, n);
+                f32x4 o = ce_grad4(acc[i][j], c, lse2[i], g[i]);
+                if (special) ce_mend4(p, o, g[i], col[i], dead[i], m, n);
                 const bf16x4 hi = __builtin_convertvector(o, bf16x4);
                 *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16*>(Cb) + (size_t)m * p.ldc + n) = hi;
                 if (p.ce_lo) *reinterpret_cast<bf16x4*>(p.ce_lo + (size_t)m * p.ldc + n) = __builtin_convertvector(o - __builtin_convertvector(hi, f32x4), bf16x4);
@@ -734,8 +737,8 @@ __device__ __forceinline__ void epilogue_rows_impl(const GemmParams& p, void* Cb
         for (int j = 0; j < 4; ++j) {
             if (EPI == EPI_CE_GRAD) {
                 const int m = m0 + CfgPhased::moff(wr, i) + mw, n = n0 + wc * 64 + j * 16 + g * 4;
-                const f32x4 v = special ? ce_grad4<true>(p, acc[i][j], p.alpha * CE_LOG2E, clse[i], cg[i], ccol[i], cdead[i], m, n)
-                                        : ce_grad4<false>(p, acc[i][j], p.alpha * CE_LOG2E, clse[i], cg[i], ccol[i], cdead[i], m, n);
+                f32x4 v = ce_grad4(acc[i][j], p.alpha * CE_LOG2E, clse[i], cg[i]);
+                if (special) ce_mend4(p, v, cg[i], ccol[i], cdead[i], m, n);
                 o[j] = __builtin_convertvector(v, bf16x4);
                 continue;
             }

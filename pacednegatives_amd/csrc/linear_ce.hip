@@ -84,19 +84,23 @@ __global__ void __launch_bounds__(256) ce_dh_kernel(const float* __restrict__ sl
     for (long long id = (long long)blockIdx.x * 256 + threadIdx.x; id < total; id += (long long)gridDim.x * 256) {
         const int r = (int)(id / d8), c = (int)(id - (long long)r * d8);
         f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+        bf16x8 x = {};
+        float e = 0.f;
+        if (labels) {                                        // requested ahead of the slabs, added after them
+            const long long label = labels[r];
+            if (label != ignore && label >= 0 && label < V) {
+                x = *reinterpret_cast<const bf16x8*>(w + (size_t)label * ldw + c * 8);
+                e = scale * err[r];
+            }
+        }
         for (int k = 0; k < count; ++k) {
             const float* src = slabs + (size_t)k * slab + (size_t)r * d + c * 8;
             a += *reinterpret_cast<const f32x4*>(src);
             b += *reinterpret_cast<const f32x4*>(src + 4);
         }
-        if (labels) {
-            const long long label = labels[r];
-            if (label != ignore && label >= 0 && label < V) {
-                const bf16x8 x = *reinterpret_cast<const bf16x8*>(w + (size_t)label * ldw + c * 8);
-                const float e = scale * err[r];
+        if (e != 0.f) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) { a[j] += e * bf2f(x[j]); b[j] += e * bf2f(x[4 + j]); }
-            }
+            for (int j = 0; j < 4; ++j) { a[j] += e * bf2f(x[j]); b[j] += e * bf2f(x[4 + j]); }
         }
         bf16x8 o;
 #pragma unroll
