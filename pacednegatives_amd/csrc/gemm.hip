@@ -28,64 +28,81 @@ __device__ __forceinline__ void* batch_c(const GemmParams& p, int b) {
 }
 
 // ---- linear-head cross entropy -----------------------------------------------------------------------------------
-// Rows of a wave's 16-row block i are on its lanes' low four bits.  What a row needs (label, log-sum-exp, weight) is loaded
-// by inline assembly that waits for itself: a load the compiler can see would drain the K loop's LDS-DMA (epilogue_rows_impl).
+// Rows of a wave's 16-row block i are on its lanes' low four bits.  What the rows need (labels, log-sum-exps, weights) is loaded
+// by one block of inline assembly that waits for itself: a load the compiler can see would drain the K loop's LDS-DMA
+// (epilogue_rows_impl).  Descriptors begin at the tile's first row and end with the last one: rows past M read as zeros, and one
+// address register serves all blocks.
 constexpr float CE_LOG2E = 1.4426950408889634f;
 
-// A row's label goes through ce_columns; its log-sum-exp and weight, where wanted, are requested ahead of the labels' own block
-// and have arrived when that block's wait is over.
-__device__ __forceinline__ void ce_request(float& v, const float* src) { asm volatile("global_load_dword %0, %1, off" : "=v"(v) : "v"(src) : "memory"); }
-
-template <int MI>
-__device__ __forceinline__ void ce_load_labels(const u32x2* const (&src)[MI], u32x2 (&v)[MI]) {
-    static_assert(MI == 2 || MI == 4 || MI == 8, "row blocks of a wave");
-    if constexpr (MI == 8)
-        asm volatile("global_load_dwordx2 %0, %8, off\n\tglobal_load_dwordx2 %1, %9, off\n\tglobal_load_dwordx2 %2, %10, off\n\tglobal_load_dwordx2 %3, %11, off\n\t"
-                     "global_load_dwordx2 %4, %12, off\n\tglobal_load_dwordx2 %5, %13, off\n\tglobal_load_dwordx2 %6, %14, off\n\tglobal_load_dwordx2 %7, %15, off\n\t"
-                     "s_waitcnt vmcnt(0) ; hidden-load wait"
-                     : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
-                     : "v"(src[0]), "v"(src[1]), "v"(src[2]), "v"(src[3]), "v"(src[4]), "v"(src[5]), "v"(src[6]), "v"(src[7]) : "memory");
-    else if constexpr (MI == 4)
-        asm volatile("global_load_dwordx2 %0, %4, off\n\tglobal_load_dwordx2 %1, %5, off\n\tglobal_load_dwordx2 %2, %6, off\n\tglobal_load_dwordx2 %3, %7, off\n\t"
-                     "s_waitcnt vmcnt(0) ; hidden-load wait"
-                     : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]) : "v"(src[0]), "v"(src[1]), "v"(src[2]), "v"(src[3]) : "memory");
-    else
-        asm volatile("global_load_dwordx2 %0, %2, off\n\tglobal_load_dwordx2 %1, %3, off\n\ts_waitcnt vmcnt(0) ; hidden-load wait"
-                     : "=&v"(v[0]), "=&v"(v[1]) : "v"(src[0]), "v"(src[1]) : "memory");
+template <class T>
+__device__ __forceinline__ u32x4 ce_descriptor(const T* rows, int count) {
+    const uint64_t a = (uint64_t)rows;
+    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)) & 0xffffu,
+                 (uint32_t)__builtin_amdgcn_readfirstlane((int)(count * sizeof(T))), 0x00020000u};
 }
+#define CE_SETTLE "s_nop 4\n\t"        // a descriptor word that a vector instruction wrote may be read five states later
+#define CE_LABEL(i, row) "buffer_load_dwordx2 %[l" #i "], %[vl], %[rl], 0 offen offset:8*" #row "\n\t"
+#define CE_ROW(i, row)                                                               \
+    "buffer_load_dword %[s" #i "], %[vs], %[rs], 0 offen offset:4*" #row "\n\t"      \
+    "buffer_load_dword %[g" #i "], %[vs], %[rg], 0 offen offset:4*" #row "\n\t"
+#define CE_WAIT "s_waitcnt vmcnt(0) ; hidden-load wait"
+#define CE_L(i) [l##i] "=&v"(v[i])
+#define CE_S(i) [s##i] "=&v"(lse[i]), [g##i] "=&v"(w[i])
 
-// labels of this lane's rows, as columns of the launch (ignored, or of another piece: outside [0, N))
-template <class Cfg>
-__device__ __forceinline__ void ce_columns(const GemmParams& p, int m0, int wm, int lane, int (&col)[Cfg::MI], bool (&dead)[Cfg::MI]) {
-    const u32x2* src[Cfg::MI];
+// labels of a lane's rows, and with ROWS their log-sum-exps and weights
+template <class Cfg, bool ROWS>
+__device__ __forceinline__ void ce_load(const GemmParams& p, int m0, int wm, int lane, u32x2 (&v)[Cfg::MI], float (&lse)[Cfg::MI], float (&w)[Cfg::MI]) {
+    constexpr int MI = Cfg::MI;
+    static_assert(MI == 2 || MI == 4 || MI == 8, "row blocks of a wave");
+    static_assert(MI == 8 ? Cfg::moff(0, 3) == 48 && Cfg::moff(0, 4) == 128 && Cfg::moff(0, 7) == 176 : Cfg::moff(0, MI - 1) == 16 * (MI - 1), "the rows in the text below");
+    const int count = min(Cfg::BM, p.M - m0), row = Cfg::moff(wm, 0) + (lane & 15);
+    const uint32_t vl = row * 8, vs = row * 4;
+    const u32x4 rl = ce_descriptor(p.ce_labels + m0, count);
+    if constexpr (!ROWS) {
+        if constexpr (MI == 8)
+            asm volatile(CE_SETTLE CE_LABEL(0, 0) CE_LABEL(1, 16) CE_LABEL(2, 32) CE_LABEL(3, 48) CE_LABEL(4, 128) CE_LABEL(5, 144) CE_LABEL(6, 160) CE_LABEL(7, 176) CE_WAIT
+                         : CE_L(0), CE_L(1), CE_L(2), CE_L(3), CE_L(4), CE_L(5), CE_L(6), CE_L(7) : [vl] "v"(vl), [rl] "s"(rl) : "memory");
+        else if constexpr (MI == 4)
+            asm volatile(CE_SETTLE CE_LABEL(0, 0) CE_LABEL(1, 16) CE_LABEL(2, 32) CE_LABEL(3, 48) CE_WAIT
+                         : CE_L(0), CE_L(1), CE_L(2), CE_L(3) : [vl] "v"(vl), [rl] "s"(rl) : "memory");
+        else
+            asm volatile(CE_SETTLE CE_LABEL(0, 0) CE_LABEL(1, 16) CE_WAIT : CE_L(0), CE_L(1) : [vl] "v"(vl), [rl] "s"(rl) : "memory");
+    } else {
+        const u32x4 rs = ce_descriptor(p.ce_lse + m0, count), rg = ce_descriptor(p.ce_g + m0, count);
+        if constexpr (MI == 8)
+            asm volatile(CE_SETTLE CE_LABEL(0, 0) CE_LABEL(1, 16) CE_LABEL(2, 32) CE_LABEL(3, 48) CE_LABEL(4, 128) CE_LABEL(5, 144) CE_LABEL(6, 160) CE_LABEL(7, 176)
+                         CE_ROW(0, 0) CE_ROW(1, 16) CE_ROW(2, 32) CE_ROW(3, 48) CE_ROW(4, 128) CE_ROW(5, 144) CE_ROW(6, 160) CE_ROW(7, 176) CE_WAIT
+                         : CE_L(0), CE_L(1), CE_L(2), CE_L(3), CE_L(4), CE_L(5), CE_L(6), CE_L(7), CE_S(0), CE_S(1), CE_S(2), CE_S(3), CE_S(4), CE_S(5), CE_S(6), CE_S(7)
+                         : [vl] "v"(vl), [vs] "v"(vs), [rl] "s"(rl), [rs] "s"(rs), [rg] "s"(rg) : "memory");
+        else if constexpr (MI == 4)
+            asm volatile(CE_SETTLE CE_LABEL(0, 0) CE_LABEL(1, 16) CE_LABEL(2, 32) CE_LABEL(3, 48) CE_ROW(0, 0) CE_ROW(1, 16) CE_ROW(2, 32) CE_ROW(3, 48) CE_WAIT
+                         : CE_L(0), CE_L(1), CE_L(2), CE_L(3), CE_S(0), CE_S(1), CE_S(2), CE_S(3)
+                         : [vl] "v"(vl), [vs] "v"(vs), [rl] "s"(rl), [rs] "s"(rs), [rg] "s"(rg) : "memory");
+        else
+            asm volatile(CE_SETTLE CE_LABEL(0, 0) CE_LABEL(1, 16) CE_ROW(0, 0) CE_ROW(1, 16) CE_WAIT
+                         : CE_L(0), CE_L(1), CE_S(0), CE_S(1) : [vl] "v"(vl), [vs] "v"(vs), [rl] "s"(rl), [rs] "s"(rs), [rg] "s"(rg) : "memory");
+    }
+}
+#undef CE_SETTLE
+#undef CE_LABEL
+#undef CE_ROW
+#undef CE_WAIT
+#undef CE_L
+#undef CE_S
+
+// labels of this lane's rows, as columns of the launch (ignored, or of another piece: outside [0, N)), and with ROWS their
+// log-sum-exps (base 2) and weights
+template <class Cfg, bool ROWS>
+__device__ __forceinline__ void ce_rows(const GemmParams& p, int m0, int wm, int lane, int (&col)[Cfg::MI], bool (&dead)[Cfg::MI],
+                                        float (&lse2)[Cfg::MI], float (&g)[Cfg::MI]) {
     u32x2 v[Cfg::MI];
-#pragma unroll
-    for (int i = 0; i < Cfg::MI; ++i)
-        src[i] = reinterpret_cast<const u32x2*>(p.ce_labels + min(m0 + Cfg::moff(wm, i) + (lane & 15), p.M - 1));
-    ce_load_labels<Cfg::MI>(src, v);
+    ce_load<Cfg, ROWS>(p, m0, wm, lane, v, lse2, g);
 #pragma unroll
     for (int i = 0; i < Cfg::MI; ++i) {
         const long long label = (long long)(((unsigned long long)v[i][1] << 32) | v[i][0]);
         dead[i] = label == p.ce_ignore || label < 0 || label >= p.ce_vocab;
         col[i] = dead[i] ? -1 : (int)label - p.ce_first;
-    }
-}
-
-// ... and their log-sum-exps (base 2) and weights
-template <class Cfg>
-__device__ __forceinline__ void ce_rows(const GemmParams& p, int m0, int wm, int lane, int (&col)[Cfg::MI], bool (&dead)[Cfg::MI],
-                                        float (&lse2)[Cfg::MI], float (&g)[Cfg::MI]) {
-#pragma unroll
-    for (int i = 0; i < Cfg::MI; ++i) {
-        const int mc = min(m0 + Cfg::moff(wm, i) + (lane & 15), p.M - 1);
-        ce_request(lse2[i], p.ce_lse + mc);
-        ce_request(g[i], p.ce_g + mc);
-    }
-    ce_columns<Cfg>(p, m0, wm, lane, col, dead);
-#pragma unroll
-    for (int i = 0; i < Cfg::MI; ++i) {
-        asm volatile("" : "+v"(lse2[i]), "+v"(g[i]) :: "memory");          // arrived: not read before this point
-        lse2[i] *= CE_LOG2E;
+        if (ROWS) lse2[i] *= CE_LOG2E;
     }
 }
 
@@ -347,7 +364,8 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, void* Cb, int m0, 
     if (EPI == EPI_CE_STATS) {
         int col[MI];
         bool dead[MI];
-        ce_columns<Cfg>(p, m0, wm, lane, col, dead);
+        float unused[MI];
+        ce_rows<Cfg, false>(p, m0, wm, lane, col, dead, unused, unused);
         const float c = p.alpha * CE_LOG2E;
         const int nw = n0 + Cfg::noff(wn, 0), nl = (lane >> 4) * 4;        // the wave's first column; this lane's within 16
         if (nw >= p.N) return;
@@ -398,7 +416,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, void* Cb, int m0, 
         int col[MI];
         bool dead[MI];
         float lse2[MI], g[MI];
-        ce_rows<Cfg>(p, m0, wm, lane, col, dead, lse2, g);
+        ce_rows<Cfg, true>(p, m0, wm, lane, col, dead, lse2, g);
         const float c = p.alpha * CE_LOG2E;
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
@@ -724,7 +742,7 @@ __device__ __forceinline__ void epilogue_rows_impl(const GemmParams& p, void* Cb
     int ccol[8];
     bool cdead[8];
     float clse[8], cg[8];
-    if (EPI == EPI_CE_GRAD) ce_rows<CfgPhased>(p, m0, wr, lane, ccol, cdead, clse, cg);
+    if (EPI == EPI_CE_GRAD) ce_rows<CfgPhased, true>(p, m0, wr, lane, ccol, cdead, clse, cg);
     const bool has_drop = (EPI == EPI_RES_DROP || EPI == EPI_RELU_DROP) && p.drop.thresh != 0;
     const float scale = (EPI == EPI_MASK || EPI == EPI_MASK_BITS) ? p.alpha * p.mask_scale : p.alpha;
 

@@ -18,25 +18,25 @@ constexpr int BK = 64;
 }  // namespace
 struct CfgSmall {
     static constexpr int BM = 128, BN = 128, WGM = 2, WGN = 2, MI = 4, NJ = 4;
-    static __device__ __forceinline__ int moff(int wm, int i) { return wm * 64 + i * 16; }
-    static __device__ __forceinline__ int noff(int wn, int j) { return wn * 64 + j * 16; }
+    static constexpr __device__ __forceinline__ int moff(int wm, int i) { return wm * 64 + i * 16; }
+    static constexpr __device__ __forceinline__ int noff(int wn, int j) { return wn * 64 + j * 16; }
 };
 // small8: the 128x128 tile with eight waves of 32x64: two waves to a SIMD, so that one's fragment reads run under the other's
 //           MFMAs where a CU has a single tile (linear_ce.hip's mid-sized products).  64 columns a wave, as in the small tile.
 struct CfgSmall8 {
     static constexpr int BM = 128, BN = 128, WGM = 4, WGN = 2, MI = 2, NJ = 4;
-    static __device__ __forceinline__ int moff(int wm, int i) { return wm * 32 + i * 16; }
-    static __device__ __forceinline__ int noff(int wn, int j) { return wn * 64 + j * 16; }
+    static constexpr __device__ __forceinline__ int moff(int wm, int i) { return wm * 32 + i * 16; }
+    static constexpr __device__ __forceinline__ int noff(int wn, int j) { return wn * 64 + j * 16; }
 };
 struct CfgTiny {
     static constexpr int BM = 64, BN = 64, WGM = 2, WGN = 2, MI = 2, NJ = 2;
-    static __device__ __forceinline__ int moff(int wm, int i) { return wm * 32 + i * 16; }
-    static __device__ __forceinline__ int noff(int wn, int j) { return wn * 32 + j * 16; }
+    static constexpr __device__ __forceinline__ int moff(int wm, int i) { return wm * 32 + i * 16; }
+    static constexpr __device__ __forceinline__ int noff(int wn, int j) { return wn * 32 + j * 16; }
 };
 struct CfgPhased {
     static constexpr int BM = 256, BN = 256, WGM = 2, WGN = 4, MI = 8, NJ = 4;
-    static __device__ __forceinline__ int moff(int wm, int i) { return (i >> 2) * 128 + wm * 64 + (i & 3) * 16; }
-    static __device__ __forceinline__ int noff(int wn, int j) { return wn * 64 + j * 16; }   // B halves interleave 32-column blocks
+    static constexpr __device__ __forceinline__ int moff(int wm, int i) { return (i >> 2) * 128 + wm * 64 + (i & 3) * 16; }
+    static constexpr __device__ __forceinline__ int noff(int wn, int j) { return wn * 64 + j * 16; }   // B halves interleave 32-column blocks
 };
 namespace {
 
