@@ -163,7 +163,8 @@ int paced_rmsnorm_bwd(const void* dy, const void* x, const void* w, const float*
  * bwd: x is what was normalised (xsum where there was a residual);  g = dy w,  xh = (x - mean) rstd,
  *      dx = rstd (g - sum(g)/d - xh sum(g xh)/d) + dres (dres may be NULL);
  *      dw[d] += sum dy xh and db[d] += sum dy (fp32, each may be NULL; added in a fixed order, no atomics), through a
- *      workspace of paced_layernorm_workspace_bytes(M, d) bytes (not read or written when dw and db are both NULL).
+ *      workspace of paced_layernorm_workspace_bytes(M, d) bytes (not needed when dw and db are both NULL; not kept between
+ *      calls, for one stream at a time).
  * An output may be the very tensor of an input of its shape (y = x, xsum = res, dx = dy or dres); partial overlaps may not. */
 int paced_layernorm_max_width(void);
 int paced_layernorm_fwd(const void* x, int ldx, const void* res, int ldr, void* xsum, int lds, const void* w, const void* b,
@@ -184,7 +185,8 @@ int paced_layernorm_bwd(const void* dy, int lddy, const void* x, int ldx, const 
  * dweight: dw [M, N] fp32 (+)= dy^T x for the checkpoint's values x [T, N] and dy [T, M] bf16 (rows of lddy elements, or
  * head-major as in paced_gemm_bf16_heads: lddy = 64 and dy_heads > 0; the rows up to the next multiple of 64 must then be
  * finite); M % 8 == 0, N % 16 == 0, lddw % 4 == 0.  Products are exact, sums fp32 in a fixed order (no atomics).
- * accumulate = 0: dw is written, 1: added to.  workspace: paced_act8_dweight_workspace_bytes(T, M, N, accumulate) bytes. */
+ * accumulate = 0: dw is written, 1: added to.  workspace, 16-byte aligned, not kept between calls, for one stream at a time:
+ * paced_act8_dweight_workspace_bytes(T, M, N, accumulate) bytes (0: none needed). */
 int paced_act8_quantize(const void* x, int ldx, void* q, void* scale, int T, int n, void* stream);
 int paced_act8_dequantize(const void* q, const void* scale, void* y, int ldy, int T, int n, void* stream);
 size_t paced_act8_dweight_workspace_bytes(int T, int M, int N, int accumulate);
@@ -271,9 +273,13 @@ int paced_cross_entropy(const float* logits, const long long* labels, float* los
  *      losses keep their relative precision.
  * bwd: gloss[r] = d objective / d loss[r] (fp32); dh [R, d] bf16 is written, dw [V, d] is written in bf16 (dw_f32 = 0) or added
  *      to in fp32 (dw_f32 = 1); each may be NULL.  The logits' gradient gloss (softmax - onehot) scale is rounded to bf16
- *      between the products, as paced_cross_entropy's dlogits are; sums are fp32 in a fixed order, without atomics.  An
- *      ignored row's h must be finite where dw is wanted (0 times it is added).
- * workspace: ..._workspace_bytes() bytes (256 MiB + about 64 MiB at most, whatever V is, up to R of half a million). */
+ *      between the products, as paced_cross_entropy's dlogits are; what the label's entry loses in it is added to dh again,
+ *      and up to 64 rows dw takes every entry's low part as well.  Sums are fp32 in a fixed order, without atomics.  An
+ *      ignored row's h must be finite where dw is wanted (0 times it is added), w where dh is.
+ * Row strides are at most 2^22 elements; bwd refuses an h whose R rows span 4 GiB or more.
+ * workspace, 16-byte aligned, not kept between calls, for one stream at a time: ..._workspace_bytes() bytes; fwd V R / 4 +
+ * 4 R, bwd the bf16 gradient of a piece of the vocabulary (256 MiB at most up to half a million rows; twice that up to 64 rows)
+ * and fp32 partial sums of dh (4 R d bytes each, 64 at most, the fewer the more rows). */
 size_t paced_linear_ce_fwd_workspace_bytes(int R, int V);
 int paced_linear_ce_fwd(const void* h, int ldh, const void* w, int ldw, const long long* labels, float* loss, float* lse,
                         int R, int V, int d, long long ignore_index, float scale, void* workspace, size_t workspace_bytes, void* stream);

@@ -10,7 +10,7 @@
 // (eight tokens of one feature) share one scale, and v_cvt_scalef32_pk_bf16_fp8 applies it while it converts.
 // Writing and reading are bound by memory: 139264 x 768 in 51.5 us (6.3 TB/s) and 55 us (5.9 TB/s).  The gradient is bound by the
 // matrix cores where tokens are many: 2304 x 768 from 139264 tokens in 411 us with the slabs' sum, 1.20 PFLOP/s (the bf16
-// products of gemm.hip reach 1.25 to 1.35 on large squares, the vendor's 1.39); 512 x 2048 from 1001 tokens in 10.4 us, by latency.
+// products of gemm.hip reach 1.25 to 1.35 on large squares, the vendor's 1.39); 512 x 2048 from 1001 tokens in 9.7 us, by latency.
 #include "gemm_tiles.h"
 
 namespace {
@@ -245,7 +245,8 @@ __global__ void __launch_bounds__(256) act8_dw_kernel(DwParams p, int ntm, int n
 // 256x256 tiles: the phased kernel of gemm.hip (same ring order, phases, barriers and A halves) with B halves of codes: 8 KiB
 // instead of 16, one LDS-DMA instruction per wave instead of two, half the fragment reads; a fragment is converted behind its
 // phase's barrier.  Codes of a half: [64 tokens][128] bytes, 16-byte unit u of token k at u ^ (k & 7) ^ ((k >> 3) & 1) (the
-// sixteen tokens that two lane groups gather lie on different banks); half h holds the h-th 32 features of every 64.  With each step's first B half every wave fetches the scales of its own 64 features.
+// sixteen tokens that two lane groups gather lie on different banks); half h holds the h-th 32 features of every 64.  With each
+// step's first B half every wave fetches the scales of its own 64 features.
 // Instructions in flight behind a phase's wait (the six youngest half-tiles; B half 0 and its scales 2, A halves 2, B half 1 1):
 // 11 after B half 0 and A half 0 were issued, 10 after B half 1 and A half 1.
 // LDS: ring slots 0, 2, .. 8 are B halves (5 x 8 KiB), 1, 3, .. 9 A halves (5 x 16 KiB), three sets of scales (a set is read in
