@@ -11,7 +11,7 @@
 // dh is summed over pieces and slices of a piece in fp32 slabs with one owner per element, dw is complete with its piece:
 // nothing is added atomically, equal inputs give equal bits.
 // Matrix-core bound: 2 R V d operations forward, three times that backward.  Measured, loss and both gradients: 8192 rows x
-// 50001 entries x 1024 in 3.0 ms (1.12 PFLOP/s over the four products, the statistics alone 1.1), 1088 x 32128 x 768 in 254
+// 50001 entries x 1024 in 2.9 to 3.0 ms (1.14 PFLOP/s over the four products), 1088 x 32128 x 768 in 254
 // to 280 us on different cards (0.77 to 0.85 PFLOP/s: 4.25 x 125.5 tiles of 256 do not fill whole rounds of 256 compute units);
 // the loss of 16 rows 15 us, of which the weights' 49 MB take 11.
 #include "gemm.h"
