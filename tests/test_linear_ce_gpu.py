@@ -103,6 +103,20 @@ def test_sizes_that_choose_their_own_tiles(R, V, d):
     assert all(torch.equal(a, b) for a, b in zip((loss, lse, dh, dw), again))
 
 
+@pytest.mark.parametrize("R,V", [(2816, 2900), (4300, 2561), (2561, 5000)])
+def test_more_than_eight_tiles_each_way(R, V):
+    """(11 x 12, 17 x 11 and 11 x 20 tiles of 256: bands of unequal width, the last one of a tile's single row or column)"""
+    K.gemm_set_tile(256)
+    try:
+        h, w, labels, gl = make(R, V, 64, 11)
+        o = oracle(h, w, labels, gl, 1.0)
+        loss, lse, dh, dw = run(h, w, labels, gl)
+    finally:
+        K.gemm_set_tile(0)
+    check_loss(o, loss, lse)
+    check_grads(o, dh, dw)
+
+
 @pytest.mark.parametrize("R,V,d,f32", [(20000, 7001, 64, False), (9000, 20001, 256, True)])
 def test_vocabulary_in_several_pieces(R, V, d, f32):
     h, w, labels, gl = make(R, V, d, 5)
