@@ -9,7 +9,8 @@
 // over all rows that a team works on, are added over a workgroup's teams in LDS, and leave as one partial row per workgroup;
 // a second kernel adds those in a fixed order (no atomics: equal inputs give equal bits).
 // Measured, 139264 x 768 bf16 with the residual sum: forward 150 us for its four streams (5.7 TB/s; a copy of 256 MB reaches
-// 5.4), backward 168 us for its four (5.1 TB/s), column sums 4.5 us.  5001 x 1023 fp32: 10, 19 and 4 us.
+// 5.4), backward 168 us for its four (5.1 TB/s), column sums 4.5 us.  139264 x 767 (fp32, no residual): 166 and
+// 258 us against 147 and 226 for 768.  5001 x 1023 fp32: 10, 14 and 4 us.
 #include "common.h"
 
 namespace {
@@ -19,7 +20,7 @@ constexpr int LN_MAX_D = 8192;
 
 // 16 bytes of a row in a register quad.  The vector types carry the element's alignment only: gfx950 loads and stores 16 bytes
 // at any element address, so rows of odd width or stride take the same path (single elements instead: 23 us for the backward
-// pass of 5001 x 1023 fp32).  The last piece of a row that ends inside it (TAIL) is moved element by element.
+// pass of 5001 x 1023 fp32).  down(n): element n becomes the first, zeros follow the last.  store_first(n): the first n alone.
 template <class T> struct Piece;
 template <> struct Piece<bf16> {
     static constexpr int V = 8;
@@ -38,6 +39,19 @@ template <> struct Piece<bf16> {
         r[j >> 1] = (j & 1) ? (r[j >> 1] & 0xffffu) | (u << 16) : (r[j >> 1] & 0xffff0000u) | u;
     }
     __device__ __forceinline__ bf16 one(int j) const { return __builtin_bit_cast(bf16, (unsigned short)(r[j >> 1] >> (16 * (j & 1)))); }
+    __device__ __forceinline__ void down(int n) {
+        if (n & 4) r = u32x4{r[2], r[3], 0u, 0u};
+        if (n & 2) r = u32x4{r[1], r[2], r[3], 0u};
+        if (n & 1) r = u32x4{r[0] >> 16 | r[1] << 16, r[1] >> 16 | r[2] << 16, r[2] >> 16 | r[3] << 16, r[3] >> 16};
+    }
+    __device__ __forceinline__ void store_first(int n, bf16* at) const {
+        typedef u32x2 __attribute__((aligned(2))) At4;
+        typedef uint32_t __attribute__((aligned(2))) At2;
+        u32x4 v = r;
+        if (n & 4) { *reinterpret_cast<At4*>(at) = u32x2{v[0], v[1]}; v = u32x4{v[2], v[3], 0u, 0u}; at += 4; }
+        if (n & 2) { *reinterpret_cast<At2*>(at) = v[0]; v[0] = v[1]; at += 2; }
+        if (n & 1) *at = __builtin_bit_cast(bf16, (unsigned short)v[0]);
+    }
 };
 template <> struct Piece<float> {
     static constexpr int V = 4;
@@ -47,28 +61,52 @@ template <> struct Piece<float> {
     __device__ __forceinline__ void put(const float (&f)[4]) { r = f32x4{f[0], f[1], f[2], f[3]}; }
     __device__ __forceinline__ void put_one(int j, float x) { r[j] = x; }
     __device__ __forceinline__ float one(int j) const { return r[j]; }
+    __device__ __forceinline__ void down(int n) {
+        if (n & 2) r = f32x4{r[2], r[3], 0.f, 0.f};
+        if (n & 1) r = f32x4{r[1], r[2], r[3], 0.f};
+    }
+    __device__ __forceinline__ void store_first(int n, float* at) const {
+        typedef f32x2 __attribute__((aligned(4))) At2;
+        f32x4 v = r;
+        if (n & 2) { *reinterpret_cast<At2*>(at) = f32x2{v[0], v[1]}; v[0] = v[2]; at += 2; }
+        if (n & 1) *at = v[0];
+    }
 };
-// elements c .. c + V - 1 of a row of d (zeros past its end); STREAM: read once, past the caches
-template <bool STREAM, bool TAIL, class T>
+// How a row ends.  FITS: with a whole piece.  LAPS: inside its last piece, which is loaded whole from d - V on and moved down by
+// `settle` when all loads are on their way (single elements, each waited for: 139264 x 767 bf16 forward 144 us, backward 311).
+// SHORT: the row is shorter than a piece; single elements.  Elements past the end are zeros.
+enum End : int { FITS, LAPS, SHORT };
+// STREAM: read once, past the caches
+template <bool STREAM, End END, class T>
 __device__ __forceinline__ void load_piece(Piece<T>& p, const T* row, int c, int d) {
     typedef typename Piece<T>::At At;
     p.r = decltype(p.r){};
-    if (!TAIL || c + Piece<T>::V <= d) {
-        if (c < d) p.r = STREAM ? __builtin_nontemporal_load(reinterpret_cast<const At*>(row + c)) : *reinterpret_cast<const At*>(row + c);
-    } else if (c < d) {
+    if (END == SHORT) {
 #pragma unroll
         for (int j = 0; j < Piece<T>::V; ++j) if (c + j < d) p.put_one(j, row[c + j]);
+    } else if (c < d) {
+        const At* at = reinterpret_cast<const At*>(row + (END == LAPS ? min(c, d - Piece<T>::V) : c));
+        p.r = STREAM ? __builtin_nontemporal_load(at) : *at;
     }
 }
-template <bool TAIL, class T>
+template <End END, class T>
+__device__ __forceinline__ void settle(Piece<T>& p, int c, int d) {
+    if (END == LAPS && c < d && c + Piece<T>::V > d) p.down(Piece<T>::V - d % Piece<T>::V);
+}
+template <End END, class T>
 __device__ __forceinline__ void store_piece(const Piece<T>& p, T* row, int c, int d) {
     typedef typename Piece<T>::At At;
-    if (!TAIL || c + Piece<T>::V <= d) {
-        if (c < d) __builtin_nontemporal_store(p.r, reinterpret_cast<At*>(row + c));
-    } else if (c < d) {
+    if (END == SHORT) {
 #pragma unroll
         for (int j = 0; j < Piece<T>::V; ++j) if (c + j < d) row[c + j] = p.one(j);
-    }
+    } else if (END == FITS || c + Piece<T>::V <= d) {
+        if (c < d) {
+            // past the caches, but for bf16 rows at odd addresses, whose pieces share lines (139264 x 767: forward 108 us against
+            // 114, backward 167 against 187; fp32 the other way, 168 against 166 and 270 against 266)
+            if (END == LAPS && sizeof(T) == 2) *reinterpret_cast<At*>(row + c) = p.r;
+            else __builtin_nontemporal_store(p.r, reinterpret_cast<At*>(row + c));
+        }
+    } else if (c < d) p.store_first(d % Piece<T>::V, row + c);
 }
 
 // sum over the TEAM threads of a row (16 or 64 lanes of a wave, or the whole workgroup through `sh`, two sets of four slots)
@@ -94,12 +132,13 @@ template <class T> struct LnFwd {
 
 // (w and b are requested together with the row: behind the row's sums, from the caches, 1 x 768 took 5.2 us instead of 4.7,
 // 4000 x 768 8.0 instead of 7.2, 139264 x 768 the same 148)
-template <class T, int TEAM, int PER, bool TAIL>
+template <class T, int TEAM, int PER, End END>
 __global__ void __launch_bounds__(LN_BLOCK) ln_fwd_kernel(LnFwd<T> a) {
     constexpr int V = Piece<T>::V, RPB = LN_BLOCK / TEAM;
     __shared__ float sh[4][4];
     const int l = threadIdx.x % TEAM, t = threadIdx.x / TEAM;
     const float inv_d = 1.f / (float)a.d;
+    const int last = a.d % V;                               // elements of a last piece that the row ends inside
     for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.M; row0 += (long long)gridDim.x * RPB) {
         const bool ok = row0 + t < a.M;
         const size_t row = ok ? row0 + t : a.M - 1;         // a team past the end repeats the last row and stores nothing
@@ -107,34 +146,47 @@ __global__ void __launch_bounds__(LN_BLOCK) ln_fwd_kernel(LnFwd<T> a) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int c = (l + i * TEAM) * V;
-            load_piece<true, TAIL>(p[i], a.x + row * a.ldx, c, a.d);
-            if (a.res) load_piece<true, TAIL>(q[i], a.res + row * a.ldr, c, a.d);
-            load_piece<false, TAIL>(w[i], a.w, c, a.d);
-            load_piece<false, TAIL>(b[i], a.b, c, a.d);
+            load_piece<true, END>(p[i], a.x + row * a.ldx, c, a.d);
+            if (a.res) load_piece<true, END>(q[i], a.res + row * a.ldr, c, a.d);
+            load_piece<false, END>(w[i], a.w, c, a.d);
+            load_piece<false, END>(b[i], a.b, c, a.d);
         }
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int c = (l + i * TEAM) * V;
+            settle<END>(p[i], c, a.d);
+            settle<END>(w[i], c, a.d);
+            settle<END>(b[i], c, a.d);
             if (a.res) {
+                settle<END>(q[i], c, a.d);
                 float f[V];
 #pragma unroll
                 for (int j = 0; j < V; ++j) f[j] = p[i].get(j) + q[i].get(j);
                 p[i].put(f);
-                if (ok) store_piece<TAIL>(p[i], a.xsum + row * a.lds, c, a.d);
+                if (END != LAPS && ok) store_piece<END>(p[i], a.xsum + row * a.lds, c, a.d);
             }
 #pragma unroll
             for (int j = 0; j < V; ++j) sum += p[i].get(j);
         }
         const float mean = team_sum<TEAM>(sum, sh[0]) * inv_d;
+        if (END == LAPS && a.res && ok)                     // (xsum may be res: behind the sum, when pieces that lap have been read)
+#pragma unroll
+            for (int i = 0; i < PER; ++i) store_piece<END>(p[i], a.xsum + row * a.lds, (l + i * TEAM) * V, a.d);
         float sq = 0.f;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int c = (l + i * TEAM) * V;
-            if (c < a.d) {
+            if (END == FITS ? c < a.d : c + V <= a.d) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const float f = TAIL && c + j >= a.d ? 0.f : p[i].get(j) - mean;
+                    const float f = p[i].get(j) - mean;
+                    sq += f * f;
+                }
+            } else if (END != FITS && c < a.d) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float f = j < last ? p[i].get(j) - mean : 0.f;
                     sq += f * f;
                 }
             }
@@ -152,7 +204,7 @@ __global__ void __launch_bounds__(LN_BLOCK) ln_fwd_kernel(LnFwd<T> a) {
 #pragma unroll
             for (int j = 0; j < V; ++j) f[j] = (p[i].get(j) - mean) * rstd * w[i].get(j) + b[i].get(j);
             o.put(f);
-            if (ok) store_piece<TAIL>(o, a.y + row * a.ldy, c, a.d);
+            if (ok) store_piece<END>(o, a.y + row * a.ldy, c, a.d);
         }
         if (TEAM > 64) __syncthreads();                     // the next row's sums reuse `sh`
     }
@@ -169,7 +221,7 @@ template <class T> struct LnBwd {
 
 // two waves per SIMD: a thread carries its pieces of three rows and two column sums in up to 256 registers (one wave and 512
 // for fp32 rows of more than 4096)
-template <class T, int TEAM, int PER, bool TAIL>
+template <class T, int TEAM, int PER, End END>
 __global__ void __launch_bounds__(LN_BLOCK) __attribute__((amdgpu_waves_per_eu(PER < 8 ? 2 : 1)))
 ln_bwd_kernel(LnBwd<T> a) {
     constexpr int V = Piece<T>::V, RPB = LN_BLOCK / TEAM;
@@ -189,10 +241,10 @@ ln_bwd_kernel(LnBwd<T> a) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int c = (l + i * TEAM) * V;
-            load_piece<true, TAIL>(p[i], a.dy + row * a.lddy, c, a.d);
-            load_piece<true, TAIL>(q[i], a.x + row * a.ldx, c, a.d);
+            load_piece<true, END>(p[i], a.dy + row * a.lddy, c, a.d);
+            load_piece<true, END>(q[i], a.x + row * a.ldx, c, a.d);
             r[i].r = decltype(r[i].r){};
-            if (a.dres) load_piece<true, TAIL>(r[i], a.dres + row * a.ldr, c, a.d);
+            if (a.dres) load_piece<true, END>(r[i], a.dres + row * a.ldr, c, a.d);
         }
         const float mean = a.mean[row], rstd = a.rstd[row];
         float sg = 0.f, sgx = 0.f;
@@ -201,7 +253,10 @@ ln_bwd_kernel(LnBwd<T> a) {
             const int c = (l + i * TEAM) * V;
             if (c < a.d) {                                  // (past the end of a row dy and w are zeros)
                 Piece<T> w;
-                load_piece<false, TAIL>(w, a.w, c, a.d);
+                load_piece<false, END>(w, a.w, c, a.d);
+                settle<END>(p[i], c, a.d);
+                settle<END>(q[i], c, a.d);
+                settle<END>(w, c, a.d);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const float dy = p[i].get(j), xh = (q[i].get(j) - mean) * rstd, g = dy * w.get(j);
@@ -217,7 +272,9 @@ ln_bwd_kernel(LnBwd<T> a) {
         for (int i = 0; i < PER; ++i) {
             const int c = (l + i * TEAM) * V;
             Piece<T> w, o;
-            load_piece<false, TAIL>(w, a.w, c, a.d);
+            load_piece<false, END>(w, a.w, c, a.d);
+            settle<END>(r[i], c, a.d);
+            settle<END>(w, c, a.d);
             float f[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) {
@@ -225,7 +282,7 @@ ln_bwd_kernel(LnBwd<T> a) {
                 f[j] = rstd * (p[i].get(j) * w.get(j) - sg - xh * sgx) + r[i].get(j);
             }
             o.put(f);
-            if (ok) store_piece<TAIL>(o, a.dx + row * a.lddx, c, a.d);
+            if (ok) store_piece<END>(o, a.dx + row * a.lddx, c, a.d);
         }
         if (TEAM > 64) __syncthreads();
     }
@@ -297,22 +354,22 @@ __global__ void __launch_bounds__(32 * COLS_LANES) ln_cols_kernel(const float* _
 
 constexpr int LN_BWD_PER_CU = 4;           // most workgroups of the backward kernel for a compute unit (the workspace's rows)
 
-template <class T, int TEAM, int PER, bool TAIL>
+template <class T, int TEAM, int PER, End END>
 int ln_go(const LnFwd<T>& a, hipStream_t s) {
     const long long blocks = ((long long)a.M + LN_BLOCK / TEAM - 1) / (LN_BLOCK / TEAM);
     const int grid = (int)(blocks < 8192 ? blocks : 8192);
-    hipLaunchKernelGGL((ln_fwd_kernel<T, TEAM, PER, TAIL>), dim3(grid), dim3(LN_BLOCK), 0, s, a);
+    hipLaunchKernelGGL((ln_fwd_kernel<T, TEAM, PER, END>), dim3(grid), dim3(LN_BLOCK), 0, s, a);
     PACED_CHECK_LAUNCH();
     return PACED_OK;
 }
-template <class T, int TEAM, int PER, bool TAIL>
+template <class T, int TEAM, int PER, End END>
 int ln_go(const LnBwd<T>& a, hipStream_t s) {
     // resident workgroups: up to 16 elements a thread need at most 128 registers, four to a compute unit; more need up to 256
     const int most = (PER * Piece<T>::V <= 16 ? LN_BWD_PER_CU : 2) * paced_cu_count();
     const long long rounds_of = ((long long)a.M + LN_BLOCK / TEAM - 1) / (LN_BLOCK / TEAM), rounds = (rounds_of + most - 1) / most;
     const int grid = (int)((rounds_of + rounds - 1) / rounds);          // every workgroup the same number of row groups
     const int smem = TEAM < LN_BLOCK && a.part ? 4 * a.d * 4 : 0;              // 32 KiB at most: these teams take d <= 2048
-    hipLaunchKernelGGL((ln_bwd_kernel<T, TEAM, PER, TAIL>), dim3(grid), dim3(LN_BLOCK), smem, s, a);
+    hipLaunchKernelGGL((ln_bwd_kernel<T, TEAM, PER, END>), dim3(grid), dim3(LN_BLOCK), smem, s, a);
     PACED_CHECK_LAUNCH();
     if (!a.part) return PACED_OK;
     hipLaunchKernelGGL(ln_cols_kernel, dim3((2 * a.d + 31) / 32), dim3(32 * COLS_LANES), 0, s, a.part, grid, a.d, a.dw, a.db);
@@ -321,24 +378,26 @@ int ln_go(const LnBwd<T>& a, hipStream_t s) {
 }
 
 // the narrowest team whose registers hold a row of d elements
-template <class T, bool TAIL, class Args>
+template <class T, End END, class Args>
 int ln_team(const Args& a, hipStream_t s) {
     const int n = (a.d + Piece<T>::V - 1) / Piece<T>::V;     // pieces of a row
-    if (n <= 16) return ln_go<T, 16, 1, TAIL>(a, s);
-    if (n <= 32) return ln_go<T, 16, 2, TAIL>(a, s);
-    if (n <= 64) return ln_go<T, 16, 4, TAIL>(a, s);
-    if (n <= 96) return ln_go<T, 16, 6, TAIL>(a, s);
-    if (n <= 128) return ln_go<T, 64, 2, TAIL>(a, s);
-    if (n <= 256) return ln_go<T, 64, 4, TAIL>(a, s);
-    if (n <= 512) return ln_go<T, 256, 2, TAIL>(a, s);
-    if (n <= 1024) return ln_go<T, 256, 4, TAIL>(a, s);
-    if constexpr (Piece<T>::V * 1024 < LN_MAX_D) return ln_go<T, 256, 8, TAIL>(a, s);
+    if (n <= 16) return ln_go<T, 16, 1, END>(a, s);
+    if constexpr (END != SHORT) {
+        if (n <= 32) return ln_go<T, 16, 2, END>(a, s);
+        if (n <= 64) return ln_go<T, 16, 4, END>(a, s);
+        if (n <= 96) return ln_go<T, 16, 6, END>(a, s);
+        if (n <= 128) return ln_go<T, 64, 2, END>(a, s);
+        if (n <= 256) return ln_go<T, 64, 4, END>(a, s);
+        if (n <= 512) return ln_go<T, 256, 2, END>(a, s);
+        if (n <= 1024) return ln_go<T, 256, 4, END>(a, s);
+        if constexpr (Piece<T>::V * 1024 < LN_MAX_D) return ln_go<T, 256, 8, END>(a, s);
+    }
     return PACED_ERR_ARG;                                    // (d <= LN_MAX_D was checked)
 }
 template <class T, class Args>
 int ln_launch(const Args& a, hipStream_t s) {
     static_assert(1024 * Piece<bf16>::V >= LN_MAX_D && 2048 * Piece<float>::V >= LN_MAX_D, "the widest teams hold the widest row");
-    return a.d % Piece<T>::V ? ln_team<T, true>(a, s) : ln_team<T, false>(a, s);
+    return a.d < Piece<T>::V ? ln_team<T, SHORT>(a, s) : a.d % Piece<T>::V ? ln_team<T, LAPS>(a, s) : ln_team<T, FITS>(a, s);
 }
 
 template <class T>

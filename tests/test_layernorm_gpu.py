@@ -117,6 +117,29 @@ def test_outputs_in_the_place_of_inputs():
     assert torch.equal(d2, dx)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("d", [3, 9, 127, 250, 767, 1001, 1535, 2049, 4093, 8190])
+def test_rows_that_end_inside_a_piece_in_the_place_of_inputs(d, dtype):
+    """(every team's width, rows whose last piece is read from the one before it)"""
+    M = 70
+    x, res, dy, dres, w, b = make(M, d, dtype, d)
+    y, mean, rstd = torch.empty_like(x), torch.empty(M, device="cuda"), torch.empty(M, device="cuda")
+    s = (x.float() + res.float()).to(dtype)
+    r2 = res.clone()
+    K.layernorm_fwd(x, w, b, y, mean, rstd, res=r2, xsum=r2)
+    assert torch.equal(r2, s)
+    check_fwd(y, s, w, b, 1e-5)
+    x2, r3 = x.clone(), res.clone()
+    K.layernorm_fwd(x2, w, b, x2, res=r3, xsum=r3)
+    assert torch.equal(x2, y) and torch.equal(r3, s)
+    dx, dw, db = torch.empty_like(x), torch.full((d,), 0.5, device="cuda"), torch.full((d,), -0.25, device="cuda")
+    K.layernorm_bwd(dy, s, w, mean, rstd, dx, dres=dres, dw=dw, db=db)
+    check_bwd(dx, dw, db, dy, s, w, dres, 1e-5, 0.5, -0.25)
+    d2 = dy.clone()
+    K.layernorm_bwd(d2, s, w, mean, rstd, d2, dres=dres)
+    assert torch.equal(d2, dx)
+
+
 def test_gradients_are_the_same_bits_every_time_and_each_is_optional():
     x, _, dy, _, w, b = make(4000, 768, BF16, 8)
     y, mean, rstd, dx = torch.empty_like(x), torch.empty(4000, device="cuda"), torch.empty(4000, device="cuda"), torch.empty_like(x)
