@@ -23,7 +23,7 @@ PROFILE = None
 
 def _stream():
     # (the raw handle: torch.cuda.current_stream() builds a Stream object, 2.5 us for each of a step's launches)
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _p(t):
@@ -52,14 +52,15 @@ def _elsewhere(**tensors):
     for name, t in tensors.items():
         if t is None:
             continue
-        d = t.device
-        if d.type != "cuda":
+        d = t.get_device()                               # (an int, -1 for host memory: a device object costs twice that)
+        if d == dev:
+            continue
+        if d < 0:
             raise ValueError(f"{name} must be a device tensor")
-        if dev is None:
-            dev = d
-        elif d != dev:
-            raise ValueError(f"{name} is on {d}, the tensors before it on {dev}")
-    return None if dev.index == torch.cuda.current_device() else dev
+        if dev is not None:
+            raise ValueError(f"{name} is on {t.device}, the tensors before it on cuda:{dev}")
+        dev = d
+    return None if dev == torch._C._cuda_getDevice() else torch.device("cuda", dev)
 
 
 def _rows_of(t, shape, dtype, name):
