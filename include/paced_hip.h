@@ -186,10 +186,10 @@ int paced_layernorm_bwd(const void* dy, int lddy, const void* x, int ldx, const 
  * head-major as in paced_gemm_bf16_heads: lddy = 64 and dy_heads > 0; the rows up to the next multiple of 64 must then be
  * finite); M % 8 == 0, N % 16 == 0, lddw % 4 == 0.  Products are exact, sums fp32 in a fixed order (no atomics).
  * accumulate = 0: dw is written, 1: added to.  workspace, 16-byte aligned, not kept between calls, for one stream at a time:
- * paced_act8_dweight_workspace_bytes(T, M, N, accumulate) bytes (0: none needed). */
+ * paced_act8_dweight_workspace_bytes(T, M, N) bytes (0: none needed). */
 int paced_act8_quantize(const void* x, int ldx, void* q, void* scale, int T, int n, void* stream);
 int paced_act8_dequantize(const void* q, const void* scale, void* y, int ldy, int T, int n, void* stream);
-size_t paced_act8_dweight_workspace_bytes(int T, int M, int N, int accumulate);
+size_t paced_act8_dweight_workspace_bytes(int T, int M, int N);
 int paced_act8_dweight(const void* dy, int lddy, long long dy_heads, const void* q, const void* scale, float* dw, int lddw,
                        int T, int M, int N, int accumulate, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -9,9 +9,11 @@
 // Blocks run along the tokens because a weight gradient contracts over tokens: all eight values of a lane's MFMA fragment
 // (eight tokens of one feature) share one scale, and v_cvt_scalef32_pk_bf16_fp8 applies it while it converts.
 // Writing and reading are bound by memory: 139264 x 768 in 51.5 us (6.3 TB/s) and 55 us (5.9 TB/s).  The gradient is bound by the
-// matrix cores where tokens are many: 2304 x 768 from 139264 tokens in 411 us with the slabs' sum, 1.20 PFLOP/s (the bf16
-// products of gemm.hip reach 1.25 to 1.35 on large squares, the vendor's 1.39); 512 x 2048 from 1001 tokens in 9.7 us, by latency.
+// matrix cores where tokens are many: 2304 x 768 from 139264 tokens in 411 to 442 us on different cards, slabs' sum
+// included (1.12 to 1.20 PFLOP/s; the bf16 products of gemm.hip reach 1.25 to 1.35 on large squares, the vendor's 1.39);
+// 512 x 2048 from 1001 tokens in 8.5 us, by latency.
 #include "gemm_tiles.h"
+#include <type_traits>
 
 namespace {
 
@@ -98,7 +100,7 @@ __global__ void __launch_bounds__(256) act8_dequantize_kernel(const unsigned cha
 
 // ------------------------------------------------------------------------------------------------ weight gradient
 // dw[m][n] = sum over tokens t of dy[t][m] x[t][n], x the checkpoint's values.  The tokens are cut into `splits` slices whose
-// sums go to slabs [splits][M][N] and are added by a second kernel in a fixed order; one slice writes dw itself.
+// sums go to slabs [splits][M][N] and are added by a second kernel in a fixed order; one slice writes dw, or adds to it, itself.
 struct DwParams {
     const bf16* dy;
     const unsigned char *q, *scale;
@@ -107,7 +109,14 @@ struct DwParams {
     long long heads;                   // > 0: dy is head-major (features 64h .. 64h + 63 at dy + h * heads, rows of 64)
     int k_per_split;                   // a multiple of 64
     long long slab;                    // elements between the slabs
+    int add;                           // out is dw and is added to
 };
+
+template <bool ADD>
+__device__ __forceinline__ void put4(float* at, f32x4 v) {
+    if (ADD) v += *reinterpret_cast<const f32x4*>(at);
+    *reinterpret_cast<f32x4*>(at) = v;
+}
 
 struct DwItem {
     int m0, n0, split, kbeg, kend;
@@ -148,34 +157,34 @@ __device__ __forceinline__ bf16x8 act8_fragment(u32x2 c, uint32_t code) {
     return bf16x8{a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
 }
 
-// 64x64 tile, four waves of 32x32, a ring of NS K steps (64 tokens) per workgroup, three workgroups to a compute unit.
+// 64x64 tile, eight waves, a ring of NS K steps (64 tokens) per workgroup, three workgroups to a compute unit.  Waves 0-3 hold
+// 32x32 quarters of a step's first 32 tokens' product, waves 4-7 of the second's; their sums meet in LDS at the end.  Four
+// waves with all 64 tokens took 9.2 us instead of 8.5 for 512 x 2048 from 1001 tokens, 12.2 instead of 10.9 for 2048 x 512 from
+// 1500, but 4.4 instead of 4.9 from 33.
 // LDS of one step: dy's image [64 tokens][64] bf16 (gemm_tiles.h), the codes' image [64 tokens][64] bytes whose 16-byte
 // units u of token k sit at u ^ ((k >> 2) & 1) (the eight tokens that ds_read_b64_tr_b8 gathers then fall on different
-// banks), and each wave's 2 x 32 scale bytes.
-constexpr int DW_A = 8192, DW_B = 4096, DW_STEP = DW_A + DW_B + 1024, DW_NS = 4, DW_PER = 4;
-__global__ void __launch_bounds__(256) act8_dw_kernel(DwParams p, int ntm, int ntn, int total) {
+// banks), and each quarter's 2 x 32 scale bytes.
+constexpr int DW_A = 8192, DW_B = 4096, DW_STEP = DW_A + DW_B + 1024, DW_NS = 4, DW_PER = 2;
+__global__ void __launch_bounds__(512) act8_dw_kernel(DwParams p, int ntm, int ntn, int total) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave >> 2, w = wave & 3;
     const int wm = w >> 1, wn = w & 1;
     const DwItem it = dw_item<64, 64>(p, xcd_remap(blockIdx.x, total), ntm, ntn);
-    uint32_t offA[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) offA[i] = stage_offset<true, 64>((i * 4 + w) * 64 + lane, p.lddy, p.heads);
+    const uint32_t offA = stage_offset<true, 64>(wave * 64 + lane, p.lddy, p.heads);
+    // waves 0-3 fetch the codes too, waves 4-7 the scales: lanes 0-7 the step's first 32 tokens' of a quarter's 32 features,
+    // lanes 8-15 the second's; the others' offset lies outside every descriptor
     const int gk = (w * 64 + lane) >> 2, gc = ((w * 64 + lane) & 3) ^ ((gk >> 2) & 1);
     const uint32_t offB = (uint32_t)(gk * p.N + gc * 16);
-    // lanes 0-7: the step's first 32 tokens' scales of this wave's 32 features, lanes 8-15: the second's; the others' offset
-    // lies outside every descriptor
     const uint32_t offS = lane < 16 ? (uint32_t)((lane >> 3) * p.N + wn * 32 + (lane & 7) * 4) : 0x80000000u;
     const uint32_t strideA = (uint32_t)p.lddy * 2u;
     const int nsteps = (it.kend - it.kbeg + BK - 1) / BK;
     auto stage = [&](int t, int buf) {
         char* l = smem + buf * DW_STEP;
         const uint32_t k = (uint32_t)t * BK;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(it.rA, LDS_PTR(l + (i * 4 + w) * 1024), 16, offA[i], k * strideA, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(it.rB, LDS_PTR(l + DW_A + w * 1024), 16, offB, k * (uint32_t)p.N, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(it.rS, LDS_PTR(l + DW_A + DW_B + w * 256), 4, offS, (k / QBLOCK) * (uint32_t)p.N, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(it.rA, LDS_PTR(l + wave * 1024), 16, offA, k * strideA, 0, 0);
+        if (half == 0) __builtin_amdgcn_raw_ptr_buffer_load_lds(it.rB, LDS_PTR(l + DW_A + w * 1024), 16, offB, k * (uint32_t)p.N, 0, 0);
+        else __builtin_amdgcn_raw_ptr_buffer_load_lds(it.rS, LDS_PTR(l + DW_A + DW_B + w * 256), 4, offS, (k / QBLOCK) * (uint32_t)p.N, 0, 0);
     };
     f32x4 acc[2][2];
 #pragma unroll
@@ -186,58 +195,63 @@ __global__ void __launch_bounds__(256) act8_dw_kernel(DwParams p, int ntm, int n
     for (int s = 0; s < DW_NS - 1; ++s)
         if (s < nsteps) stage(s, s);
     int buf = 0, nbuf = DW_NS - 1;
-    // addresses of this lane's fragment reads inside a step's images (kk = 0; kk = 1 is 32 tokens on)
+    // addresses of this lane's fragment reads inside a step's images
     const int g = lane >> 4, i16 = lane & 15;
     uint32_t rdA[2], rdB[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int u = (wm * 32 + i * 16) >> 4, hk = ((i16 >> 2) | ((g & 1) << 2)) & 3;
-        rdA[i] = (uint32_t)((8 * g + (i16 >> 2)) * 128 + ((u ^ hk) << 5) + (i16 & 3) * 8);
+        rdA[i] = (uint32_t)((half * 32 + 8 * g + (i16 >> 2)) * 128 + ((u ^ hk) << 5) + (i16 & 3) * 8);
         const int kb = 8 * g + (i16 >> 1);
-        rdB[i] = (uint32_t)(DW_A + kb * 64 + (((wn * 2 + i) ^ ((kb >> 2) & 1)) << 4) + (i16 & 1) * 8);
+        rdB[i] = (uint32_t)(DW_A + (half * 32 + kb) * 64 + (((wn * 2 + i) ^ ((kb >> 2) & 1)) << 4) + (i16 & 1) * 8);
     }
-    const uint32_t rdS = (uint32_t)(DW_A + DW_B + w * 256 + i16);
+    const uint32_t rdS = (uint32_t)(DW_A + DW_B + w * 256 + half * 32 + i16);
     for (int t = 0; t < nsteps; ++t) {
         if (t + DW_NS - 2 < nsteps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DW_NS - 2) * DW_PER) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         PACED_PINNED_BARRIER();
         if (t + DW_NS - 1 < nsteps) stage(t + DW_NS - 1, nbuf);
         const uint32_t l = (uint32_t)(uintptr_t)LDS_PTR(smem + buf * DW_STEP);
+        bf16x4 lo[2], hi[2];
+        u32x2 c[2];
+        uint32_t s[2];
+        // (inline assembly: next to LDS-DMA the compiler would drain every load in flight ahead of a read it can see)
+        asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+                     "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+                     "ds_read_b64_tr_b8 %4, %10\n\tds_read_b64_tr_b8 %5, %11\n\t"
+                     "ds_read_u8 %6, %13\n\tds_read_u8 %7, %13 offset:16\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(c[0]), "=&v"(c[1]), "=&v"(s[0]), "=&v"(s[1])
+                     : "v"(l + rdA[0]), "v"(l + rdA[1]), "v"(l + rdB[0]), "v"(l + rdB[1]), "n"(4 * 128), "v"(l + rdS)
+                     : "memory");
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            bf16x4 lo[2], hi[2];
-            u32x2 c[2];
-            uint32_t s[2];
-            // (inline assembly: next to LDS-DMA the compiler would drain every load in flight ahead of a read it can see)
-            asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
-                         "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
-                         "ds_read_b64_tr_b8 %4, %10 offset:%14\n\tds_read_b64_tr_b8 %5, %11 offset:%14\n\t"
-                         "ds_read_u8 %6, %15 offset:%16\n\tds_read_u8 %7, %15 offset:%17\n\ts_waitcnt lgkmcnt(0)"
-                         : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(c[0]), "=&v"(c[1]), "=&v"(s[0]), "=&v"(s[1])
-                         : "v"(l + rdA[0]), "v"(l + rdA[1]), "v"(l + rdB[0]), "v"(l + rdB[1]), "n"(kk * 32 * 128), "n"(kk * 32 * 128 + 4 * 128),
-                           "n"(kk * 32 * 64), "v"(l + rdS), "n"(kk * 32), "n"(kk * 32 + 16)
-                         : "memory");
-            __builtin_amdgcn_sched_barrier(0);
+        for (int j = 0; j < 2; ++j) {
+            const bf16x8 fb = act8_fragment(c[j], s[j]);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const bf16x8 fb = act8_fragment(c[j], s[j]);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, __builtin_shufflevector(lo[i], hi[i], 0, 1, 2, 3, 4, 5, 6, 7), acc[i][j], 0, 0, 0);
-            }
+            for (int i = 0; i < 2; ++i)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, __builtin_shufflevector(lo[i], hi[i], 0, 1, 2, 3, 4, 5, 6, 7), acc[i][j], 0, 0, 0);
         }
         buf = buf + 1 == DW_NS ? 0 : buf + 1;
         nbuf = nbuf + 1 == DW_NS ? 0 : nbuf + 1;
     }
+    __syncthreads();                                  // the last step has been read: its LDS takes the second half's sums
+    f32x4* const sums = reinterpret_cast<f32x4*>(smem) + w * 256 + lane;
+    if (half)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sums[k * 64] = acc[k >> 1][k & 1];
+    __syncthreads();
+    if (half) return;
     float* out = p.out + (size_t)it.split * p.slab;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int m = it.m0 + wm * 32 + i * 16 + i16;
-        if (m >= p.M) continue;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int n = it.n0 + wn * 32 + j * 16 + g * 4;
-            if (n < p.N) *reinterpret_cast<f32x4*>(out + (size_t)m * p.ldout + n) = acc[i][j];        // N is a multiple of 16
+            const f32x4 v = acc[i][j] + sums[(i * 2 + j) * 64];
+            if (m >= p.M || n >= p.N) continue;                                                      // N is a multiple of 16
+            if (p.add) put4<true>(out + (size_t)m * p.ldout + n, v);
+            else put4<false>(out + (size_t)m * p.ldout + n, v);
         }
     }
 }
@@ -413,16 +427,19 @@ __global__ void __launch_bounds__(512) act8_dw_phased_kernel(DwParams p, int ntm
         }
         if (wr == 0) __builtin_amdgcn_s_barrier();       // both groups run their epilogues side by side (see gemm.hip)
         float* out = p.out + (size_t)cur.split * p.slab;
+        auto store = [&](auto add) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int m = cur.m0 + CfgPhased::moff(wr, i) + i16;
-            if (m >= p.M) continue;
+            for (int i = 0; i < 8; ++i) {
+                const int m = cur.m0 + CfgPhased::moff(wr, i) + i16;
+                if (m >= p.M) continue;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int n = cur.n0 + CfgPhased::noff(wc, j) + g * 4;
-                if (n < p.N) *reinterpret_cast<f32x4*>(out + (size_t)m * p.ldout + n) = acc[i][j];
+                for (int j = 0; j < 4; ++j) {
+                    const int n = cur.n0 + CfgPhased::noff(wc, j) + g * 4;
+                    if (n < p.N) put4<add()>(out + (size_t)m * p.ldout + n, acc[i][j]);
+                }
             }
-        }
+        };
+        if (p.add) store(std::true_type()); else store(std::false_type());
         const int Ln = item_of(b, ++round, G, total);
         if (Ln < 0) break;
         cur = dw_item<256, 256>(p, Ln, ntm, ntn);
@@ -450,31 +467,31 @@ __global__ void __launch_bounds__(256) slab_sum_kernel(const float* __restrict__
     }
 }
 
-// Which tiles, and how many slices of the tokens.  256x256 tiles run at almost three times the rate of 64x64 ones, so they are
-// taken when they waste less than that at the output's edges and when tiles times slices (of 12 K steps or more) give most
-// compute units one.  Both sides, slabs' sum apart: 139264 tokens, 2304 x 768 in 468 us against 1160, 17408, 768 x 2048 in 61
-// against 89, 4352, 2304 x 768 in 36.6 against 36.8; but 8704, 768 x 768 in 34 against 23, 1001, 512 x 2048 in 35 against 10.5.
+// Which tiles, and how many slices of the tokens: the plan with the least time by what the kernels were measured to take.  A
+// 64x64 tile's workgroup 3.2 us and 0.31 for each K step of 64 tokens, half of that more for each further workgroup of its
+// compute unit; a 256x256 tile's 10 us and 1.4 for a step; several slices 3 us for the second kernel, and their slabs written
+// and read at 4.5 and 7.5 TB/s.  Good to about a tenth.  Both sides of it, in us: 1001 tokens, 768 x 768, 64x64 tiles, 1 slice
+// 8.0, 4 slices 14.0; 4352, 512 x 512, 4 slices 12.7, 1 slice 23.1, 12 slices 16.6; 4352, 2304 x 768, 64x64 30.5, 256x256 38.5;
+// 8704, 768 x 768, 5 slices 25.5, 4 slices 27.7; 8704, 2304 x 768, 64x64 56, 256x256 50; 139264, 768 x 768, 64x64 300, 256x256 156.
 struct DwPlan { int tile, ntm, ntn, splits, k_per_split; };
 DwPlan dw_plan(int T, int M, int N) {
-    DwPlan pl;
     const int ktiles = (T + BK - 1) / BK, cus = paced_cu_count();
-    const long long t256 = (long long)((M + 255) / 256) * ((N + 255) / 256), t64 = (long long)((M + 63) / 64) * ((N + 63) / 64);
-    long long splits = t256 >= cus ? 1 : cus / t256;
-    if (splits > ktiles / 12) splits = ktiles / 12 > 0 ? ktiles / 12 : 1;
-    if (t256 * splits * 8 >= cus * 5 && t256 * 16 * 2 < t64 * 5) {
-        pl.tile = 256;
-        pl.ntm = (M + 255) / 256;
-        pl.ntn = (N + 255) / 256;
-    } else {
-        pl.tile = 64;
-        pl.ntm = (M + 63) / 64;
-        pl.ntn = (N + 63) / 64;
-        splits = t64 >= 3LL * cus || (t64 * 4 >= cus * 3 && ktiles <= 24) ? 1 : 3LL * cus / t64;       // (few tokens: the slabs would cost more than they save)
-        if (splits > (ktiles + 3) / 4) splits = (ktiles + 3) / 4;
+    const double slab = (double)M * N * 8.;
+    DwPlan pl = {};
+    double best = 1e300;
+    for (int tile = 64; tile <= 256; tile += 192) {
+        const long long tiles = (long long)((M + tile - 1) / tile) * ((N + tile - 1) / tile);
+        for (const int c : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 0, -1}) {                     // 0, -1: one or three tiles to a compute unit
+            int splits = c > 0 ? c : (int)((c ? 3 : 1) * cus / tiles < 64 ? (c ? 3 : 1) * cus / tiles : 64);
+            if (splits > ktiles || splits < 1) continue;
+            const int per = (ktiles + splits - 1) / splits;
+            splits = (ktiles + per - 1) / per;
+            const double groups = (double)((tiles * splits + cus - 1) / cus);
+            double us = tile == 64 ? 3.2 + per * 0.31 * (0.5 + 0.5 * groups) : 10. + per * 1.4 * groups;
+            if (splits > 1) us += 3. + splits * slab / (tile == 64 ? 4.5e6 : 7.5e6);
+            if (us < best) { best = us; pl = DwPlan{tile, (M + tile - 1) / tile, (N + tile - 1) / tile, splits, per * BK}; }
+        }
     }
-    const int per = (int)((ktiles + splits - 1) / splits);
-    pl.k_per_split = per * BK;
-    pl.splits = (ktiles + per - 1) / per;
     return pl;
 }
 
@@ -510,10 +527,10 @@ extern "C" int paced_act8_dequantize(const void* q, const void* scale, void* y, 
     return PACED_OK;
 }
 
-extern "C" size_t paced_act8_dweight_workspace_bytes(int T, int M, int N, int accumulate) {
+extern "C" size_t paced_act8_dweight_workspace_bytes(int T, int M, int N) {
     if (T <= 0 || M <= 0 || N <= 0) return 0;
     const DwPlan pl = dw_plan(T, M, N);
-    return pl.splits == 1 && !accumulate ? 0 : (size_t)pl.splits * M * N * 4;
+    return pl.splits == 1 ? 0 : (size_t)pl.splits * M * N * 4;
 }
 
 extern "C" int paced_act8_dweight(const void* dy, int lddy, long long dy_heads, const void* q, const void* scale, float* dw, int lddw,
@@ -534,7 +551,7 @@ extern "C" int paced_act8_dweight(const void* dy, int lddy, long long dy_heads, 
         return PACED_OK;
     }
     const DwPlan pl = dw_plan(T, M, N);
-    const size_t need = paced_act8_dweight_workspace_bytes(T, M, N, accumulate);
+    const size_t need = paced_act8_dweight_workspace_bytes(T, M, N);
     PACED_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                     "paced_act8_dweight: a 16-byte aligned workspace of %zu bytes is needed, got %zu", need, workspace_bytes);
     // offsets inside one slice are 32-bit
@@ -548,6 +565,7 @@ extern "C" int paced_act8_dweight(const void* dy, int lddy, long long dy_heads, 
     p.out = need ? (float*)workspace : dw;
     p.ldout = need ? N : lddw;
     p.slab = (long long)M * N;
+    p.add = !need && accumulate;
     const int total = pl.ntm * pl.ntn * pl.splits;
     if (pl.tile == 256) {
         static PerDeviceOnce once;
@@ -559,7 +577,7 @@ extern "C" int paced_act8_dweight(const void* dy, int lddy, long long dy_heads, 
         }
         const int cus = paced_cu_count();
         hipLaunchKernelGGL(act8_dw_phased_kernel, dim3(total < cus ? total : cus), dim3(512), DP_LDS, s, p, pl.ntm, pl.ntn, total);
-    } else hipLaunchKernelGGL(act8_dw_kernel, dim3(total), dim3(256), DW_NS * DW_STEP, s, p, pl.ntm, pl.ntn, total);
+    } else hipLaunchKernelGGL(act8_dw_kernel, dim3(total), dim3(512), DW_NS * DW_STEP, s, p, pl.ntm, pl.ntn, total);
     PACED_CHECK_LAUNCH();
     if (need) {
         hipLaunchKernelGGL(slab_sum_kernel, dim3(flat_blocks((long long)M * (N >> 2))), dim3(256), 0, s, p.out, pl.splits, p.slab, dw, lddw, M, N, accumulate);

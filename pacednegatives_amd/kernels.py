@@ -356,7 +356,7 @@ def act8_dweight(dy, q, scale, dw, *, accumulate=True, workspace=None):
         M, heads = dy.shape[1], 0
         lddy = _rows_of(dy, (T, M), BF16, "dy")
     lddw = _rows_of(dw, (M, N), F32, "dw")
-    need = lib.paced_act8_dweight_workspace_bytes(T, M, N, int(bool(accumulate)))
+    need = lib.paced_act8_dweight_workspace_bytes(T, M, N)
     ws = _workspace(workspace, need, dy.device)
     _lib.check(lib.paced_act8_dweight(_p(dy), lddy, heads, _p(q), _p(scale), _p(dw), lddw, T, M, N, int(bool(accumulate)), _p(ws), need,
                                       _stream()), "paced_act8_dweight")

@@ -150,6 +150,19 @@ def test_weight_gradient_exact_at_sizes_that_take_large_tiles(T, M, N):
     assert torch.equal(dw, want)
 
 
+@pytest.mark.parametrize("T,M,N", [(600, 4096, 4096), (9000, 2312, 784), (40000, 768, 768)])
+def test_weight_gradient_of_256_tiles_is_written_and_added_to(T, M, N):
+    """(one slice, which writes or adds itself; edges inside a tile; many slices)"""
+    dy, x, dyd, q, scale = whole(T, M, N, T + M)
+    want = (dy.cuda().t() @ x.cuda()).float()
+    dw = torch.full((M + 1, N), float("nan"), device="cuda")
+    dw[M] = 5
+    K.act8_dweight(dyd, q, scale, dw[:M], accumulate=False)
+    assert torch.equal(dw[:M], want) and (dw[M] == 5).all()
+    K.act8_dweight(dyd, q, scale, dw[:M])
+    assert torch.equal(dw[:M], 2 * want) and (dw[M] == 5).all()
+
+
 @pytest.mark.parametrize("T", [65, 1000])
 @pytest.mark.parametrize("H,N", [(1, 64), (3, 80), (12, 768)])
 def test_weight_gradient_of_head_major_and_strided_dy(T, H, N):

@@ -60,7 +60,7 @@ def test_calls_on_several_streams_at_once():
 def test_workspaces_of_the_callers():
     """A workspace that is large enough is used up to the size asked for and not beyond; a smaller one is not used at all."""
     lib = _lib.load()
-    R, V, d, T = 300, 1000, 128, 500
+    R, V, d, T = 300, 1000, 128, 4000
     h, w, gl = (rn(1, R, d) * 0.1).to(BF16), rn(2, V, d).to(BF16), rn(3, R).abs()
     labels = torch.arange(R, device="cuda")
     x, dy, n = rn(4, T, d).to(BF16), rn(5, T, 64).to(BF16), torch.ones(d, device="cuda", dtype=BF16)
@@ -75,7 +75,7 @@ def test_workspaces_of_the_callers():
         K.linear_ce_fwd(h, w, labels, loss, lse, workspace=ws(lib.paced_linear_ce_fwd_workspace_bytes(R, V)))
         K.linear_ce_bwd(h, w, labels, lse, gl, dh, dw, workspace=ws(lib.paced_linear_ce_bwd_workspace_bytes(R, V, d)))
         K.layernorm_bwd(y, x, n, mean, rstd, dx, dw=dn, workspace=ws(lib.paced_layernorm_workspace_bytes(T, d)))
-        K.act8_dweight(dy, q, s, dw8, accumulate=False, workspace=ws(lib.paced_act8_dweight_workspace_bytes(T, 64, d, 0)))
+        K.act8_dweight(dy, q, s, dw8, accumulate=False, workspace=ws(lib.paced_act8_dweight_workspace_bytes(T, 64, d)))
         return [t.clone() for t in (loss, lse, dh, dw, dx, dn, dw8)]
     want = calls(lambda need: None)
     given = []
