@@ -1445,7 +1445,7 @@ int launch(const GemmParams& p, int splits, hipStream_t stream) {
         if (ktiles >= 3 && ktiles <= 32 && t64 <= 3LL * cu_count()) return launch_cfg<CfgTiny, TA, TB, EPI>(p, 0, stream);
     }
     bool large;
-    if (force_tile == 128) large = false;
+    if (force_tile == 128 || (eff_tile() == 0 && p.tile == 64)) large = false;
     else if (force_tile == 256) large = true;
     else {
         // the 256x256 tile pays off once there is about one tile per CU (split slices count for atomics)

@@ -74,29 +74,46 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const f32x2* __restrict__ 
     if (lse) lse[row] = t + l;
 }
 
-// dh = bf16 of the slabs' sum, slab by slab, and of scale err[r] w[label], the label's entry's share that P's rounding lost
-// (labels NULL: the sum alone)
+// dh = bf16 of the slabs' sum and of scale err[r] w[label], the label's entry's share that P's rounding lost (labels NULL: the
+// sum alone).  G groups of a workgroup's threads add every G-th slab each, group by group in the end: 8 where one thread to
+// eight features leaves compute units without work (128 rows x 768 from 42 slabs:
+// one group 15 us, eight 5), else 1.
+template <int G>
 __global__ void __launch_bounds__(256) ce_dh_kernel(const float* __restrict__ slabs, int count, long long slab, bf16* __restrict__ dh, int lddh, int R, int d,
                                                     const long long* __restrict__ labels, long long ignore, int V, const float* __restrict__ err,
                                                     const bf16* __restrict__ w, int ldw, float scale) {
-    const int d8 = d >> 3;
+    constexpr int L = 256 / G;
+    __shared__ f32x4 sh[G > 1 ? 2 * 256 : 1];
+    const int d8 = d >> 3, group = threadIdx.x / L, l = threadIdx.x % L;
     const long long total = (long long)R * d8;
-    for (long long id = (long long)blockIdx.x * 256 + threadIdx.x; id < total; id += (long long)gridDim.x * 256) {
+    for (long long id0 = (long long)blockIdx.x * L; id0 < total; id0 += (long long)gridDim.x * L) {
+        const long long id = id0 + l < total ? id0 + l : total - 1;
+        const bool ok = id0 + l < total && group == 0;
         const int r = (int)(id / d8), c = (int)(id - (long long)r * d8);
         f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
         bf16x8 x = {};
         float e = 0.f;
-        if (labels) {                                        // requested ahead of the slabs, added after them
+        if (ok && labels) {                                  // requested ahead of the slabs, added after them
             const long long label = labels[r];
             if (label != ignore && label >= 0 && label < V) {
                 x = *reinterpret_cast<const bf16x8*>(w + (size_t)label * ldw + c * 8);
                 e = scale * err[r];
             }
         }
-        for (int k = 0; k < count; ++k) {
+        for (int k = group; k < count; k += G) {
             const float* src = slabs + (size_t)k * slab + (size_t)r * d + c * 8;
             a += *reinterpret_cast<const f32x4*>(src);
             b += *reinterpret_cast<const f32x4*>(src + 4);
+        }
+        if (G > 1) {
+            sh[threadIdx.x] = a;
+            sh[256 + threadIdx.x] = b;
+            __syncthreads();
+            if (group == 0) {
+#pragma unroll
+                for (int k = 1; k < G; ++k) { a += sh[k * L + l]; b += sh[256 + k * L + l]; }
+            }
+            __syncthreads();                                 // the next round writes the sums again
         }
         if (e != 0.f) {
 #pragma unroll
@@ -105,7 +122,7 @@ __global__ void __launch_bounds__(256) ce_dh_kernel(const float* __restrict__ sl
         bf16x8 o;
 #pragma unroll
         for (int j = 0; j < 4; ++j) { o[j] = f2bf(a[j]); o[4 + j] = f2bf(b[j]); }
-        *reinterpret_cast<bf16x8*>(dh + (size_t)r * lddh + c * 8) = o;
+        if (ok) *reinterpret_cast<bf16x8*>(dh + (size_t)r * lddh + c * 8) = o;
     }
 }
 
@@ -178,13 +195,22 @@ int blocks_for(long long items) {
 
 size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// Microseconds of a product of M x N tiles of edge `tile` over `steps` K steps of 64, from what the kernels of gemm.hip reach:
-// a 256x256 step 1.75 (1.2 PFLOP/s over the chip) and 8 to fill and drain a tile's ring; 128x128 and 64x64 tiles run three to a
-// compute unit and give it a step in 0.75 and 0.3.  Good to about a fifth: it only chooses between tiles and slices.
+// Microseconds of a product of M x N in tiles of edge `tile`, `steps` K steps of 64 cut into `slices`, as fitted to 650 launches
+// of gemm.hip's kernels at 40 sizes (off by 4 to 10 % in the mean): a launch, and for every round of the chip's compute units
+// the K steps and what a tile costs beside them.  Kernels as launch_cfg chooses them: rings for one and two 128x128 tiles and
+// up to three 64x64 tiles a compute unit, several workgroups with one buffer beyond.
 double product_us(int tile, int M, int N, int slices, int steps) {
     const long long items = (long long)((M + tile - 1) / tile) * ((N + tile - 1) / tile) * slices, cus = paced_cu_count();
-    const double rounds = (double)((items + cus - 1) / cus), per = (double)((steps + slices - 1) / slices);
-    return tile == 256 ? rounds * (per * 1.75 + 8.) : tile == 128 ? rounds * per * 0.75 + 6. : rounds * per * 0.3 + 6.;
+    const double rounds = (double)((items + cus - 1) / cus), load = (double)items / (double)cus, per = (double)((steps + slices - 1) / slices);
+    const bool ring = per >= 3.;
+    if (tile == 256) return 2.3 + rounds * (per * (1.35 + 0.3 * (load < 1. ? load : 1.)) + 5.7);
+    if (tile == 128) {
+        if (ring && items <= cus) return 5.5 + per * (0.55 + 0.14 * load);
+        if (ring && items <= 2 * cus) return 5.0 + per * (0.51 + 0.245 * load);
+        return 4.4 + rounds * (per * 0.65 + 2.3);
+    }
+    if (ring && items <= 3 * cus) return 5.0 + per * (items <= cus ? 0.33 : items <= 2 * cus ? 0.375 : 0.57);
+    return 5.0 + (load < 1. ? 1. : load) * (per * 0.2 + 0.4);
 }
 int best_tile(int M, int N, int steps) {
     double best = 1e30;
@@ -198,23 +224,26 @@ int best_tile(int M, int N, int steps) {
 }
 
 // Tile and slices of dh's product over a piece: more slices give it more workgroups and its second kernel more slabs to add
-// (written and read at about 4 TB/s).
+// (written and read at about 7 TB/s).  Of 13 sizes measured with 6 to 18 plans each the best is chosen at 10, one 2 to 10 %
+// behind at three.  1088 x 768 from 32128: 9 slices of 128x128 tiles 67 us, 17 of 256x256 68, 14 of 128x128 (three
+// workgroups a compute unit) 99; 512 x 768 from 8704: 5 of 64x64 19, 8 of 128x128 22, 32 of 256x256 30.
 double dh_us(int R, int d, int steps, int* tile, int* slices) {
     double best = 1e30;
     for (int t = 256; t >= 64; t /= 2) {
         if (t == 256 && (R < 256 || d < 256)) continue;
         for (int s = 1; s <= 64 && s * 3 <= steps + 2; ++s) {
-            const double us = product_us(t, R, d, s, steps) + (double)s * R * d * 8. / 4e6;
+            const double us = product_us(t, R, d, s, steps) + (double)s * R * d * 8. / 7e6;
             if (us < best) { best = us; *slices = s; *tile = t; }
-            if (t != 64 && (long long)((R + t - 1) / t) * ((d + t - 1) / t) * s > 4ll * paced_cu_count()) break;
+            if ((long long)((R + t - 1) / t) * ((d + t - 1) / t) * s > 4ll * paced_cu_count()) break;
         }
     }
     return best;
 }
 
 // Pieces of the vocabulary: P takes at most 256 MiB (256 columns at least), a piece of the weights 2 GiB (the products address
-// a transposed operand with 32-bit byte offsets).  Where it takes several, sixteen widths between
-// half and all of that are compared by the rounds of tiles that they come to.
+// a transposed operand with 32-bit byte offsets).  Where it takes several, sixteen widths between half and all of that are
+// compared by their estimated times; a narrower one has to gain 3 % (8192 rows x 32128 x 768: 64 tiles 1234 us, 42 tiles, on a
+// par by the estimate, 1270).
 struct CePlan { int piece, ldp, slabs, dh_tile; };
 CePlan ce_plan(int R, int V, int d) {
     CePlan pl;
@@ -237,7 +266,7 @@ CePlan ce_plan(int R, int V, int d) {
                 us += (part ? 1 : full) * (product_us(best_tile(R, n, d / 64), R, n, 1, d / 64) + dh_us(R, d, (n + 63) / 64, &tile, &slices) +
                                            product_us(best_tile(n, d, k), n, d, 1, k));
             }
-            if (us < best) { best = us; piece = c * 256; }
+            if (us < best * 0.97) { best = us; piece = c * 256; }
         }
     }
     pl.piece = (int)piece;
@@ -264,9 +293,7 @@ GemmParams product(const void* A, int lda, const void* B, int ldb, void* C, int 
 // 4).  Up to 64 rows 64x64 tiles read the weights fastest (16 rows: 16.6 us against 18.4 with 128x128).
 int ce_logits(GemmParams p, int epilogue, hipStream_t s) {
     const int steps = (p.K + 63) / 64, R = p.M, full = R / 256 * 256;
-    if (R <= 64) p.tile = 64;
-    else p.tile = best_tile(R, p.N, steps);
-    if (p.tile < 128 && R > 64) p.tile = 128;
+    p.tile = R <= FEW ? 64 : best_tile(R, p.N, steps);
     if (full > 0 && full < R && p.N >= 256) {
         const double split = product_us(256, full, p.N, 1, steps) + product_us(128, R - full, p.N, 1, steps);
         if (split < product_us(p.tile, R, p.N, 1, steps)) {
@@ -344,7 +371,7 @@ extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ld
     PACED_CHECK_ARG(!dw || (lddw >= d && lddw % 8 == 0 && ((uintptr_t)dw & 15) == 0), "paced_linear_ce_bwd: dw needs 16-byte aligned rows, a stride of at least d and a multiple of 8 (lddw=%d)", lddw);
     if (R == 0) {                                     // no row: dw's sum is empty
         if (!dw || dw_f32) return PACED_OK;
-        hipLaunchKernelGGL(ce_dh_kernel, dim3(blocks_for((long long)V * (d >> 3))), dim3(256), 0, s, nullptr, 0, 0LL, (bf16*)dw, lddw, V, d,
+        hipLaunchKernelGGL(ce_dh_kernel<1>, dim3(blocks_for((long long)V * (d >> 3))), dim3(256), 0, s, nullptr, 0, 0LL, (bf16*)dw, lddw, V, d,
                            nullptr, 0LL, 0, nullptr, nullptr, 0, 0.f);
         PACED_CHECK_LAUNCH();
         return PACED_OK;
@@ -393,8 +420,13 @@ extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ld
         }
     }
     if (dh) {
-        hipLaunchKernelGGL(ce_dh_kernel, dim3(blocks_for((long long)R * (d >> 3))), dim3(256), 0, s, slabs, pl.slabs, (long long)R * d, (bf16*)dh, lddh, R, d,
-                           labels, ignore_index, V, err, (const bf16*)w, ldw, scale);
+        const long long pieces = (long long)R * (d >> 3);
+        if (pieces < 256LL * paced_cu_count())
+            hipLaunchKernelGGL(ce_dh_kernel<8>, dim3(blocks_for(pieces * 8)), dim3(256), 0, s, slabs, pl.slabs, (long long)R * d, (bf16*)dh, lddh, R, d,
+                               labels, ignore_index, V, err, (const bf16*)w, ldw, scale);
+        else
+            hipLaunchKernelGGL(ce_dh_kernel<1>, dim3(blocks_for(pieces)), dim3(256), 0, s, slabs, pl.slabs, (long long)R * d, (bf16*)dh, lddh, R, d,
+                               labels, ignore_index, V, err, (const bf16*)w, ldw, scale);
         PACED_CHECK_LAUNCH();
     }
     return PACED_OK;
