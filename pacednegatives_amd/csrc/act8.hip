@@ -551,7 +551,7 @@ extern "C" int paced_act8_dweight(const void* dy, int lddy, long long dy_heads, 
         return PACED_OK;
     }
     const DwPlan pl = dw_plan(T, M, N);
-    const size_t need = paced_act8_dweight_workspace_bytes(T, M, N);
+    const size_t need = pl.splits == 1 ? 0 : (size_t)pl.splits * M * N * 4;
     PACED_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                     "paced_act8_dweight: a 16-byte aligned workspace of %zu bytes is needed, got %zu", need, workspace_bytes);
     // offsets inside one slice are 32-bit

@@ -198,10 +198,11 @@ size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
 // Microseconds of a product of M x N in tiles of edge `tile`, `steps` K steps of 64 cut into `slices`, as fitted to 650 launches
 // of gemm.hip's kernels at 40 sizes (off by 4 to 10 % in the mean): a launch, and for every round of the chip's compute units
 // the K steps and what a tile costs beside them.  Kernels as launch_cfg chooses them: rings for one and two 128x128 tiles and
-// up to three 64x64 tiles a compute unit, several workgroups with one buffer beyond.
-double product_us(int tile, int M, int N, int slices, int steps) {
-    const long long items = (long long)((M + tile - 1) / tile) * ((N + tile - 1) / tile) * slices, cus = paced_cu_count();
-    const double rounds = (double)((items + cus - 1) / cus), load = (double)items / (double)cus, per = (double)((steps + slices - 1) / slices);
+// up to three 64x64 tiles a compute unit, several workgroups with one buffer beyond.  (A plan asks it
+// some hundred times: 2 us, 9 for several pieces.)
+long long tiles_of(int tile, int M, int N) { return (long long)((M + tile - 1) / tile) * ((N + tile - 1) / tile); }
+double product_us(int tile, long long items, int slices, int steps, int cus) {
+    const double rounds = (double)((items + cus - 1) / cus), load = (double)items / cus, per = (double)((steps + slices - 1) / slices);
     const bool ring = per >= 3.;
     if (tile == 256) return 2.3 + rounds * (per * (1.35 + 0.3 * (load < 1. ? load : 1.)) + 5.7);
     if (tile == 128) {
@@ -212,12 +213,13 @@ double product_us(int tile, int M, int N, int slices, int steps) {
     if (ring && items <= 3 * cus) return 5.0 + per * (items <= cus ? 0.33 : items <= 2 * cus ? 0.375 : 0.57);
     return 5.0 + (load < 1. ? 1. : load) * (per * 0.2 + 0.4);
 }
-int best_tile(int M, int N, int steps) {
+double tile_us(int tile, int M, int N, int steps, int cus) { return product_us(tile, tiles_of(tile, M, N), 1, steps, cus); }
+int best_tile(int M, int N, int steps, int cus) {
     double best = 1e30;
     int tile = 64;
     for (int t = 256; t >= 64; t /= 2) {
         if (t == 256 && (M < 256 || N < 256)) continue;
-        const double us = product_us(t, M, N, 1, steps);
+        const double us = tile_us(t, M, N, steps, cus);
         if (us < best) { best = us; tile = t; }
     }
     return tile;
@@ -227,14 +229,15 @@ int best_tile(int M, int N, int steps) {
 // (written and read at about 7 TB/s).  Of 13 sizes measured with 6 to 18 plans each the best is chosen at 10, one 2 to 10 %
 // behind at three.  1088 x 768 from 32128: 9 slices of 128x128 tiles 67 us, 17 of 256x256 68, 14 of 128x128 (three
 // workgroups a compute unit) 99; 512 x 768 from 8704: 5 of 64x64 19, 8 of 128x128 22, 32 of 256x256 30.
-double dh_us(int R, int d, int steps, int* tile, int* slices) {
+double dh_us(int R, int d, int steps, int* tile, int* slices, int cus) {
     double best = 1e30;
     for (int t = 256; t >= 64; t /= 2) {
         if (t == 256 && (R < 256 || d < 256)) continue;
+        const long long tiles = tiles_of(t, R, d);
         for (int s = 1; s <= 64 && s * 3 <= steps + 2; ++s) {
-            const double us = product_us(t, R, d, s, steps) + (double)s * R * d * 8. / 7e6;
+            const double us = product_us(t, tiles * s, s, steps, cus) + (double)s * R * d * 8. / 7e6;
             if (us < best) { best = us; *slices = s; *tile = t; }
-            if ((long long)((R + t - 1) / t) * ((d + t - 1) / t) * s > 4ll * paced_cu_count()) break;
+            if (tiles * s > 4ll * cus) break;
         }
     }
     return best;
@@ -246,6 +249,7 @@ double dh_us(int R, int d, int steps, int* tile, int* slices) {
 // par by the estimate, 1270).
 struct CePlan { int piece, ldp, slabs, dh_tile; };
 CePlan ce_plan(int R, int V, int d) {
+    const int cus = paced_cu_count();
     CePlan pl;
     long long fit = (256ll << 20) / 2 / (R > 0 ? R : 1) / 256;       // in tiles of 256 columns
     const long long reach = (1ll << 30) / d / 256;
@@ -263,8 +267,8 @@ CePlan ce_plan(int R, int V, int d) {
                 const int n = part ? rest : (int)c * 256;
                 if (n == 0 || (!part && !full)) continue;
                 int tile = 64, slices = 1;
-                us += (part ? 1 : full) * (product_us(best_tile(R, n, d / 64), R, n, 1, d / 64) + dh_us(R, d, (n + 63) / 64, &tile, &slices) +
-                                           product_us(best_tile(n, d, k), n, d, 1, k));
+                us += (part ? 1 : full) * (tile_us(best_tile(R, n, d / 64, cus), R, n, d / 64, cus) + dh_us(R, d, (n + 63) / 64, &tile, &slices, cus) +
+                                           tile_us(best_tile(n, d, k, cus), n, d, k, cus));
             }
             if (us < best * 0.97) { best = us; piece = c * 256; }
         }
@@ -274,7 +278,7 @@ CePlan ce_plan(int R, int V, int d) {
     const int steps = (pl.piece + 63) / 64;
     pl.slabs = 1;
     pl.dh_tile = 64;
-    dh_us(R, d, steps, &pl.dh_tile, &pl.slabs);
+    dh_us(R, d, steps, &pl.dh_tile, &pl.slabs, cus);
     const int per = (steps + pl.slabs - 1) / pl.slabs;
     pl.slabs = (steps + per - 1) / per;
     return pl;
@@ -292,11 +296,11 @@ GemmParams product(const void* A, int lda, const void* B, int ldb, void* C, int 
 // the rest in 128x128 tiles where that saves a round of tiles (1088 rows x 32128 entries: 3 rounds for 4.25 tiles of rows, 2 for
 // 4).  Up to 64 rows 64x64 tiles read the weights fastest (16 rows: 16.6 us against 18.4 with 128x128).
 int ce_logits(GemmParams p, int epilogue, hipStream_t s) {
-    const int steps = (p.K + 63) / 64, R = p.M, full = R / 256 * 256;
-    p.tile = R <= FEW ? 64 : best_tile(R, p.N, steps);
+    const int steps = (p.K + 63) / 64, R = p.M, full = R / 256 * 256, cus = paced_cu_count();
+    p.tile = R <= FEW ? 64 : best_tile(R, p.N, steps, cus);
     if (full > 0 && full < R && p.N >= 256) {
-        const double split = product_us(256, full, p.N, 1, steps) + product_us(128, R - full, p.N, 1, steps);
-        if (split < product_us(p.tile, R, p.N, 1, steps)) {
+        const double split = tile_us(256, full, p.N, steps, cus) + tile_us(128, R - full, p.N, steps, cus);
+        if (split < tile_us(p.tile, R, p.N, steps, cus)) {
             GemmParams rest = p;
             p.M = full;
             p.tile = 256;
@@ -356,10 +360,14 @@ extern "C" int paced_linear_ce_fwd(const void* h, int ldh, const void* w, int ld
     return PACED_OK;
 }
 
-extern "C" size_t paced_linear_ce_bwd_workspace_bytes(int R, int V, int d) {
-    if (R <= 0 || V <= 0 || d <= 0) return 0;
-    const CePlan pl = ce_plan(R, V, d);
+namespace {
+size_t ce_workspace(const CePlan& pl, int R, int d) {
     return (R <= FEW ? 2 : 1) * round256((size_t)R * pl.ldp * 2) + round256((size_t)R * 4) + (size_t)pl.slabs * R * d * 4;
+}
+}  // namespace
+
+extern "C" size_t paced_linear_ce_bwd_workspace_bytes(int R, int V, int d) {
+    return R <= 0 || V <= 0 || d <= 0 ? 0 : ce_workspace(ce_plan(R, V, d), R, d);
 }
 
 extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ldw, const long long* labels, const float* lse, const float* gloss,
@@ -379,7 +387,7 @@ extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ld
     PACED_CHECK_ARG(lse && gloss, "paced_linear_ce_bwd: null operand");
     PACED_CHECK_ARG(!dh || (lddh >= d && lddh % 8 == 0 && ((uintptr_t)dh & 15) == 0), "paced_linear_ce_bwd: dh needs 16-byte aligned rows, a stride of at least d and a multiple of 8 (lddh=%d)", lddh);
     const CePlan pl = ce_plan(R, V, d);
-    const size_t need = paced_linear_ce_bwd_workspace_bytes(R, V, d);
+    const size_t need = ce_workspace(pl, R, d);
     PACED_CHECK_ARG(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
                     "paced_linear_ce_bwd: a 16-byte aligned workspace of %zu bytes is needed, got %zu", need, workspace_bytes);
     // a transposed operand is addressed with 32-bit byte offsets from its first row
@@ -415,7 +423,7 @@ extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ld
         } else if (dw) {
             p = product(P, pl.ldp, h, ldh, dw_f32 ? (void*)((float*)dw + (size_t)v0 * lddw) : (void*)((bf16*)dw + (size_t)v0 * lddw), lddw, n, d, R, scale);
             p.accumulate = 1;
-            p.tile = best_tile(n, d, (R + 63) / 64);
+            p.tile = best_tile(n, d, (R + 63) / 64, paced_cu_count());
             if ((r = paced_gemm_launch(p, true, true, dw_f32 ? EPI_SLAB_F32 : EPI_BF16, 1, s)) != PACED_OK) return r;
         }
     }
