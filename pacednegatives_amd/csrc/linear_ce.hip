@@ -225,6 +225,15 @@ int best_tile(int M, int N, int steps, int cus) {
     return tile;
 }
 
+// what a product in two launches takes beside them (32128 x 768 from 300 rows: by the launches alone 26 us against 30 for one,
+// measured 32 against 28)
+constexpr double TWO_LAUNCHES = 6.;
+// of M x N 256x256 tiles, the rows that fill whole rounds of the compute units
+int whole_rounds(int M, int N, int cus) {
+    const int wide = (N + 255) / 256, a_round = cus / wide;
+    return a_round ? M / 256 / a_round * a_round * 256 : 0;
+}
+
 // Tile and slices of dh's product over a piece: more slices give it more workgroups and its second kernel more slabs to add
 // (written and read at about 7 TB/s).  Of 13 sizes measured with 6 to 18 plans each the best is chosen at 10, one 2 to 10 %
 // behind at three.  1088 x 768 from 32128: 9 slices of 128x128 tiles 67 us, 17 of 256x256 68, 14 of 128x128 (three
@@ -247,6 +256,7 @@ double dh_us(int R, int d, int steps, int* tile, int* slices, int cus) {
 // a transposed operand with 32-bit byte offsets).  Where it takes several, sixteen widths between half and all of that are
 // compared by their estimated times; a narrower one has to gain 3 % (8192 rows x 32128 x 768: 64 tiles 1234 us, 42 tiles, on a
 // par by the estimate, 1270).
+double dw_us(int n, int d, int steps, int cus, int* rows);
 struct CePlan { int piece, ldp, slabs, dh_tile; };
 CePlan ce_plan(int R, int V, int d) {
     const int cus = paced_cu_count();
@@ -266,9 +276,9 @@ CePlan ce_plan(int R, int V, int d) {
             for (int part = 0; part < 2; ++part) {
                 const int n = part ? rest : (int)c * 256;
                 if (n == 0 || (!part && !full)) continue;
-                int tile = 64, slices = 1;
+                int tile = 64, slices = 1, rows;
                 us += (part ? 1 : full) * (tile_us(best_tile(R, n, d / 64, cus), R, n, d / 64, cus) + dh_us(R, d, (n + 63) / 64, &tile, &slices, cus) +
-                                           tile_us(best_tile(n, d, k, cus), n, d, k, cus));
+                                           dw_us(n, d, k, cus, &rows));
             }
             if (us < best * 0.97) { best = us; piece = c * 256; }
         }
@@ -292,30 +302,74 @@ GemmParams product(const void* A, int lda, const void* B, int ldb, void* C, int 
     return p;
 }
 
-// One product of the logits (EPI_CE_STATS or EPI_CE_GRAD) of all rows: in one launch, or the rows that fill 256x256 tiles and
-// the rest in 128x128 tiles where that saves a round of tiles (1088 rows x 32128 entries: 3 rounds for 4.25 tiles of rows, 2 for
-// 4).  Up to 64 rows 64x64 tiles read the weights fastest (16 rows: 16.6 us against 18.4 with 128x128).
+// One product of the logits (EPI_CE_STATS or EPI_CE_GRAD): in one launch, or in two, 256x256 tiles and what they leave over in
+// 128x128 tiles, where that saves a round: the rows that fill tiles and the rest (1088 rows x 32128 entries: 3 rounds for 4.25
+// tiles of rows, 2 for 4), or the columns that fill whole rounds and the rest (1000 x 50001: 3.06 rounds).  Both launches leave
+// statistics of 64 columns.  Up to 64 rows 64x64 tiles read the weights fastest (16 rows: 16.6 us against 18.4 with 128x128).
 int ce_logits(GemmParams p, int epilogue, hipStream_t s) {
     const int steps = (p.K + 63) / 64, R = p.M, full = R / 256 * 256, cus = paced_cu_count();
     p.tile = R <= FEW ? 64 : best_tile(R, p.N, steps, cus);
-    if (full > 0 && full < R && p.N >= 256) {
-        const double split = tile_us(256, full, p.N, steps, cus) + tile_us(128, R - full, p.N, steps, cus);
-        if (split < tile_us(p.tile, R, p.N, steps, cus)) {
-            GemmParams rest = p;
-            p.M = full;
-            p.tile = 256;
-            const int rc = paced_gemm_launch(p, false, false, epilogue, 1, s);
-            if (rc != PACED_OK) return rc;
-            rest.M = R - full;
-            rest.tile = 128;
-            rest.A += (size_t)full * p.lda;
-            rest.ce_labels += full;
-            if (epilogue == EPI_CE_STATS) { rest.ce_part += full; rest.ce_target += full; }
-            else { rest.ce_lse += full; rest.ce_g += full; rest.ce_err += full; rest.C = (bf16*)rest.C + (size_t)full * p.ldc; }
-            return paced_gemm_launch(rest, false, false, epilogue, 1, s);
+    GemmParams rest = p;
+    double best = tile_us(p.tile, R, p.N, steps, cus);
+    int rows = 0, cols = 0;                                      // of the first launch (0: one launch)
+    if (full > 0 && p.N >= 256 && !paced_gemm_forced_tile()) {   // (a forced tile may take kernels of both widths of statistics)
+        if (full < R) {
+            const double us = tile_us(256, full, p.N, steps, cus) + tile_us(128, R - full, p.N, steps, cus) + TWO_LAUNCHES;
+            if (us < best) { best = us; rows = full; }
         }
+        const int fill = whole_rounds(p.N, R, cus);
+        if (fill > 0 && fill < p.N && tile_us(256, R, fill, steps, cus) + tile_us(128, R, p.N - fill, steps, cus) + TWO_LAUNCHES < best) { rows = 0; cols = fill; }
     }
-    return paced_gemm_launch(p, false, false, epilogue, 1, s);
+    if (!rows && !cols) return paced_gemm_launch(p, false, false, epilogue, 1, s);
+    p.tile = 256;
+    rest.tile = 128;
+    if (rows) {
+        p.M = rows;
+        rest.M -= rows;
+        rest.A += (size_t)rows * p.lda;
+        rest.ce_labels += rows;
+        if (epilogue == EPI_CE_STATS) { rest.ce_part += rows; rest.ce_target += rows; }
+        else { rest.ce_lse += rows; rest.ce_g += rows; rest.ce_err += rows; rest.C = (bf16*)rest.C + (size_t)rows * p.ldc; }
+    } else {
+        p.N = cols;
+        rest.N -= cols;
+        rest.B += (size_t)cols * p.ldb;
+        rest.ce_first += cols;
+        if (epilogue == EPI_CE_STATS) rest.ce_part += (size_t)(cols / 64) * p.ce_rows;
+        else rest.C = (bf16*)rest.C + cols;
+    }
+    const int rc = paced_gemm_launch(p, false, false, epilogue, 1, s);
+    return rc != PACED_OK ? rc : paced_gemm_launch(rest, false, false, epilogue, 1, s);
+}
+
+// dw's product over a piece, rows of P^T split like the logits' columns (32128 x 768: 378 tiles of 256 in two rounds, or 255 in
+// one and the rest in 128x128 tiles: from 4096 rows 424 us with the logits again, then 405; from 1088 both 133).
+double dw_us(int n, int d, int steps, int cus, int* rows) {
+    const double one = tile_us(best_tile(n, d, steps, cus), n, d, steps, cus);
+    *rows = 0;
+    const int fill = d >= 256 ? whole_rounds(n, d, cus) : 0;
+    if (fill == 0 || fill >= n) return one;
+    const double two = tile_us(256, fill, d, steps, cus) + tile_us(best_tile(n - fill, d, steps, cus), n - fill, d, steps, cus) + TWO_LAUNCHES;
+    if (two >= one) return one;
+    *rows = fill;
+    return two;
+}
+int ce_dw(GemmParams p, int epilogue, size_t element, hipStream_t s) {
+    const int steps = (p.K + 63) / 64, cus = paced_cu_count();
+    int rows;
+    dw_us(p.M, p.N, steps, cus, &rows);
+    if (rows) {
+        GemmParams first = p;
+        first.M = rows;
+        first.tile = 256;
+        const int rc = paced_gemm_launch(first, true, true, epilogue, 1, s);
+        if (rc != PACED_OK) return rc;
+        p.M -= rows;
+        p.A += rows;
+        p.C = (char*)p.C + (size_t)rows * p.ldc * element;
+    }
+    p.tile = best_tile(p.M, p.N, steps, cus);
+    return paced_gemm_launch(p, true, true, epilogue, 1, s);
 }
 
 int ce_check(const char* who, const void* h, int ldh, const void* w, int ldw, const long long* labels, int R, int V, int d) {
@@ -423,8 +477,7 @@ extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ld
         } else if (dw) {
             p = product(P, pl.ldp, h, ldh, dw_f32 ? (void*)((float*)dw + (size_t)v0 * lddw) : (void*)((bf16*)dw + (size_t)v0 * lddw), lddw, n, d, R, scale);
             p.accumulate = 1;
-            p.tile = best_tile(n, d, (R + 63) / 64, paced_cu_count());
-            if ((r = paced_gemm_launch(p, true, true, dw_f32 ? EPI_SLAB_F32 : EPI_BF16, 1, s)) != PACED_OK) return r;
+            if ((r = ce_dw(p, dw_f32 ? EPI_SLAB_F32 : EPI_BF16, dw_f32 ? 4 : 2, s)) != PACED_OK) return r;
         }
     }
     if (dh) {

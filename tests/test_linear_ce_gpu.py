@@ -103,6 +103,30 @@ def test_sizes_that_choose_their_own_tiles(R, V, d):
     assert all(torch.equal(a, b) for a, b in zip((loss, lse, dh, dw), again))
 
 
+@pytest.mark.parametrize("R,V,d,f32", [(1000, 17001, 512, False), (600, 33000, 512, False), (1500, 33000, 768, True), (1088, 32128, 256, False)])
+def test_products_in_two_launches(R, V, d, f32):
+    """(columns or rows that fill whole rounds of tiles, and the rest)"""
+    h, w, labels, gl = make(R, V, d, 12)
+    labels[:5] = torch.tensor([V - 1, V - 2, 16383, 16384, 32], device="cuda")
+    o = oracle(h, w, labels, gl, 1.0)
+    loss, lse, dh, dw = run(h, w, labels, gl, f32=f32)
+    check_loss(o, loss, lse)
+    check_grads(o, dh, dw, torch.full_like(dw, 0.25) if f32 else None)
+
+
+@pytest.mark.parametrize("size", [64, 128, 256])
+def test_a_forced_tile_where_both_widths_of_statistics_could_meet(size):
+    K.gemm_set_tile(size)
+    try:
+        h, w, labels, gl = make(1100, 13000, 64, 13)
+        o = oracle(h, w, labels, gl, 1.0)
+        loss, lse, dh, dw = run(h, w, labels, gl)
+    finally:
+        K.gemm_set_tile(0)
+    check_loss(o, loss, lse)
+    check_grads(o, dh, dw)
+
+
 @pytest.mark.parametrize("R,V", [(2816, 2900), (4300, 2561), (2561, 5000)])
 def test_more_than_eight_tiles_each_way(R, V):
     """(11 x 12, 17 x 11 and 11 x 20 tiles of 256: bands of unequal width, the last one of a tile's single row or column)"""
