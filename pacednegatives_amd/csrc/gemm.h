@@ -20,44 +20,45 @@ enum Epi : int {
     EPI_SLAB_F32 = 11    // C(f32) + split * strideC elements (+)= acc * alpha: one owner per element, no atomics
 };
 
+// Every field has a value from the start: a launch reads fields (tile, accumulate, ce_*) that most callers never set.
 struct GemmParams {
-    const bf16* A;
-    const bf16* B;
-    void* C;
-    const bf16* aux;
-    int M, N, K;
-    int lda, ldb, ldc, ldaux;
-    int k_per_split;   // multiple of BK
+    const bf16* A = nullptr;
+    const bf16* B = nullptr;
+    void* C = nullptr;
+    const bf16* aux = nullptr;
+    int M = 0, N = 0, K = 0;
+    int lda = 0, ldb = 0, ldc = 0, ldaux = 0;
+    int k_per_split = 0;   // multiple of BK
     // Head-major operands (> 0: elements between heads; the operand's leading dimension is then 64): the operand's feature
     // columns [64h, 64h + 64) are the contiguous [rows, 64] matrix at base + h * stride instead of a column block of rows of
     // ld elements.  A: features = K (not transposed) or M (transposed); B: transposed only, features = N; C: plain bf16
     // epilogue only, features = N.
-    long long a_heads, b_heads, c_heads;
-    int batch;         // independent problems of the same shape; operand b starts strideX * b elements after operand 0
-    long long strideA, strideB, strideC;
-    float alpha;       // scales acc before the epilogue
-    float mask_scale;
-    DropCfg drop;
-    int drop_narrow;   // the output has at most 2^34 elements: dropout's quad numbers fit 32 bits
+    long long a_heads = 0, b_heads = 0, c_heads = 0;
+    int batch = 1;         // independent problems of the same shape; operand b starts strideX * b elements after operand 0
+    long long strideA = 0, strideB = 0, strideC = 0;
+    float alpha = 1.f;     // scales acc before the epilogue
+    float mask_scale = 1.f;
+    DropCfg drop = {};
+    int drop_narrow = 0;   // the output has at most 2^34 elements: dropout's quad numbers fit 32 bits
     // pool scorer only
-    unsigned long long* tk_cand;
-    unsigned int* tk_cnt;
-    const float* tk_thr;
-    int tk_cap;
-    unsigned int tk_row_base;
+    unsigned long long* tk_cand = nullptr;
+    unsigned int* tk_cnt = nullptr;
+    const float* tk_thr = nullptr;
+    int tk_cap = 0;
+    unsigned int tk_row_base = 0;
     // linear-head cross entropy only
-    const long long* ce_labels;   // [M]; a label counts when it is not ce_ignore and lies in [0, ce_vocab)
-    const float* ce_lse;          // [M]
-    const float* ce_g;            // [M]
-    float* ce_err;                // [M] EPI_CE_GRAD: what the label's entry lost in its rounding (rows with a label among the columns)
-    bf16* ce_lo;                  // EPI_CE_GRAD, small tiles: what every entry lost, in bf16, laid out as C (NULL: not wanted)
-    f32x2* ce_part;
-    float* ce_target;
-    long long ce_ignore;
-    int ce_vocab, ce_first;       // vocabulary size, entry of column 0
-    int ce_rows;                  // rows of part (a launch may cover some of them)
-    int accumulate;               // EPI_SLAB_F32: add to what is there
-    int tile;                     // tile edge the caller has chosen (0: the launch's own rule; paced_gemm_set_tile overrides)
+    const long long* ce_labels = nullptr;   // [M]; a label counts when it is not ce_ignore and lies in [0, ce_vocab)
+    const float* ce_lse = nullptr;          // [M]
+    const float* ce_g = nullptr;            // [M]
+    float* ce_err = nullptr;                // [M] EPI_CE_GRAD: what the label's entry lost in its rounding (rows with a label among the columns)
+    bf16* ce_lo = nullptr;                  // EPI_CE_GRAD, small tiles: what every entry lost, in bf16, laid out as C (NULL: not wanted)
+    f32x2* ce_part = nullptr;
+    float* ce_target = nullptr;
+    long long ce_ignore = 0;
+    int ce_vocab = 0, ce_first = 0;         // vocabulary size, entry of column 0
+    int ce_rows = 0;                        // rows of part (a launch may cover some of them)
+    int accumulate = 0;                     // EPI_SLAB_F32: add to what is there
+    int tile = 0;                           // tile edge the caller has chosen (0: the launch's own rule; paced_gemm_set_tile overrides)
 };
 
 // Order-preserving 64-bit key: larger key <=> (higher score, then lower pool row).

@@ -1607,14 +1607,13 @@ static int gemm_entry(const void* A, const void* B, void* C, const void* aux,
     PACED_CHECK_ARG(splits <= 1 || epilogue == EPI_ATOMIC_F32, "paced_gemm_bf16: split contraction needs the atomic epilogue");
     if (epilogue != EPI_ATOMIC_F32) splits = 1;
 
-    GemmParams p;
+    GemmParams p = {};
     p.A = (const bf16*)A; p.B = (const bf16*)B; p.C = C; p.aux = (const bf16*)aux;
     p.M = M; p.N = N; p.K = K; p.lda = lda; p.ldb = ldb; p.ldc = ldc; p.ldaux = ldaux;
     p.k_per_split = K; p.a_heads = a_heads; p.b_heads = b_heads; p.c_heads = c_heads;
     p.alpha = alpha; p.mask_scale = mask_scale;
     p.drop = make_drop(drop_p, drop_seed);
     p.drop_narrow = (unsigned long long)M * (unsigned long long)N <= (1ull << 34);
-    p.tk_cand = nullptr; p.tk_cnt = nullptr; p.tk_thr = nullptr; p.tk_cap = 0; p.tk_row_base = 0;
     p.batch = batch; p.strideA = strideA; p.strideB = strideB; p.strideC = strideC;
     return paced_gemm_launch(p, trans_a != 0, trans_b != 0, epilogue, splits, (hipStream_t)stream);
 }
