@@ -287,6 +287,12 @@ size_t paced_linear_ce_bwd_workspace_bytes(int R, int V, int d);
 int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ldw, const long long* labels, const float* lse, const float* gloss,
                         void* dh, int lddh, void* dw, int lddw, int dw_f32, int R, int V, int d, long long ignore_index, float scale,
                         void* workspace, size_t workspace_bytes, void* stream);
+/* paced_linear_ce_bwd with the losses of the forward pass (fp32 [R]; NULL: as paced_linear_ce_bwd).  The label's entry is then
+ * gloss (exp(-loss) - 1) and keeps its relative precision however small the loss; from lse alone it is gloss (exp(z - lse) - 1),
+ * off by about 2^-22 (|lse| + |z|) gloss whatever the loss: 1 % of itself at a loss of 1e-4, all of it below 1e-6. */
+int paced_linear_ce_bwd_ex(const void* h, int ldh, const void* w, int ldw, const long long* labels, const float* loss, const float* lse,
+                           const float* gloss, void* dh, int lddh, void* dw, int lddw, int dw_f32, int R, int V, int d, long long ignore_index,
+                           float scale, void* workspace, size_t workspace_bytes, void* stream);
 /* lceT5.py:119-121 after the caller's view at :134,151: ce[r] = pce[r] + sum|mean nce[r*n..(r+1)*n) */
 int paced_lce_group(const float* pce, const float* nce, float* ce, int R, int n, int use_mean, void* stream);
 /* LCEWeights.forward, lceT5.py:91-99, vectorised, plus the reductions training_step needs (:138-147):

@@ -16,7 +16,7 @@ enum Epi : int {
     // ---- internal to the linear-head cross entropy (linear_ce.hip); rows m are tokens, columns n vocabulary entries
     EPI_CE_STATS = 9,    // part[n / W * ce_rows + m] = (max, sum of 2^(z - max)) of z = acc * alpha * log2 e over W columns but the label's
                          // (W = paced_gemm_stat_width(), 32 or 64); target[m] = the label's acc * alpha
-    EPI_CE_GRAD = 10,    // C(bf16) = g[m] (2^(z - lse[m] log2 e) - [n is m's label]); columns N .. next multiple of 64 are zeros
+    EPI_CE_GRAD = 10,    // C(bf16) = g[m] 2^(z - lse[m] log2 e), the label's g[m] (exp(-loss[m]) - 1); columns N .. next multiple of 64 are zeros
     EPI_SLAB_F32 = 11    // C(f32) + split * strideC elements (+)= acc * alpha: one owner per element, no atomics
 };
 
@@ -50,6 +50,7 @@ struct GemmParams {
     const long long* ce_labels = nullptr;   // [M]; a label counts when it is not ce_ignore and lies in [0, ce_vocab)
     const float* ce_lse = nullptr;          // [M]
     const float* ce_g = nullptr;            // [M]
+    const float* ce_loss = nullptr;         // [M] (NULL: the label's entry is made from ce_lse)
     float* ce_err = nullptr;                // [M] EPI_CE_GRAD: what the label's entry lost in its rounding (rows with a label among the columns)
     bf16* ce_lo = nullptr;                  // EPI_CE_GRAD, small tiles: what every entry lost, in bf16, laid out as C (NULL: not wanted)
     f32x2* ce_part = nullptr;

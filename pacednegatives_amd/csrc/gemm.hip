@@ -44,14 +44,17 @@ __device__ __forceinline__ u32x4 ce_descriptor(const T* rows, int count) {
 #define CE_LABEL(i, row) "buffer_load_dwordx2 %[l" #i "], %[vl], %[rl], 0 offen offset:8*" #row "\n\t"
 #define CE_ROW(i, row)                                                               \
     "buffer_load_dword %[s" #i "], %[vs], %[rs], 0 offen offset:4*" #row "\n\t"      \
-    "buffer_load_dword %[g" #i "], %[vs], %[rg], 0 offen offset:4*" #row "\n\t"
+    "buffer_load_dword %[g" #i "], %[vs], %[rg], 0 offen offset:4*" #row "\n\t"      \
+    "buffer_load_dword %[o" #i "], %[vs], %[ro], 0 offen offset:4*" #row "\n\t"
 #define CE_WAIT "s_waitcnt vmcnt(0) ; hidden-load wait"
 #define CE_L(i) [l##i] "=&v"(v[i])
-#define CE_S(i) [s##i] "=&v"(lse[i]), [g##i] "=&v"(w[i])
+#define CE_S(i) [s##i] "=&v"(lse[i]), [g##i] "=&v"(w[i]), [o##i] "=&v"(loss[i])
 
-// labels of a lane's rows, and with ROWS their log-sum-exps and weights
+// labels of a lane's rows, and with ROWS their log-sum-exps, weights and losses (zeros where the launch has no losses: a
+// descriptor of no bytes)
 template <class Cfg, bool ROWS>
-__device__ __forceinline__ void ce_load(const GemmParams& p, int m0, int wm, int lane, u32x2 (&v)[Cfg::MI], float (&lse)[Cfg::MI], float (&w)[Cfg::MI]) {
+__device__ __forceinline__ void ce_load(const GemmParams& p, int m0, int wm, int lane, u32x2 (&v)[Cfg::MI], float (&lse)[Cfg::MI], float (&w)[Cfg::MI],
+                                        float (&loss)[Cfg::MI]) {
     constexpr int MI = Cfg::MI;
     static_assert(MI == 2 || MI == 4 || MI == 8, "row blocks of a wave");
     static_assert(MI == 8 ? Cfg::moff(0, 3) == 48 && Cfg::moff(0, 4) == 128 && Cfg::moff(0, 7) == 176 : Cfg::moff(0, MI - 1) == 16 * (MI - 1), "the rows in the text below");
@@ -69,18 +72,19 @@ __device__ __forceinline__ void ce_load(const GemmParams& p, int m0, int wm, int
             asm volatile(CE_SETTLE CE_LABEL(0, 0) CE_LABEL(1, 16) CE_WAIT : CE_L(0), CE_L(1) : [vl] "v"(vl), [rl] "s"(rl) : "memory");
     } else {
         const u32x4 rs = ce_descriptor(p.ce_lse + m0, count), rg = ce_descriptor(p.ce_g + m0, count);
+        const u32x4 ro = ce_descriptor(p.ce_loss + m0, p.ce_loss ? count : 0);
         if constexpr (MI == 8)
             asm volatile(CE_SETTLE CE_LABEL(0, 0) CE_LABEL(1, 16) CE_LABEL(2, 32) CE_LABEL(3, 48) CE_LABEL(4, 128) CE_LABEL(5, 144) CE_LABEL(6, 160) CE_LABEL(7, 176)
                          CE_ROW(0, 0) CE_ROW(1, 16) CE_ROW(2, 32) CE_ROW(3, 48) CE_ROW(4, 128) CE_ROW(5, 144) CE_ROW(6, 160) CE_ROW(7, 176) CE_WAIT
                          : CE_L(0), CE_L(1), CE_L(2), CE_L(3), CE_L(4), CE_L(5), CE_L(6), CE_L(7), CE_S(0), CE_S(1), CE_S(2), CE_S(3), CE_S(4), CE_S(5), CE_S(6), CE_S(7)
-                         : [vl] "v"(vl), [vs] "v"(vs), [rl] "s"(rl), [rs] "s"(rs), [rg] "s"(rg) : "memory");
+                         : [vl] "v"(vl), [vs] "v"(vs), [rl] "s"(rl), [rs] "s"(rs), [rg] "s"(rg), [ro] "s"(ro) : "memory");
         else if constexpr (MI == 4)
             asm volatile(CE_SETTLE CE_LABEL(0, 0) CE_LABEL(1, 16) CE_LABEL(2, 32) CE_LABEL(3, 48) CE_ROW(0, 0) CE_ROW(1, 16) CE_ROW(2, 32) CE_ROW(3, 48) CE_WAIT
                          : CE_L(0), CE_L(1), CE_L(2), CE_L(3), CE_S(0), CE_S(1), CE_S(2), CE_S(3)
-                         : [vl] "v"(vl), [vs] "v"(vs), [rl] "s"(rl), [rs] "s"(rs), [rg] "s"(rg) : "memory");
+                         : [vl] "v"(vl), [vs] "v"(vs), [rl] "s"(rl), [rs] "s"(rs), [rg] "s"(rg), [ro] "s"(ro) : "memory");
         else
             asm volatile(CE_SETTLE CE_LABEL(0, 0) CE_LABEL(1, 16) CE_ROW(0, 0) CE_ROW(1, 16) CE_WAIT
-                         : CE_L(0), CE_L(1), CE_S(0), CE_S(1) : [vl] "v"(vl), [vs] "v"(vs), [rl] "s"(rl), [rs] "s"(rs), [rg] "s"(rg) : "memory");
+                         : CE_L(0), CE_L(1), CE_S(0), CE_S(1) : [vl] "v"(vl), [vs] "v"(vs), [rl] "s"(rl), [rs] "s"(rs), [rg] "s"(rg), [ro] "s"(ro) : "memory");
     }
 }
 #undef CE_SETTLE
@@ -91,18 +95,22 @@ __device__ __forceinline__ void ce_load(const GemmParams& p, int m0, int wm, int
 #undef CE_S
 
 // labels of this lane's rows, as columns of the launch (ignored, or of another piece: outside [0, N)), and with ROWS their
-// log-sum-exps (base 2) and weights
+// log-sum-exps (base 2), weights, and label entries where the losses are known: g (exp(-loss) - 1), which keeps the digits of a
+// small loss; g 2^(z - lse) - g has lost them in lse's and the power's rounding
 template <class Cfg, bool ROWS>
 __device__ __forceinline__ void ce_rows(const GemmParams& p, int m0, int wm, int lane, int (&col)[Cfg::MI], bool (&dead)[Cfg::MI],
-                                        float (&lse2)[Cfg::MI], float (&g)[Cfg::MI]) {
+                                        float (&lse2)[Cfg::MI], float (&g)[Cfg::MI], float (&own)[Cfg::MI]) {
     u32x2 v[Cfg::MI];
-    ce_load<Cfg, ROWS>(p, m0, wm, lane, v, lse2, g);
+    ce_load<Cfg, ROWS>(p, m0, wm, lane, v, lse2, g, own);
 #pragma unroll
     for (int i = 0; i < Cfg::MI; ++i) {
         const long long label = (long long)(((unsigned long long)v[i][1] << 32) | v[i][0]);
         dead[i] = label == p.ce_ignore || label < 0 || label >= p.ce_vocab;
         col[i] = dead[i] ? -1 : (int)label - p.ce_first;
-        if (ROWS) lse2[i] *= CE_LOG2E;
+        if (ROWS) {
+            lse2[i] *= CE_LOG2E;
+            if (p.ce_loss) own[i] = g[i] * expm1f(-own[i]);
+        }
     }
 }
 
@@ -116,10 +124,10 @@ __device__ __forceinline__ f32x4 ce_grad4(const f32x4& a, float c, float lse2, f
 // ... and what a block of 16 rows x 64 columns needs where a label is among its columns, a row is ignored (its logits may be
 // anything) or the vocabulary ends in it.  The label's entry, nearly -g for most rows, dominates dh: what its rounding to bf16
 // loses is kept for the kernel that finishes dh.
-__device__ __forceinline__ void ce_mend4(const GemmParams& p, f32x4& v, float g, int col, bool dead, int m, int n) {
+__device__ __forceinline__ void ce_mend4(const GemmParams& p, f32x4& v, float g, float own, int col, bool dead, int m, int n) {
     const int at = col - n;
     if (at >= 0 && at < 4) {
-        const float x = (at == 0 ? v[0] : at == 1 ? v[1] : at == 2 ? v[2] : v[3]) - g;
+        const float x = p.ce_loss ? own : (at == 0 ? v[0] : at == 1 ? v[1] : at == 2 ? v[2] : v[3]) - g;
         if (at == 0) v[0] = x;
         if (at == 1) v[1] = x;
         if (at == 2) v[2] = x;
@@ -382,7 +390,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, void* Cb, int m0, 
         int col[MI];
         bool dead[MI];
         float unused[MI];
-        ce_rows<Cfg, false>(p, m0, wm, lane, col, dead, unused, unused);
+        ce_rows<Cfg, false>(p, m0, wm, lane, col, dead, unused, unused, unused);
         const float c = p.alpha * CE_LOG2E;
         const int nw = n0 + Cfg::noff(wn, 0), nl = (lane >> 4) * 4;        // the wave's first column; this lane's within 16
         if (nw >= p.N) return;
@@ -432,8 +440,8 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, void* Cb, int m0, 
     if (EPI == EPI_CE_GRAD) {
         int col[MI];
         bool dead[MI];
-        float lse2[MI], g[MI];
-        ce_rows<Cfg, true>(p, m0, wm, lane, col, dead, lse2, g);
+        float lse2[MI], g[MI], own[MI];
+        ce_rows<Cfg, true>(p, m0, wm, lane, col, dead, lse2, g, own);
         const float c = p.alpha * CE_LOG2E;
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
@@ -445,7 +453,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, void* Cb, int m0, 
                 const int n = n0 + Cfg::noff(wn, j) + (lane >> 4) * 4;
                 if (n >= ((p.N + 63) & ~63)) continue;
                 f32x4 o = ce_grad4(acc[i][j], c, lse2[i], g[i]);
-                if (special) ce_mend4(p, o, g[i], col[i], dead[i], m, n);
+                if (special) ce_mend4(p, o, g[i], own[i], col[i], dead[i], m, n);
                 const bf16x4 hi = __builtin_convertvector(o, bf16x4);
                 *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16*>(Cb) + (size_t)m * p.ldc + n) = hi;
                 if (p.ce_lo) *reinterpret_cast<bf16x4*>(p.ce_lo + (size_t)m * p.ldc + n) = __builtin_convertvector(o - __builtin_convertvector(hi, f32x4), bf16x4);
@@ -758,8 +766,8 @@ __device__ __forceinline__ void epilogue_rows_impl(const GemmParams& p, void* Cb
     const int roff = rr * 128 + ((c ^ rr) << 4);
     int ccol[8];
     bool cdead[8];
-    float clse[8], cg[8];
-    if (EPI == EPI_CE_GRAD) ce_rows<CfgPhased, true>(p, m0, wr, lane, ccol, cdead, clse, cg);
+    float clse[8], cg[8], cown[8];
+    if (EPI == EPI_CE_GRAD) ce_rows<CfgPhased, true>(p, m0, wr, lane, ccol, cdead, clse, cg, cown);
     const bool has_drop = (EPI == EPI_RES_DROP || EPI == EPI_RELU_DROP) && p.drop.thresh != 0;
     const float scale = (EPI == EPI_MASK || EPI == EPI_MASK_BITS) ? p.alpha * p.mask_scale : p.alpha;
 
@@ -773,7 +781,7 @@ __device__ __forceinline__ void epilogue_rows_impl(const GemmParams& p, void* Cb
             if (EPI == EPI_CE_GRAD) {
                 const int m = m0 + CfgPhased::moff(wr, i) + mw, n = n0 + wc * 64 + j * 16 + g * 4;
                 f32x4 v = ce_grad4(acc[i][j], p.alpha * CE_LOG2E, clse[i], cg[i]);
-                if (special) ce_mend4(p, v, cg[i], ccol[i], cdead[i], m, n);
+                if (special) ce_mend4(p, v, cg[i], cown[i], ccol[i], cdead[i], m, n);
                 o[j] = __builtin_convertvector(v, bf16x4);
                 continue;
             }

@@ -3,7 +3,8 @@
 //   P_rv = g_r (exp(z_rv - lse_r) - [v = label_r])       dh = scale P w      dw = scale P^T h
 // Forward: one product whose epilogue (EPI_CE_STATS in gemm.hip) leaves a maximum and a sum for every row and 64 columns, and
 // a second kernel that joins them; the logits never leave the registers.  The label's term is kept out of the sums, so that
-// a confident row's loss log(1 + sum of the others / its own) keeps its relative precision.
+// a confident row's loss log(1 + sum of the others / its own) keeps its relative precision.  So does its gradient where the
+// backward pass is given the losses: the label's entry is then g (exp(-loss) - 1).
 // Backward: the vocabulary goes by in pieces.  A piece's logits are computed again and leave as P in bf16 (the MFMA operand
 // type; half a step of 2^-8 relative to each entry, as paced_cross_entropy's dlogits), which feeds the two other products.  What
 // the label's entry, the largest of a row, loses in that rounding is given back where dh is finished; up to 64 rows, where
@@ -329,7 +330,7 @@ int ce_logits(GemmParams p, int epilogue, hipStream_t s) {
         rest.A += (size_t)rows * p.lda;
         rest.ce_labels += rows;
         if (epilogue == EPI_CE_STATS) { rest.ce_part += rows; rest.ce_target += rows; }
-        else { rest.ce_lse += rows; rest.ce_g += rows; rest.ce_err += rows; rest.C = (bf16*)rest.C + (size_t)rows * p.ldc; }
+        else { rest.ce_lse += rows; rest.ce_g += rows; rest.ce_err += rows; if (p.ce_loss) rest.ce_loss += rows; rest.C = (bf16*)rest.C + (size_t)rows * p.ldc; }
     } else {
         p.N = cols;
         rest.N -= cols;
@@ -424,9 +425,9 @@ extern "C" size_t paced_linear_ce_bwd_workspace_bytes(int R, int V, int d) {
     return R <= 0 || V <= 0 || d <= 0 ? 0 : ce_workspace(ce_plan(R, V, d), R, d);
 }
 
-extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ldw, const long long* labels, const float* lse, const float* gloss,
-                                   void* dh, int lddh, void* dw, int lddw, int dw_f32, int R, int V, int d, long long ignore_index, float scale,
-                                   void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int paced_linear_ce_bwd_ex(const void* h, int ldh, const void* w, int ldw, const long long* labels, const float* loss, const float* lse,
+                                      const float* gloss, void* dh, int lddh, void* dw, int lddw, int dw_f32, int R, int V, int d,
+                                      long long ignore_index, float scale, void* workspace, size_t workspace_bytes, void* stream) {
     const int rc = ce_check("paced_linear_ce_bwd", h, ldh, w, ldw, labels, R, V, d);
     if (rc != PACED_OK) return rc;
     hipStream_t s = (hipStream_t)stream;
@@ -457,7 +458,7 @@ extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ld
         const int n = V - v0 < pl.piece ? V - v0 : pl.piece;
         const bf16* wp = (const bf16*)w + (size_t)v0 * ldw;
         GemmParams p = product(h, ldh, wp, ldw, P, pl.ldp, R, n, d, scale);
-        p.ce_labels = labels; p.ce_lse = lse; p.ce_g = gloss;
+        p.ce_labels = labels; p.ce_lse = lse; p.ce_g = gloss; p.ce_loss = loss;
         p.ce_ignore = ignore_index; p.ce_vocab = V; p.ce_first = v0;
         p.ce_err = err; p.ce_lo = low;
         int r = ce_logits(p, EPI_CE_GRAD, s);
@@ -491,4 +492,11 @@ extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ld
         PACED_CHECK_LAUNCH();
     }
     return PACED_OK;
+}
+
+extern "C" int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ldw, const long long* labels, const float* lse, const float* gloss,
+                                   void* dh, int lddh, void* dw, int lddw, int dw_f32, int R, int V, int d, long long ignore_index, float scale,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+    return paced_linear_ce_bwd_ex(h, ldh, w, ldw, labels, nullptr, lse, gloss, dh, lddh, dw, lddw, dw_f32, R, V, d, ignore_index, scale,
+                                  workspace, workspace_bytes, stream);
 }

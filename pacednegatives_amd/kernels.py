@@ -578,16 +578,17 @@ def linear_ce_fwd(h, w, labels, loss, lse=None, *, ignore_index=-100, scale=1.0,
     return loss
 
 
-def linear_ce_bwd(h, w, labels, lse, grad_loss, dh=None, dw=None, *, ignore_index=-100, scale=1.0, workspace=None):
+def linear_ce_bwd(h, w, labels, lse, grad_loss, dh=None, dw=None, *, ignore_index=-100, scale=1.0, loss=None, workspace=None):
     """Gradients of sum(grad_loss * loss) of ``linear_ce_fwd``: ``dh`` (bf16 [R, d]) is written, ``dw`` [V, d] is written
-    (bf16) or added to (fp32); either may be left out."""
+    (bf16) or added to (fp32); either may be left out.  ``loss``, the forward pass's losses, keeps the digits of confident
+    rows' gradients (see include/paced_hip.h)."""
     lib = _lib.load()
-    other = _elsewhere(h=h, w=w, labels=labels, lse=lse, grad_loss=grad_loss, dh=dh, dw=dw)
+    other = _elsewhere(h=h, w=w, labels=labels, lse=lse, grad_loss=grad_loss, dh=dh, dw=dw, loss=loss)
     if other is not None:
         with torch.cuda.device(other):
-            return linear_ce_bwd(h, w, labels, lse, grad_loss, dh, dw, ignore_index=ignore_index, scale=scale, workspace=workspace)
+            return linear_ce_bwd(h, w, labels, lse, grad_loss, dh, dw, ignore_index=ignore_index, scale=scale, loss=loss, workspace=workspace)
     R, V, d, ldh, ldw = _head_operands(h, w, labels)
-    _flat(lse, R, F32, "lse"); _flat(grad_loss, R, F32, "grad_loss")
+    _flat(lse, R, F32, "lse"); _flat(grad_loss, R, F32, "grad_loss"); _flat(loss, R, F32, "loss")
     lddh = _rows_of(dh, (R, d), BF16, "dh")
     if dw is not None and dw.dtype not in (BF16, F32):
         raise ValueError(f"dw must be bf16 or fp32, got {dw.dtype}")
@@ -597,8 +598,8 @@ def linear_ce_bwd(h, w, labels, lse, grad_loss, dh=None, dw=None, *, ignore_inde
         return None
     need = lib.paced_linear_ce_bwd_workspace_bytes(R, V, d)
     ws = _workspace(workspace, need, h.device)
-    _lib.check(lib.paced_linear_ce_bwd(_p(h), ldh, _p(w), ldw, _p(labels), _p(lse), _p(grad_loss), _p(dh), lddh, _p(dw), lddw, int(f32),
-                                       R, V, d, ignore_index, scale, _p(ws), need, _stream()), "paced_linear_ce_bwd")
+    _lib.check(lib.paced_linear_ce_bwd_ex(_p(h), ldh, _p(w), ldw, _p(labels), _p(loss), _p(lse), _p(grad_loss), _p(dh), lddh, _p(dw), lddw, int(f32),
+                                          R, V, d, ignore_index, scale, _p(ws), need, _stream()), "paced_linear_ce_bwd_ex")
     return dh
 
 

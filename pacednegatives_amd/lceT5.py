@@ -462,7 +462,7 @@ class LCEModel:
                     on_rows(rows)
                 for k, (st, l, c) in enumerate(zip(states, lab, cuts)):
                     dy = torch.empty_like(st.y)
-                    K.linear_ce_bwd(st.y, head, l, lses[k], weight[c], dy, self.model.params.grad("shared"), ignore_index=ign)
+                    K.linear_ce_bwd(st.y, head, l, lses[k], weight[c], dy, self.model.params.grad("shared"), ignore_index=ign, loss=ce[c])
                     last = k == len(states) - 1                 # the last pass over the gradients
                     self.model.engine.backward(st, dy=dy, on_segments_done=on_segments_done if last else None)
             elif len(states) == 1:
