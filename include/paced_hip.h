@@ -184,7 +184,8 @@ int paced_layernorm_bwd(const void* dy, int lddy, const void* x, int ldx, const 
  * dequantize gives the checkpoint's values, all of which are bf16 values.
  * dweight: dw [M, N] fp32 (+)= dy^T x for the checkpoint's values x [T, N] and dy [T, M] bf16 (rows of lddy elements, or
  * head-major as in paced_gemm_bf16_heads: lddy = 64 and dy_heads > 0; the rows up to the next multiple of 64 must then be
- * finite); M % 8 == 0, N % 16 == 0, lddw % 4 == 0.  Products are exact, sums fp32 in a fixed order (no atomics).
+ * finite); M % 8 == 0, N % 16 == 0, lddw % 4 == 0.  64 tokens of dy, or four of its heads, must span less than 2 GiB: lddy
+ * up to 2^24 - 72, dy_heads up to 2^28 - 1032; any number of tokens otherwise.  Products are exact, sums fp32 in a fixed order (no atomics).
  * accumulate = 0: dw is written, 1: added to.  workspace, 16-byte aligned, not kept between calls, for one stream at a time:
  * paced_act8_dweight_workspace_bytes(T, M, N) bytes (0: none needed). */
 int paced_act8_quantize(const void* x, int ldx, void* q, void* scale, int T, int n, void* stream);

@@ -554,19 +554,14 @@ extern "C" int paced_act8_dweight(const void* dy, int lddy, long long dy_heads, 
     const size_t need = pl.splits == 1 ? 0 : (size_t)pl.splits * M * N * 4;
     PACED_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                     "paced_act8_dweight: a 16-byte aligned workspace of %zu bytes is needed, got %zu", need, workspace_bytes);
-    // offsets inside one slice are 32-bit
-    const unsigned long long span = (dy_heads > 0 ? 4ull * dy_heads : (unsigned long long)pl.k_per_split * lddy) * 2 + (unsigned long long)pl.k_per_split * 128;
-    PACED_CHECK_ARG(span < (1ull << 31) && (unsigned long long)pl.k_per_split * N < (1ull << 31),
-                    "paced_act8_dweight: a slice of %d tokens spans more than 2 GiB; pass fewer tokens at a time", pl.k_per_split);
-    DwParams p;
-    p.dy = (const bf16*)dy; p.q = (const unsigned char*)q; p.scale = (const unsigned char*)scale;
-    p.M = M; p.N = N; p.T = T; p.lddy = lddy; p.heads = dy_heads > 0 ? dy_heads : 0;
-    p.k_per_split = pl.k_per_split;
-    p.out = need ? (float*)workspace : dw;
-    p.ldout = need ? N : lddw;
-    p.slab = (long long)M * N;
-    p.add = !need && accumulate;
-    const int total = pl.ntm * pl.ntn * pl.splits;
+    // Offsets inside one slice are 32-bit: `reach` tokens of dy (a tile's four heads, or whole rows) and of the codes span less than
+    // 2 GiB.  Where the plan's slices are longer, the tokens go by in passes of at most as many slices, each added to the one
+    // before (139264 tokens, 8192 x 2048: two).
+    const long long most = (1ll << 31) - 1, apart = dy_heads > 0 ? 8 * dy_heads : 0;
+    const long long by_dy = (most - apart) / (dy_heads > 0 ? 128 : 2ll * lddy + 128), by_codes = most / N;
+    const long long reach = (by_dy < by_codes ? by_dy : by_codes) / BK * BK;
+    PACED_CHECK_ARG(apart < most && reach > 0, "paced_act8_dweight: 64 tokens of dy (lddy=%d, heads %lld elements apart) span more than 2 GiB", lddy, dy_heads);
+    const int passes = (int)((T + pl.splits * reach - 1) / (pl.splits * reach));
     if (pl.tile == 256) {
         static PerDeviceOnce once;
         bool& attr_set = once.flag();
@@ -575,13 +570,30 @@ extern "C" int paced_act8_dweight(const void* dy, int lddy, long long dy_heads, 
             if (e != hipSuccess) { paced_set_error("paced_act8_dweight: hipFuncSetAttribute(%d bytes LDS) failed: %s", DP_LDS, hipGetErrorString(e)); return PACED_ERR_HIP; }
             attr_set = true;
         }
-        const int cus = paced_cu_count();
-        hipLaunchKernelGGL(act8_dw_phased_kernel, dim3(total < cus ? total : cus), dim3(512), DP_LDS, s, p, pl.ntm, pl.ntn, total);
-    } else hipLaunchKernelGGL(act8_dw_kernel, dim3(total), dim3(512), DW_NS * DW_STEP, s, p, pl.ntm, pl.ntn, total);
-    PACED_CHECK_LAUNCH();
-    if (need) {
-        hipLaunchKernelGGL(slab_sum_kernel, dim3(flat_blocks((long long)M * (N >> 2))), dim3(256), 0, s, p.out, pl.splits, p.slab, dw, lddw, M, N, accumulate);
+    }
+    const int ktiles = (T + BK - 1) / BK, a_pass = (ktiles + passes - 1) / passes;
+    for (int first = 0; first < ktiles; first += a_pass) {
+        const int steps = a_pass < ktiles - first ? a_pass : ktiles - first, t0 = first * BK;
+        const int per = (steps + pl.splits - 1) / pl.splits, splits = (steps + per - 1) / per;
+        const int add = accumulate || first > 0;
+        DwParams p;
+        p.dy = (const bf16*)dy + (size_t)t0 * lddy;                  // (rows of 64 where it is head-major)
+        p.q = (const unsigned char*)q + (size_t)t0 * N;
+        p.scale = (const unsigned char*)scale + (size_t)(t0 / QBLOCK) * N;
+        p.M = M; p.N = N; p.T = first + steps < ktiles ? steps * BK : T - t0; p.lddy = lddy; p.heads = dy_heads > 0 ? dy_heads : 0;
+        p.k_per_split = per * BK;
+        p.out = need ? (float*)workspace : dw;
+        p.ldout = need ? N : lddw;
+        p.slab = (long long)M * N;
+        p.add = !need && add;
+        const int total = pl.ntm * pl.ntn * splits, cus = paced_cu_count();
+        if (pl.tile == 256) hipLaunchKernelGGL(act8_dw_phased_kernel, dim3(total < cus ? total : cus), dim3(512), DP_LDS, s, p, pl.ntm, pl.ntn, total);
+        else hipLaunchKernelGGL(act8_dw_kernel, dim3(total), dim3(512), DW_NS * DW_STEP, s, p, pl.ntm, pl.ntn, total);
         PACED_CHECK_LAUNCH();
+        if (need) {
+            hipLaunchKernelGGL(slab_sum_kernel, dim3(flat_blocks((long long)M * (N >> 2))), dim3(256), 0, s, p.out, splits, p.slab, dw, lddw, M, N, add);
+            PACED_CHECK_LAUNCH();
+        }
     }
     return PACED_OK;
 }
