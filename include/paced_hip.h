@@ -180,7 +180,7 @@ int paced_layernorm_bwd(const void* dy, int lddy, const void* x, int ldx, const 
  * of n bytes) and scale [ceil(T/32), n] (exponent + 127 in a byte, one for 32 tokens of a feature): value = code *
  * 2^(scale - 127).  The scale is the smallest power of two, 2^-117 at least, that brings the block's largest magnitude to
  * 448 or less; codes round to nearest, ties to even (and stop at 240 under the scale 2^120).  A block with a NaN or an
- * infinity reads back as NaN throughout (scale 255).  n % 16 == 0, 16-byte aligned operands, row strides % 8 == 0; T >= 0.
+ * infinity reads back as NaN throughout (scale 255).  n % 16 == 0, 16-byte aligned operands, row strides % 8 == 0; 0 <= T <= 2^31 - 64.
  * dequantize gives the checkpoint's values, all of which are bf16 values.
  * dweight: dw [M, N] fp32 (+)= dy^T x for the checkpoint's values x [T, N] and dy [T, M] bf16 (rows of lddy elements, or
  * head-major as in paced_gemm_bf16_heads: lddy = 64 and dy_heads > 0; the rows up to the next multiple of 64 must then be

@@ -18,6 +18,7 @@
 namespace {
 
 constexpr int QBLOCK = 32;                 // tokens per scale
+constexpr int MAX_T = 0x7fffffff - 63;     // tokens of a call: rounded up to K steps they are still an int
 constexpr int MIN_CODE = 127 - 117, MAX_CODE = 127 + 120, NAN_CODE = 255;
 
 // ------------------------------------------------------------------------------------------------ writing and reading
@@ -503,7 +504,7 @@ int flat_blocks(long long items) {
 }  // namespace
 
 extern "C" int paced_act8_quantize(const void* x, int ldx, void* q, void* scale, int T, int n, void* stream) {
-    PACED_CHECK_ARG(T >= 0 && n > 0 && n % 16 == 0, "paced_act8_quantize: need T >= 0 and n a multiple of 16 (T=%d n=%d)", T, n);
+    PACED_CHECK_ARG(T >= 0 && T <= MAX_T && n > 0 && n % 16 == 0, "paced_act8_quantize: need T >= 0, at most %d, and n a multiple of 16 (T=%d n=%d)", MAX_T, T, n);
     if (T == 0) return PACED_OK;
     PACED_CHECK_ARG(x && q && scale, "paced_act8_quantize: null operand");
     PACED_CHECK_ARG(ldx >= n && ldx % 8 == 0 && (((uintptr_t)x | (uintptr_t)q | (uintptr_t)scale) & 15) == 0,
@@ -516,7 +517,7 @@ extern "C" int paced_act8_quantize(const void* x, int ldx, void* q, void* scale,
 }
 
 extern "C" int paced_act8_dequantize(const void* q, const void* scale, void* y, int ldy, int T, int n, void* stream) {
-    PACED_CHECK_ARG(T >= 0 && n > 0 && n % 16 == 0, "paced_act8_dequantize: need T >= 0 and n a multiple of 16 (T=%d n=%d)", T, n);
+    PACED_CHECK_ARG(T >= 0 && T <= MAX_T && n > 0 && n % 16 == 0, "paced_act8_dequantize: need T >= 0, at most %d, and n a multiple of 16 (T=%d n=%d)", MAX_T, T, n);
     if (T == 0) return PACED_OK;
     PACED_CHECK_ARG(q && scale && y, "paced_act8_dequantize: null operand");
     PACED_CHECK_ARG(ldy >= n && ldy % 8 == 0 && (((uintptr_t)y | (uintptr_t)q | (uintptr_t)scale) & 15) == 0,
@@ -528,15 +529,15 @@ extern "C" int paced_act8_dequantize(const void* q, const void* scale, void* y, 
 }
 
 extern "C" size_t paced_act8_dweight_workspace_bytes(int T, int M, int N) {
-    if (T <= 0 || M <= 0 || N <= 0) return 0;
+    if (T <= 0 || T > MAX_T || M <= 0 || N <= 0) return 0;
     const DwPlan pl = dw_plan(T, M, N);
     return pl.splits == 1 ? 0 : (size_t)pl.splits * M * N * 4;
 }
 
 extern "C" int paced_act8_dweight(const void* dy, int lddy, long long dy_heads, const void* q, const void* scale, float* dw, int lddw,
                                   int T, int M, int N, int accumulate, void* workspace, size_t workspace_bytes, void* stream) {
-    PACED_CHECK_ARG(T >= 0 && M > 0 && N > 0 && M % 8 == 0 && N % 16 == 0,
-                    "paced_act8_dweight: need T >= 0, M a multiple of 8 and N a multiple of 16 (T=%d M=%d N=%d)", T, M, N);
+    PACED_CHECK_ARG(T >= 0 && T <= MAX_T && M > 0 && N > 0 && M % 8 == 0 && N % 16 == 0,
+                    "paced_act8_dweight: need T >= 0, at most %d, M a multiple of 8 and N a multiple of 16 (T=%d M=%d N=%d)", MAX_T, T, M, N);
     PACED_CHECK_ARG(dw && lddw >= N && lddw % 4 == 0 && ((uintptr_t)dw & 15) == 0,
                     "paced_act8_dweight: dw must be 16-byte aligned with a row stride of at least N and a multiple of 4 (lddw=%d)", lddw);
     PACED_CHECK_ARG(T == 0 || (dy && q && scale && (((uintptr_t)dy | (uintptr_t)q | (uintptr_t)scale) & 15) == 0), "paced_act8_dweight: dy, q and scale must be 16-byte aligned");
