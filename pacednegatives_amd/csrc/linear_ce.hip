@@ -441,13 +441,21 @@ extern "C" int paced_linear_ce_bwd_ex(const void* h, int ldh, const void* w, int
     }
     PACED_CHECK_ARG(lse && gloss, "paced_linear_ce_bwd: null operand");
     PACED_CHECK_ARG(!dh || (lddh >= d && lddh % 8 == 0 && ((uintptr_t)dh & 15) == 0), "paced_linear_ce_bwd: dh needs 16-byte aligned rows, a stride of at least d and a multiple of 8 (lddh=%d)", lddh);
-    const CePlan pl = ce_plan(R, V, d);
+    CePlan pl = ce_plan(R, V, d);
     const size_t need = ce_workspace(pl, R, d);
     PACED_CHECK_ARG(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
                     "paced_linear_ce_bwd: a 16-byte aligned workspace of %zu bytes is needed, got %zu", need, workspace_bytes);
     // a transposed operand is addressed with 32-bit byte offsets from its first row
     PACED_CHECK_ARG((unsigned long long)R * (ldh > pl.ldp ? ldh : pl.ldp) < (1ull << 31), "paced_linear_ce_bwd: %d rows of h with a stride of %d span 4 GiB or more; pass fewer at a time", R, ldh);
-    PACED_CHECK_ARG((unsigned long long)pl.piece * ldw < (1ull << 31), "paced_linear_ce_bwd: %d rows of w with a stride of %d span 4 GiB or more; pass w with a smaller stride", pl.piece, ldw);
+    // (of w only a piece: one whose rows lie so far apart that the plan's piece is out of reach goes by in narrower ones, which
+    // need no more of the workspace: 256 rows at the largest stride)
+    const int reach = (int)(((1u << 31) - 1) / (unsigned)ldw / 256 * 256);
+    if (pl.piece > reach) {
+        pl.piece = reach;
+        pl.ldp = reach;
+        const int steps = reach / 64, per = (steps + pl.slabs - 1) / pl.slabs;
+        pl.slabs = (steps + per - 1) / per;                       // (the first piece writes every slab)
+    }
     bf16* P = (bf16*)workspace;
     const size_t part = round256((size_t)R * pl.ldp * 2);
     const int forced = paced_gemm_forced_tile();                  // (the low part is written by the 64x64 tiles' epilogue)
