@@ -275,7 +275,8 @@ int paced_cross_entropy(const float* logits, const long long* labels, float* los
  * bwd: gloss[r] = d objective / d loss[r] (fp32); dh [R, d] bf16 is written, dw [V, d] is written in bf16 (dw_f32 = 0) or added
  *      to in fp32 (dw_f32 = 1); each may be NULL.  The logits' gradient gloss (softmax - onehot) scale is rounded to bf16
  *      between the products, as paced_cross_entropy's dlogits are; what the label's entry loses in it is added to dh again,
- *      and up to 64 rows dw takes every entry's low part as well.  Sums are fp32 in a fixed order, without atomics.  An
+ *      and up to 64 rows dw takes every entry's low part as well (2^-16 of each addend is lost).  From 65 rows on an element of dw
+ *      is off by up to 2^-8 of the sum of its addends' magnitudes, be it one row's (a label of its own) or many rows'.  Sums are fp32 in a fixed order, without atomics.  An
  *      ignored row's h must be finite where dw is wanted (0 times it is added), w where dh is.
  * Row strides are at most 2^22 elements; bwd refuses an h whose R rows span 4 GiB or more.
  * workspace, 16-byte aligned, not kept between calls, for one stream at a time: ..._workspace_bytes() bytes; fwd V R / 4 +

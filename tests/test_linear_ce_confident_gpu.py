@@ -75,3 +75,29 @@ def test_refusals():
     for loss, words in ((v[:4], "loss must hold"), (v.double(), "loss must be"), (v.cpu(), "device tensor")):
         with pytest.raises(ValueError, match=words):
             K.linear_ce_bwd(h, w, labels, v, v, torch.empty_like(h), loss=loss)
+
+
+@pytest.mark.parametrize("R,V,d", [(65, 5000, 256), (300, 1000, 512), (1088, 6401, 256)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_beyond_64_rows_dw_loses_half_a_step_of_p_and_no_more(R, V, d, f32):
+    """Rows with labels of their own, so that one addend is most of an element, and rows that share one.  P's entries are off by
+    a uniform error of at most 2^-8 of themselves, 2^-8 / sqrt(3) in the root mean square: by that much of the root of the sum of
+    P^2 h^2 as a whole (a tenth more for chance), by 2^-8 of the sum of |P h| element by element (and 2^-11 for logits
+    off by D < 2^-13 twice and sums of up to 1088 addends in 32 bits); dw's own rounding adds the same of dw."""
+    from test_linear_ce_gpu import make, oracle
+    h, w, labels, gl = make(R, V, d, R, ignored=0.0, size=1.0)
+    labels[:R // 2] = torch.arange(R // 2, device="cuda")
+    labels[R // 2:R // 2 + 9] = V - 1
+    o = oracle(h, w, labels, gl, 1.0)
+    assert o["D"].max() < 2.0 ** -13
+    loss, lse = torch.empty(R, device="cuda"), torch.empty(R, device="cuda")
+    dw = torch.zeros(V, d, device="cuda", dtype=F32 if f32 else BF16)
+    K.linear_ce_fwd(h, w, labels, loss, lse)
+    K.linear_ce_bwd(h, w, labels, lse, gl, None, dw, loss=loss)
+    want, half = o["P"].t() @ o["h"], 2.0 ** -8
+    err = dw.to(F64) - want
+    root = (o["P"].square().t() @ o["h"].square()).sum().sqrt()
+    own = 0.0 if f32 else half / 3 ** 0.5 * want.norm()
+    assert err.norm() <= 1.1 * ((half / 3 ** 0.5 * root) ** 2 + own ** 2) ** 0.5
+    size = o["P"].abs().t() @ o["h"].abs()
+    assert (err.abs() <= (half + 2.0 ** -11) * size + (0 if f32 else half * (1 + half) * want.abs() + 2.0 ** -133)).all()
