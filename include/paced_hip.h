@@ -289,6 +289,12 @@ size_t paced_linear_ce_bwd_workspace_bytes(int R, int V, int d);
 int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ldw, const long long* labels, const float* lse, const float* gloss,
                         void* dh, int lddh, void* dw, int lddw, int dw_f32, int R, int V, int d, long long ignore_index, float scale,
                         void* workspace, size_t workspace_bytes, void* stream);
+/* paced_linear_ce_fwd with the launch option grid_limit of paced_gemm_opts (< 0: the process default; 0: one workgroup to a compute
+ * unit; n > 0: at most n for a launch of 256x256 tiles): the training step's no-grad forwards, lceT5.py:131-133, leave compute units to
+ * the kernels of the pass beside them.  The same bits with any limit that leaves the choice of tiles as it is. */
+int paced_linear_ce_fwd_ex(const void* h, int ldh, const void* w, int ldw, const long long* labels, float* loss, float* lse,
+                           int R, int V, int d, long long ignore_index, float scale, int grid_limit, void* workspace, size_t workspace_bytes,
+                           void* stream);
 /* paced_linear_ce_bwd with the losses of the forward pass (fp32 [R]; NULL: as paced_linear_ce_bwd).  The label's entry is then
  * gloss (exp(-loss) - 1) and keeps its relative precision however small the loss; from lse alone it is gloss (exp(z - lse) - 1),
  * off by about 2^-22 (|lse| + |z|) gloss whatever the loss: 1 % of itself at a loss of 1e-4, all of it below 1e-6. */

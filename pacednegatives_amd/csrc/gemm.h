@@ -60,6 +60,7 @@ struct GemmParams {
     int ce_rows = 0;                        // rows of part (a launch may cover some of them)
     int accumulate = 0;                     // EPI_SLAB_F32: add to what is there
     int tile = 0;                           // tile edge the caller has chosen (0: the launch's own rule; paced_gemm_set_tile overrides)
+    int grid_limit = -1;                    // most workgroups of a phased launch (< 0: the call's or the process's own; 0: one to a compute unit)
 };
 
 // Order-preserving 64-bit key: larger key <=> (higher score, then lower pool row).
@@ -79,6 +80,8 @@ __host__ __device__ __forceinline__ unsigned int topk_key_row(unsigned long long
 // Launches the tiled kernel for (trans_a, trans_b, epilogue); arguments are already validated.
 // tile edge that paced_gemm_set_tile has forced (0: none)
 int paced_gemm_forced_tile();
+// most workgroups of a phased launch where GemmParams names no limit (0: one to a compute unit)
+int paced_gemm_default_grid_limit();
 // columns per statistics group of the calling thread's most recent EPI_CE_STATS launch
 int paced_gemm_stat_width();
 int paced_gemm_launch(const GemmParams& p, bool trans_a, bool trans_b, int epilogue, int splits, hipStream_t stream);

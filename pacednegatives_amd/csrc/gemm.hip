@@ -1379,7 +1379,7 @@ int launch_cfg(GemmParams p, int splits, hipStream_t stream) {
         // At most g_grid_limit workgroups: the compute units the grid leaves out stay free for the kernels of other
         // streams for as long as this launch runs (a phased workgroup holds all of a unit's LDS and registers until
         // the whole launch is over, so nothing else starts on a unit it has taken).
-        const int limit = eff_grid_limit();
+        const int limit = p.grid_limit >= 0 ? p.grid_limit : eff_grid_limit();
         if (limit > 0 && limit < slots) slots = limit;
     }
     constexpr bool RINGABLE = !PHASED && EPI != EPI_TOPK_DENSE && EPI != EPI_TOPK_FILTER;
@@ -1509,6 +1509,7 @@ extern "C" int paced_gemm_set_tile(int tile) {
 }
 
 int paced_gemm_forced_tile() { return eff_tile(); }
+int paced_gemm_default_grid_limit() { return eff_grid_limit(); }
 int paced_gemm_stat_width() { return t_stat_width; }
 extern "C" int paced_gemm_last_kernel(void) { return t_last_kernel; }
 

@@ -320,7 +320,8 @@ int ce_logits(GemmParams p, int epilogue, hipStream_t s) {
             const double us = tile_us(256, full, p.N, steps, cus) + tile_us(128, R - full, p.N, steps, cus) + TWO_LAUNCHES;
             if (us < best) { best = us; rows = full; }
         }
-        const int fill = whole_rounds(p.N, R, cus);
+        const int limit = p.grid_limit >= 0 ? p.grid_limit : paced_gemm_default_grid_limit();
+        const int fill = whole_rounds(p.N, R, limit > 0 && limit < cus ? limit : cus);
         if (fill > 0 && fill < p.N && tile_us(256, R, fill, steps, cus) + tile_us(128, R, p.N - fill, steps, cus) + TWO_LAUNCHES < best) { rows = 0; cols = fill; }
     }
     if (!rows && !cols) return paced_gemm_launch(p, false, false, epilogue, 1, s);
@@ -392,8 +393,9 @@ extern "C" size_t paced_linear_ce_fwd_workspace_bytes(int R, int V) {
     return round256((size_t)((V + 31) / 32) * R * 8) + round256((size_t)R * 4);
 }
 
-extern "C" int paced_linear_ce_fwd(const void* h, int ldh, const void* w, int ldw, const long long* labels, float* loss, float* lse,
-                                   int R, int V, int d, long long ignore_index, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int paced_linear_ce_fwd_ex(const void* h, int ldh, const void* w, int ldw, const long long* labels, float* loss, float* lse,
+                                      int R, int V, int d, long long ignore_index, float scale, int grid_limit, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
     const int rc = ce_check("paced_linear_ce_fwd", h, ldh, w, ldw, labels, R, V, d);
     if (rc != PACED_OK || R == 0) return rc;
     PACED_CHECK_ARG(loss, "paced_linear_ce_fwd: null operand");
@@ -405,6 +407,7 @@ extern "C" int paced_linear_ce_fwd(const void* h, int ldh, const void* w, int ld
     p.ce_target = (float*)((char*)workspace + round256((size_t)((V + 31) / 32) * R * 8));
     p.ce_labels = labels; p.ce_ignore = ignore_index; p.ce_vocab = V;
     p.ce_rows = R;
+    p.grid_limit = grid_limit;
     const int rg = ce_logits(p, EPI_CE_STATS, (hipStream_t)stream);
     if (rg != PACED_OK) return rg;
     const int width = paced_gemm_stat_width();
@@ -415,6 +418,11 @@ extern "C" int paced_linear_ce_fwd(const void* h, int ldh, const void* w, int ld
         hipLaunchKernelGGL(ce_join_kernel<1>, dim3(R), dim3(256), 0, (hipStream_t)stream, p.ce_part, groups, p.ce_target, labels, ignore_index, V, loss, lse, R);
     PACED_CHECK_LAUNCH();
     return PACED_OK;
+}
+
+extern "C" int paced_linear_ce_fwd(const void* h, int ldh, const void* w, int ldw, const long long* labels, float* loss, float* lse,
+                                   int R, int V, int d, long long ignore_index, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+    return paced_linear_ce_fwd_ex(h, ldh, w, ldw, labels, loss, lse, R, V, d, ignore_index, scale, -1, workspace, workspace_bytes, stream);
 }
 
 namespace {

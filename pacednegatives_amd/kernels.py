@@ -560,21 +560,21 @@ def _head_operands(h, w, labels):
     return R, V, d, _rows_of(h, (R, d), BF16, "h"), _rows_of(w, (V, d), BF16, "w")
 
 
-def linear_ce_fwd(h, w, labels, loss, lse=None, *, ignore_index=-100, scale=1.0, workspace=None):
+def linear_ce_fwd(h, w, labels, loss, lse=None, *, ignore_index=-100, scale=1.0, grid_limit=None, workspace=None):
     """Cross entropy of a linear head without its logits: loss[r] = logsumexp(z[r]) - z[r, label] for z = scale * h w^T
     (h bf16 [R, d], w bf16 [V, d], labels int64 [R]); rows whose label is ``ignore_index`` or outside [0, V) give 0.
-    ``lse`` (fp32 [R]) is what ``linear_ce_bwd`` needs."""
+    ``lse`` (fp32 [R]) is what ``linear_ce_bwd`` needs; ``grid_limit`` as in ``gemm``."""
     lib = _lib.load()
     other = _elsewhere(h=h, w=w, labels=labels, loss=loss, lse=lse)
     if other is not None:
         with torch.cuda.device(other):
-            return linear_ce_fwd(h, w, labels, loss, lse, ignore_index=ignore_index, scale=scale, workspace=workspace)
+            return linear_ce_fwd(h, w, labels, loss, lse, ignore_index=ignore_index, scale=scale, grid_limit=grid_limit, workspace=workspace)
     R, V, d, ldh, ldw = _head_operands(h, w, labels)
     _flat(loss, R, F32, "loss"); _flat(lse, R, F32, "lse")
     need = lib.paced_linear_ce_fwd_workspace_bytes(R, V)
     ws = _workspace(workspace, need, h.device)
-    _lib.check(lib.paced_linear_ce_fwd(_p(h), ldh, _p(w), ldw, _p(labels), _p(loss), _p(lse), R, V, d, ignore_index, scale, _p(ws), need,
-                                       _stream()), "paced_linear_ce_fwd")
+    _lib.check(lib.paced_linear_ce_fwd_ex(_p(h), ldh, _p(w), ldw, _p(labels), _p(loss), _p(lse), R, V, d, ignore_index, scale,
+                                          -1 if grid_limit is None else int(grid_limit), _p(ws), need, _stream()), "paced_linear_ce_fwd_ex")
     return loss
 
 

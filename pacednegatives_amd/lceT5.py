@@ -416,15 +416,28 @@ class LCEModel:
         if share and self.dropout != 0.0:
             raise ValueError("share_forward needs dropout 0: with dropout on, the reference's two passes draw different masks")
 
+        def fused_losses(states, keep_lse, gemm_grid=0):
+            """Loss rows of the head's inputs ``st.y`` of one packed state or of the positives' and the negatives' own, each
+            state's in one call (they share the head's weights); all rows, and (state, labels, rows, lse) of each."""
+            ce = torch.empty(2 * B * (1 + nneg), dtype=F32, device=self.device)
+            labels = [torch.cat([plab, nlab])] if len(states) == 1 else [plab, nlab]
+            cuts = [slice(0, ce.numel())] if len(states) == 1 else [slice(0, 2 * B), slice(2 * B, ce.numel())]
+            parts = []
+            for st, l, c in zip(states, labels, cuts):
+                lse = torch.empty_like(ce[c]) if keep_lse else None
+                K.linear_ce_fwd(st.y, head, l, ce[c], lse, ignore_index=ign, grid_limit=gemm_grid if gemm_grid > 0 else None)
+                parts.append((st, l, c, lse))
+            return ce, parts
+
         def no_grad_rows(gemm_grid=0):
             """(a) no-grad forwards and the LCE rows                                        :131-135"""
             states, plog, nlog = self._forward_pair(p, n, save=False, call=0, gemm_grid=gemm_grid)
-            pce = torch.empty(2 * B, dtype=F32, device=self.device)
-            nce = torch.empty(2 * B * nneg, dtype=F32, device=self.device)
             if self.fused_loss:
-                K.linear_ce_fwd(plog, head, plab, pce, ignore_index=ign)
-                K.linear_ce_fwd(nlog, head, nlab, nce, ignore_index=ign)
+                ce, _ = fused_losses(states, False, gemm_grid)
+                pce, nce = ce[:2 * B], ce[2 * B:]
             else:
+                pce = torch.empty(2 * B, dtype=F32, device=self.device)
+                nce = torch.empty(2 * B * nneg, dtype=F32, device=self.device)
                 K.cross_entropy(plog, plab, pce, None, ignore_index=ign)
                 K.cross_entropy(nlog, nlab, nce, None, ignore_index=ign)
             rows = torch.empty(2 * B, dtype=F32, device=self.device)
@@ -448,21 +461,15 @@ class LCEModel:
             nce2 = torch.empty(2 * B * nneg, dtype=F32, device=self.device)
             rows = torch.empty(2 * B, dtype=F32, device=self.device)
             if self.fused_loss:
-                # each state's rows in one call: the positives' and the negatives' weights differ, not the arithmetic
-                lab = [torch.cat([plab, nlab])] if len(states) == 1 else [plab, nlab]
-                ce, lses = torch.empty(2 * B * (1 + nneg), dtype=F32, device=self.device), []
-                weight = torch.full_like(ce, g_pos)
+                ce, parts = fused_losses(states, True)
+                weight = torch.full_like(ce, g_pos)          # the positives' and the negatives' weights differ, not the arithmetic
                 weight[2 * B:] = g_neg
-                cuts = [slice(0, 2 * B * (1 + nneg))] if len(states) == 1 else [slice(0, 2 * B), slice(2 * B, 2 * B * (1 + nneg))]
-                for st, l, c in zip(states, lab, cuts):
-                    lses.append(torch.empty_like(ce[c]))
-                    K.linear_ce_fwd(st.y, head, l, ce[c], lses[-1], ignore_index=ign)
                 K.lce_group(ce[:2 * B], ce[2 * B:], rows, nneg, use_mean)
                 if on_rows is not None:
                     on_rows(rows)
-                for k, (st, l, c) in enumerate(zip(states, lab, cuts)):
+                for k, (st, l, c, lse) in enumerate(parts):
                     dy = torch.empty_like(st.y)
-                    K.linear_ce_bwd(st.y, head, l, lses[k], weight[c], dy, self.model.params.grad("shared"), ignore_index=ign, loss=ce[c])
+                    K.linear_ce_bwd(st.y, head, l, lse, weight[c], dy, self.model.params.grad("shared"), ignore_index=ign, loss=ce[c])
                     last = k == len(states) - 1                 # the last pass over the gradients
                     self.model.engine.backward(st, dy=dy, on_segments_done=on_segments_done if last else None)
             elif len(states) == 1:
