@@ -289,6 +289,10 @@ size_t paced_linear_ce_bwd_workspace_bytes(int R, int V, int d);
 int paced_linear_ce_bwd(const void* h, int ldh, const void* w, int ldw, const long long* labels, const float* lse, const float* gloss,
                         void* dh, int lddh, void* dw, int lddw, int dw_f32, int R, int V, int d, long long ignore_index, float scale,
                         void* workspace, size_t workspace_bytes, void* stream);
+/* How the calling THREAD's most recent loss calls cut their products into two launches (host_ pointers; for tests and benchmarks, as
+ * paced_gemm_last_kernel): rows or columns of the logits and rows of dw in the first launch, 0 where there was one launch.  Of
+ * several pieces of the vocabulary, the last one's. */
+int paced_linear_ce_last_split(int* host_rows, int* host_cols, int* host_dw_rows);
 /* paced_linear_ce_fwd with the launch option grid_limit of paced_gemm_opts (< 0: the process default; 0: one workgroup to a compute
  * unit; n > 0: at most n for a launch of 256x256 tiles): the training step's no-grad forwards, lceT5.py:131-133, leave compute units to
  * the kernels of the pass beside them.  The same bits with any limit that leaves the choice of tiles as it is. */

@@ -305,6 +305,10 @@ GemmParams product(const void* A, int lda, const void* B, int ldb, void* C, int 
     return p;
 }
 
+// rows or columns of the logits, and rows of dw, in the first of two launches of this thread's most recent products (0: one launch)
+struct Split { int rows, cols, dw_rows; };
+thread_local Split t_split = {0, 0, 0};
+
 // One product of the logits (EPI_CE_STATS or EPI_CE_GRAD): in one launch, or in two, 256x256 tiles and what they leave over in
 // 128x128 tiles, where that saves a round: the rows that fill tiles and the rest (1088 rows x 32128 entries: 3 rounds for 4.25
 // tiles of rows, 2 for 4), or the columns that fill whole rounds and the rest (1000 x 50001: 3.06 rounds).  Both launches leave
@@ -324,6 +328,8 @@ int ce_logits(GemmParams p, int epilogue, hipStream_t s) {
         const int fill = whole_rounds(p.N, R, limit > 0 && limit < cus ? limit : cus);
         if (fill > 0 && fill < p.N && tile_us(256, R, fill, steps, cus) + tile_us(128, R, p.N - fill, steps, cus) + TWO_LAUNCHES < best) { rows = 0; cols = fill; }
     }
+    t_split.rows = rows;
+    t_split.cols = cols;
     if (!rows && !cols) return paced_gemm_launch(p, false, false, epilogue, 1, s);
     p.tile = 256;
     rest.tile = 128;
@@ -362,6 +368,7 @@ int ce_dw(GemmParams p, int epilogue, size_t element, hipStream_t s) {
     const int steps = (p.K + 63) / 64, cus = paced_cu_count();
     int rows;
     dw_us(p.M, p.N, steps, cus, &rows);
+    t_split.dw_rows = rows;
     if (rows) {
         GemmParams first = p;
         first.M = rows;
@@ -387,6 +394,14 @@ int ce_check(const char* who, const void* h, int ldh, const void* w, int ldw, co
 }
 
 }  // namespace
+
+extern "C" int paced_linear_ce_last_split(int* rows, int* cols, int* dw_rows) {
+    PACED_CHECK_ARG(rows && cols && dw_rows, "paced_linear_ce_last_split: null operand");
+    *rows = t_split.rows;
+    *cols = t_split.cols;
+    *dw_rows = t_split.dw_rows;
+    return PACED_OK;
+}
 
 extern "C" size_t paced_linear_ce_fwd_workspace_bytes(int R, int V) {
     if (R <= 0 || V <= 0) return 0;

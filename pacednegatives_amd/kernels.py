@@ -6,6 +6,7 @@ not match what its grid assumes.
 """
 from __future__ import annotations
 
+import ctypes as C
 import os
 
 import torch
@@ -576,6 +577,13 @@ def linear_ce_fwd(h, w, labels, loss, lse=None, *, ignore_index=-100, scale=1.0,
     _lib.check(lib.paced_linear_ce_fwd_ex(_p(h), ldh, _p(w), ldw, _p(labels), _p(loss), _p(lse), R, V, d, ignore_index, scale,
                                           -1 if grid_limit is None else int(grid_limit), _p(ws), need, _stream()), "paced_linear_ce_fwd_ex")
     return loss
+
+
+def linear_ce_last_split():
+    """(rows, columns, rows of dw) in the first of two launches of this thread's most recent loss products; 0 = one launch."""
+    out = [C.c_int(0) for _ in range(3)]
+    _lib.check(_lib.load().paced_linear_ce_last_split(*[C.byref(v) for v in out]), "paced_linear_ce_last_split")
+    return tuple(v.value for v in out)
 
 
 def linear_ce_bwd(h, w, labels, lse, grad_loss, dh=None, dw=None, *, ignore_index=-100, scale=1.0, loss=None, workspace=None):
