@@ -191,6 +191,8 @@ int paced_layernorm_bwd(const void* dy, int lddy, const void* x, int ldx, const 
 int paced_act8_quantize(const void* x, int ldx, void* q, void* scale, int T, int n, void* stream);
 int paced_act8_dequantize(const void* q, const void* scale, void* y, int ldy, int T, int n, void* stream);
 size_t paced_act8_dweight_workspace_bytes(int T, int M, int N);
+/* tile edge (64 or 256) of the calling THREAD's most recent paced_act8_dweight launch; for tests and benchmarks */
+int paced_act8_last_tile(void);
 int paced_act8_dweight(const void* dy, int lddy, long long dy_heads, const void* q, const void* scale, float* dw, int lddw,
                        int T, int M, int N, int accumulate, void* workspace, size_t workspace_bytes, void* stream);
 

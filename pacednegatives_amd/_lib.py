@@ -47,6 +47,7 @@ SIGNATURES = {
     "paced_layernorm_bwd": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _vp, _sz, _vp]),
     "paced_act8_quantize": (_i, [_vp, _i, _vp, _vp, _i, _i, _vp]),
     "paced_act8_dequantize": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
+    "paced_act8_last_tile": (_i, []),
     "paced_act8_dweight_workspace_bytes": (_sz, [_i, _i, _i]),
     "paced_act8_dweight": (_i, [_vp, _i, _ll, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
     "paced_embedding_fwd": (_i, [_vp, _vp, _vp, _i, _i, _i, _f, _u32, _vp]),

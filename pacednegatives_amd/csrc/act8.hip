@@ -496,6 +496,8 @@ DwPlan dw_plan(int T, int M, int N) {
     return pl;
 }
 
+thread_local int t_last_tile = 0;      // tile edge of this thread's most recent weight gradient
+
 int flat_blocks(long long items) {
     const long long g = (items + 255) / 256;
     return (int)(g < 1 ? 1 : g > 16384 ? 16384 : g);
@@ -527,6 +529,8 @@ extern "C" int paced_act8_dequantize(const void* q, const void* scale, void* y, 
     PACED_CHECK_LAUNCH();
     return PACED_OK;
 }
+
+extern "C" int paced_act8_last_tile(void) { return t_last_tile; }
 
 extern "C" size_t paced_act8_dweight_workspace_bytes(int T, int M, int N) {
     if (T <= 0 || T > MAX_T || M <= 0 || N <= 0) return 0;
@@ -572,6 +576,7 @@ extern "C" int paced_act8_dweight(const void* dy, int lddy, long long dy_heads, 
             attr_set = true;
         }
     }
+    t_last_tile = pl.tile;
     const int ktiles = (T + BK - 1) / BK, a_pass = (ktiles + passes - 1) / passes;
     for (int first = 0; first < ktiles; first += a_pass) {
         const int steps = a_pass < ktiles - first ? a_pass : ktiles - first, t0 = first * BK;
