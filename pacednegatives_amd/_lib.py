@@ -70,6 +70,7 @@ SIGNATURES = {
     "paced_linear_ce_fwd": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _ll, _f, _vp, _sz, _vp]),
     "paced_linear_ce_bwd_workspace_bytes": (_sz, [_i, _i, _i]),
     "paced_linear_ce_bwd": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _ll, _f, _vp, _sz, _vp]),
+    "paced_linear_ce_fwd_workspace_bytes_for": (_sz, [_i, _i, _i]),
     "paced_linear_ce_last_split": (_i, [C.POINTER(_i), C.POINTER(_i), C.POINTER(_i)]),
     "paced_linear_ce_fwd_ex": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _ll, _f, _i, _vp, _sz, _vp]),
     "paced_linear_ce_bwd_ex": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _ll, _f, _vp, _sz, _vp]),

@@ -59,7 +59,7 @@ struct GemmParams {
     int ce_vocab = 0, ce_first = 0;         // vocabulary size, entry of column 0
     int ce_rows = 0;                        // rows of part (a launch may cover some of them)
     int accumulate = 0;                     // EPI_SLAB_F32: add to what is there
-    int tile = 0;                           // tile edge the caller has chosen (0: the launch's own rule; paced_gemm_set_tile overrides)
+    int tile = 0;                           // tile edge the caller has chosen (0: the launch's own rule, or paced_gemm_set_tile's)
     int grid_limit = -1;                    // most workgroups of a phased launch (< 0: the call's or the process's own; 0: one to a compute unit)
 };
 

@@ -1443,7 +1443,7 @@ int launch_cfg(GemmParams p, int splits, hipStream_t stream) {
 
 template <bool TA, bool TB, int EPI>
 int launch(const GemmParams& p, int splits, hipStream_t stream) {
-    const int force_tile = eff_tile() ? eff_tile() : p.tile;
+    const int force_tile = p.tile ? p.tile : eff_tile();
     if (EPI == EPI_ATOMIC_F32 && splits <= 0 && force_tile == 0 && ring_enabled()) {
         // Short contraction into a mid-sized output (the decoder's weight gradients): the launch is bound by the
         // output, every split adds the whole output once more in atomics, and a big tile leaves CUs empty; take
@@ -1453,7 +1453,7 @@ int launch(const GemmParams& p, int splits, hipStream_t stream) {
         if (ktiles >= 3 && ktiles <= 32 && t64 <= 3LL * cu_count()) return launch_cfg<CfgTiny, TA, TB, EPI>(p, 0, stream);
     }
     bool large;
-    if (force_tile == 128 || (eff_tile() == 0 && p.tile == 64)) large = false;
+    if (force_tile == 128 || p.tile == 64) large = false;
     else if (force_tile == 256) large = true;
     else {
         // the 256x256 tile pays off once there is about one tile per CU (split slices count for atomics)

@@ -305,6 +305,10 @@ GemmParams product(const void* A, int lda, const void* B, int ldb, void* C, int 
     return p;
 }
 
+// Tile of the logits' product where it goes out as one launch.  Up to 64 rows 64x64 tiles read the weights fastest (16 rows: 16.6 us
+// against 18.4 with 128x128).  forced (0: none) is paced_gemm_set_tile's, read once by a call: its workspace's layout hangs on it.
+int ce_tile(int R, int N, int steps, int cus, int forced) { return forced ? forced : R <= FEW ? 64 : best_tile(R, N, steps, cus); }
+
 // rows or columns of the logits, and rows of dw, in the first of two launches of this thread's most recent products (0: one launch)
 struct Split { int rows, cols, dw_rows; };
 thread_local Split t_split = {0, 0, 0};
@@ -312,14 +316,14 @@ thread_local Split t_split = {0, 0, 0};
 // One product of the logits (EPI_CE_STATS or EPI_CE_GRAD): in one launch, or in two, 256x256 tiles and what they leave over in
 // 128x128 tiles, where that saves a round: the rows that fill tiles and the rest (1088 rows x 32128 entries: 3 rounds for 4.25
 // tiles of rows, 2 for 4), or the columns that fill whole rounds and the rest (1000 x 50001: 3.06 rounds).  Both launches leave
-// statistics of 64 columns.  Up to 64 rows 64x64 tiles read the weights fastest (16 rows: 16.6 us against 18.4 with 128x128).
-int ce_logits(GemmParams p, int epilogue, hipStream_t s) {
+// statistics of 64 columns.
+int ce_logits(GemmParams p, int epilogue, int forced, hipStream_t s) {
     const int steps = (p.K + 63) / 64, R = p.M, full = R / 256 * 256, cus = paced_cu_count();
-    p.tile = R <= FEW ? 64 : best_tile(R, p.N, steps, cus);
+    p.tile = ce_tile(R, p.N, steps, cus, forced);
     GemmParams rest = p;
     double best = tile_us(p.tile, R, p.N, steps, cus);
     int rows = 0, cols = 0;                                      // of the first launch (0: one launch)
-    if (full > 0 && p.N >= 256 && !paced_gemm_forced_tile()) {   // (a forced tile may take kernels of both widths of statistics)
+    if (full > 0 && p.N >= 256 && !forced) {                     // (64x64 tiles leave another width of statistics)
         if (full < R) {
             const double us = tile_us(256, full, p.N, steps, cus) + tile_us(128, R - full, p.N, steps, cus) + TWO_LAUNCHES;
             if (us < best) { best = us; rows = full; }
@@ -364,10 +368,10 @@ double dw_us(int n, int d, int steps, int cus, int* rows) {
     *rows = fill;
     return two;
 }
-int ce_dw(GemmParams p, int epilogue, size_t element, hipStream_t s) {
+int ce_dw(GemmParams p, int epilogue, size_t element, int forced, hipStream_t s) {
     const int steps = (p.K + 63) / 64, cus = paced_cu_count();
-    int rows;
-    dw_us(p.M, p.N, steps, cus, &rows);
+    int rows = 0;
+    if (!forced) dw_us(p.M, p.N, steps, cus, &rows);
     t_split.dw_rows = rows;
     if (rows) {
         GemmParams first = p;
@@ -379,7 +383,7 @@ int ce_dw(GemmParams p, int epilogue, size_t element, hipStream_t s) {
         p.A += rows;
         p.C = (char*)p.C + (size_t)rows * p.ldc * element;
     }
-    p.tile = best_tile(p.M, p.N, steps, cus);
+    p.tile = forced ? forced : best_tile(p.M, p.N, steps, cus);
     return paced_gemm_launch(p, true, true, epilogue, 1, s);
 }
 
@@ -403,9 +407,24 @@ extern "C" int paced_linear_ce_last_split(int* rows, int* cols, int* dw_rows) {
     return PACED_OK;
 }
 
+namespace {
+size_t stats_bytes(int R, int V, int width) { return round256((size_t)((V + width - 1) / width) * R * 8); }
+}  // namespace
+
+// (any d, any forced tile)
 extern "C" size_t paced_linear_ce_fwd_workspace_bytes(int R, int V) {
     if (R <= 0 || V <= 0) return 0;
-    return round256((size_t)((V + 31) / 32) * R * 8) + round256((size_t)R * 4);
+    return stats_bytes(R, V, 32) + round256((size_t)R * 4);
+}
+
+// statistics of 32 columns come from 64x64 tiles alone, which only small products take
+namespace {
+size_t fwd_workspace(int R, int V, int d, int forced) {
+    return stats_bytes(R, V, ce_tile(R, V, (d + 63) / 64, paced_cu_count(), forced) == 64 ? 32 : 64) + round256((size_t)R * 4);
+}
+}  // namespace
+extern "C" size_t paced_linear_ce_fwd_workspace_bytes_for(int R, int V, int d) {
+    return R <= 0 || V <= 0 || d <= 0 ? 0 : fwd_workspace(R, V, d, paced_gemm_forced_tile());
 }
 
 extern "C" int paced_linear_ce_fwd_ex(const void* h, int ldh, const void* w, int ldw, const long long* labels, float* loss, float* lse,
@@ -414,16 +433,17 @@ extern "C" int paced_linear_ce_fwd_ex(const void* h, int ldh, const void* w, int
     const int rc = ce_check("paced_linear_ce_fwd", h, ldh, w, ldw, labels, R, V, d);
     if (rc != PACED_OK || R == 0) return rc;
     PACED_CHECK_ARG(loss, "paced_linear_ce_fwd: null operand");
-    const size_t need = paced_linear_ce_fwd_workspace_bytes(R, V);
+    const int forced = paced_gemm_forced_tile();
+    const size_t need = fwd_workspace(R, V, d, forced);
     PACED_CHECK_ARG(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
                     "paced_linear_ce_fwd: a 16-byte aligned workspace of %zu bytes is needed, got %zu", need, workspace_bytes);
     GemmParams p = product(h, ldh, w, ldw, nullptr, 0, R, V, d, scale);
     p.ce_part = (f32x2*)workspace;
-    p.ce_target = (float*)((char*)workspace + round256((size_t)((V + 31) / 32) * R * 8));
+    p.ce_target = (float*)((char*)workspace + (need - round256((size_t)R * 4)));
     p.ce_labels = labels; p.ce_ignore = ignore_index; p.ce_vocab = V;
     p.ce_rows = R;
     p.grid_limit = grid_limit;
-    const int rg = ce_logits(p, EPI_CE_STATS, (hipStream_t)stream);
+    const int rg = ce_logits(p, EPI_CE_STATS, forced, (hipStream_t)stream);
     if (rg != PACED_OK) return rg;
     const int width = paced_gemm_stat_width();
     const int groups = (V + width - 1) / width;
@@ -494,13 +514,13 @@ extern "C" int paced_linear_ce_bwd_ex(const void* h, int ldh, const void* w, int
         p.ce_labels = labels; p.ce_lse = lse; p.ce_g = gloss; p.ce_loss = loss;
         p.ce_ignore = ignore_index; p.ce_vocab = V; p.ce_first = v0;
         p.ce_err = err; p.ce_lo = low;
-        int r = ce_logits(p, EPI_CE_GRAD, s);
+        int r = ce_logits(p, EPI_CE_GRAD, forced, s);
         if (r != PACED_OK) return r;
         if (dh) {
             p = product(P, pl.ldp, wp, ldw, slabs, d, R, d, n, scale);
             p.strideC = (long long)R * d;
             p.accumulate = v0 > 0;
-            p.tile = pl.dh_tile;
+            p.tile = forced ? forced : pl.dh_tile;
             if ((r = paced_gemm_launch(p, false, true, EPI_SLAB_F32, pl.slabs, s)) != PACED_OK) return r;
         }
         if (dw && low) {
@@ -511,7 +531,7 @@ extern "C" int paced_linear_ce_bwd_ex(const void* h, int ldh, const void* w, int
         } else if (dw) {
             p = product(P, pl.ldp, h, ldh, dw_f32 ? (void*)((float*)dw + (size_t)v0 * lddw) : (void*)((bf16*)dw + (size_t)v0 * lddw), lddw, n, d, R, scale);
             p.accumulate = 1;
-            if ((r = ce_dw(p, dw_f32 ? EPI_SLAB_F32 : EPI_BF16, dw_f32 ? 4 : 2, s)) != PACED_OK) return r;
+            if ((r = ce_dw(p, dw_f32 ? EPI_SLAB_F32 : EPI_BF16, dw_f32 ? 4 : 2, forced, s)) != PACED_OK) return r;
         }
     }
     if (dh) {

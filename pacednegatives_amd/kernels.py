@@ -572,7 +572,7 @@ def linear_ce_fwd(h, w, labels, loss, lse=None, *, ignore_index=-100, scale=1.0,
             return linear_ce_fwd(h, w, labels, loss, lse, ignore_index=ignore_index, scale=scale, grid_limit=grid_limit, workspace=workspace)
     R, V, d, ldh, ldw = _head_operands(h, w, labels)
     _flat(loss, R, F32, "loss"); _flat(lse, R, F32, "lse")
-    need = lib.paced_linear_ce_fwd_workspace_bytes(R, V)
+    need = lib.paced_linear_ce_fwd_workspace_bytes_for(R, V, d)
     ws = _workspace(workspace, need, h.device)
     _lib.check(lib.paced_linear_ce_fwd_ex(_p(h), ldh, _p(w), ldw, _p(labels), _p(loss), _p(lse), R, V, d, ignore_index, scale,
                                           -1 if grid_limit is None else int(grid_limit), _p(ws), need, _stream()), "paced_linear_ce_fwd_ex")

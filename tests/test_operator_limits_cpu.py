@@ -22,3 +22,17 @@ def test_token_counts_that_do_not_round_up_to_whole_blocks_within_an_int(lib, T)
 def test_the_largest_token_count_has_a_plan(lib):
     need = lib.paced_act8_dweight_workspace_bytes(2 ** 31 - 64, 8, 16)
     assert 0 < need <= 64 * 8 * 16 * 4
+
+
+def test_the_loss_asks_for_the_statistics_that_it_writes(lib):
+    """A float pair for a row and 64 columns, 32 only where 64x64 tiles take the product; a float a row for the label."""
+    up = lambda b: (b + 255) // 256 * 256  # noqa: E731
+    for R, V, d, width in ((8192, 50001, 1024, 64), (131072, 50001, 1024, 64), (1088, 32128, 768, 64), (16, 32128, 768, 32), (64, 32128, 768, 32), (100, 300, 64, 32)):
+        assert lib.paced_linear_ce_fwd_workspace_bytes_for(R, V, d) == up(-(-V // width) * R * 8) + up(R * 4), (R, V, d)
+        assert lib.paced_linear_ce_fwd_workspace_bytes_for(R, V, d) <= lib.paced_linear_ce_fwd_workspace_bytes(R, V)
+    assert lib.paced_linear_ce_fwd_workspace_bytes_for(0, 5, 64) == lib.paced_linear_ce_fwd_workspace_bytes_for(5, 0, 64) == lib.paced_linear_ce_fwd_workspace_bytes_for(5, 5, 0) == 0
+    lib.paced_gemm_set_tile(64)
+    try:
+        assert lib.paced_linear_ce_fwd_workspace_bytes_for(8192, 50001, 1024) == lib.paced_linear_ce_fwd_workspace_bytes(8192, 50001)
+    finally:
+        lib.paced_gemm_set_tile(0)
