@@ -11,7 +11,8 @@
 // Writing and reading are bound by memory: 139264 x 768 in 51.5 us (6.3 TB/s) and 55 us (5.9 TB/s).  The gradient is bound by the
 // matrix cores where tokens are many: 2304 x 768 from 139264 tokens in 411 to 442 us on different cards, slabs' sum
 // included (1.12 to 1.20 PFLOP/s; the bf16 products of gemm.hip reach 1.25 to 1.35 on large squares, the vendor's 1.39);
-// 512 x 2048 from 1001 tokens in 8.5 us, by latency.
+// 512 x 2048 from 1001 tokens in 8.7 us, by latency.  (A card that was idle takes some sixty launches of the large one to settle: 484 us
+// at first, 405 to 427 from then on, and 11 for the slabs' sum.)
 #include "gemm_tiles.h"
 #include <type_traits>
 

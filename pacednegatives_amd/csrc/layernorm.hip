@@ -9,8 +9,8 @@
 // over all rows that a team works on, are added over a workgroup's teams in LDS, and leave as one partial row per workgroup;
 // a second kernel adds those in a fixed order (no atomics: equal inputs give equal bits).
 // Measured, 139264 x 768 bf16 with the residual sum: forward 150 us for its four streams (5.7 TB/s; a copy of 256 MB reaches
-// 5.4), backward 168 us for its four (5.1 TB/s), column sums 4.5 us.  139264 x 767 (fp32, no residual): 166 and
-// 258 us against 147 and 226 for 768.  5001 x 1023 fp32: 10, 14 and 4 us.
+// 5.4), backward 167 to 173 us for its four (5.0 to 5.1 TB/s), column sums 4.7 us.  139264 x 767 (fp32, no residual): 166 and
+// 258 us against 147 and 226 for 768.  5001 x 1023 fp32: 11, 18 and 4.5 us.
 #include "common.h"
 
 namespace {

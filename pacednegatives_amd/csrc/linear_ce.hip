@@ -8,14 +8,15 @@
 // Backward: the vocabulary goes by in pieces.  A piece's logits are computed again and leave as P in bf16 (the MFMA operand
 // type; half a step of 2^-8 relative to each entry, as paced_cross_entropy's dlogits), which feeds the two other products.  What
 // the label's entry, the largest of a row, loses in that rounding is given back where dh is finished.  dw takes P's low part too
-// up to 64 rows, where it costs nothing (ce_dw_few_kernel is bound by writing dw); beyond, a second product of 2 R V d operations
-// would be the price, and dw is off by up to 2^-8 of each addend, whether one row or many make up an element: measured 0.0017 of
+// up to 64 rows, where it costs little (ce_dw_few_kernel; 32128 x 768, backward pass of 64 rows 47.7 us, of 65 46.6); beyond, a
+// second product of 2 R V d operations would be the price, and dw is off by up to 2^-8 of each addend, whether one row or many make up an element: measured 0.0017 of
 // its norm before its own rounding (0.0024 with it, where a result that is only rounded at the end has 0.0017).
 // dh is summed over pieces and slices of a piece in fp32 slabs with one owner per element, dw is complete with its piece:
 // nothing is added atomically, equal inputs give equal bits.
 // Matrix-core bound: 2 R V d operations forward, three times that backward.  Measured, loss and both gradients: 8192 rows x
 // 50001 entries x 1024 in 2.9 to 3.0 ms (1.14 PFLOP/s over the four products), 1088 x 32128 x 768 in 254
-// to 280 us on different cards (0.77 to 0.85 PFLOP/s: 4.25 x 125.5 tiles of 256 do not fill whole rounds of 256 compute units);
+// to 280 us on different cards (0.77 to 0.85 PFLOP/s: 4.25 x 125.5 tiles of 256 do not fill whole rounds of 256 compute units), 36
+// more where dw is added to in fp32 (148 MB more, 27 us of them);
 // the loss of 16 rows 15 us, of which the weights' 49 MB take 11.
 #include "gemm.h"
 #include "gemm_tiles.h"
@@ -131,7 +132,8 @@ __global__ void __launch_bounds__(256) ce_dh_kernel(const float* __restrict__ sl
 
 // dw (+)= scale (hi + lo)^T h for R <= 64 rows: hi, lo [R][ldp] bf16, the two parts of P.  A workgroup makes 64 entries x 256
 // features: P's parts and h come into LDS whole (LDS-DMA; rows past R read as zeros), a wave takes 16 entries, and an MFMA's 64
-// rows are all there is to contract, so the kernel is bound by writing dw.  The MFMA's sixteen columns are taken as four
+// rows are all there is to contract: writing dw bounds it (32128 x 768: 49 MB, 9 us), but P's parts and h have to arrive whole first
+// and it takes 17.4 us.  The MFMA's sixteen columns are taken as four
 // fours, eight apart, so that two products leave a lane eight consecutive features of one entry: 16-byte stores.
 constexpr int FEW = 64, FEW_P = 8192, FEW_H = 32768;
 template <bool F32>
