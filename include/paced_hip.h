@@ -278,12 +278,14 @@ int paced_cross_entropy(const float* logits, const long long* labels, float* los
  *      to in fp32 (dw_f32 = 1); each may be NULL.  The logits' gradient gloss (softmax - onehot) scale is rounded to bf16
  *      between the products, as paced_cross_entropy's dlogits are; what the label's entry loses in it is added to dh again,
  *      and up to 64 rows dw takes every entry's low part as well (2^-16 of each addend is lost).  From 65 rows on an element of dw
- *      is off by up to 2^-8 of the sum of its addends' magnitudes, be it one row's (a label of its own) or many rows'.  Sums are fp32 in a fixed order, without atomics.  An
- *      ignored row's h must be finite where dw is wanted (0 times it is added), w where dh is.
+ *      is off by up to 2^-8 of the sum of its addends' magnitudes, be it one row's (a label of its own) or many rows'.  Sums are
+ *      fp32 in a fixed order, without atomics.  An ignored row's h must be finite where dw is wanted (0 times it is added), w
+ *      where dh is.
  * Row strides are at most 2^22 elements; bwd refuses an h whose R rows span 4 GiB or more.
- * workspace, 16-byte aligned, not kept between calls, for one stream at a time: ..._workspace_bytes() bytes; fwd V R / 8 +
- * 4 R with ..._bytes_for (V R / 4 where the product is small: 64x64 tiles), ..._bytes is enough for any d; bwd the bf16 gradient of a piece of the vocabulary (256 MiB at most up to half a million rows; twice that up to 64 rows)
- * and fp32 partial sums of dh (4 R d bytes each, 64 at most, the fewer the more rows). */
+ * workspace, 16-byte aligned, not kept between calls, for one stream at a time: ..._workspace_bytes() bytes.  fwd: V R / 8 + 4 R by
+ * ..._bytes_for (V R / 4 + 4 R where the product is small: 64x64 tiles); ..._bytes is enough for any d.  bwd: the bf16 gradient of a
+ * piece of the vocabulary (256 MiB at most up to half a million rows; twice that up to 64 rows) and fp32 partial sums of dh
+ * (4 R d bytes each, 64 at most, the fewer the more rows). */
 size_t paced_linear_ce_fwd_workspace_bytes(int R, int V);
 size_t paced_linear_ce_fwd_workspace_bytes_for(int R, int V, int d);
 int paced_linear_ce_fwd(const void* h, int ldh, const void* w, int ldw, const long long* labels, float* loss, float* lse,

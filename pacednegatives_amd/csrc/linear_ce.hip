@@ -9,8 +9,9 @@
 // type; half a step of 2^-8 relative to each entry, as paced_cross_entropy's dlogits), which feeds the two other products.  What
 // the label's entry, the largest of a row, loses in that rounding is given back where dh is finished.  dw takes P's low part too
 // up to 64 rows, where it costs little (ce_dw_few_kernel; 32128 x 768, backward pass of 64 rows 47.7 us, of 65 46.6); beyond, a
-// second product of 2 R V d operations would be the price, and dw is off by up to 2^-8 of each addend, whether one row or many make up an element: measured 0.0017 of
-// its norm before its own rounding (0.0024 with it, where a result that is only rounded at the end has 0.0017).
+// second product of 2 R V d operations would be the price, and dw is off by up to 2^-8 of each addend, whether one row or many
+// make up an element: measured 0.0017 of its norm before its own rounding (0.0024 with it, where a result that is only rounded at
+// the end has 0.0017).
 // dh is summed over pieces and slices of a piece in fp32 slabs with one owner per element, dw is complete with its piece:
 // nothing is added atomically, equal inputs give equal bits.
 // Matrix-core bound: 2 R V d operations forward, three times that backward.  Measured, loss and both gradients: 8192 rows x
@@ -505,6 +506,7 @@ extern "C" int paced_linear_ce_bwd_ex(const void* h, int ldh, const void* w, int
     }
     bf16* P = (bf16*)workspace;
     const size_t part = round256((size_t)R * pl.ldp * 2);
+    t_split = Split{0, 0, 0};
     const int forced = paced_gemm_forced_tile();                  // (the low part is written by the 64x64 tiles' epilogue)
     bf16* low = dw && R <= FEW && (forced == 0 || forced == 64) ? (bf16*)((char*)workspace + part) : nullptr;
     float* err = (float*)((char*)workspace + (R <= FEW ? 2 : 1) * part);

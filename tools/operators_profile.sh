@@ -1,6 +1,6 @@
 #!/bin/bash
 # Kernel times and counters of the operators' cases: writes operators_kernel_times.txt and operators_counters.txt into $1
-# (tools/operators_tables.py makes them from rocprofv3's files).  Run on the GPU machine, from the repository's root, on a built tree.
+# (tools/operators_tables.py makes them from rocprofv3's files).  Run with a GPU, from the repository's root, on a built tree.
 set -e
 out=${1:?usage: operators_profile.sh DIRECTORY}
 here=$PWD
